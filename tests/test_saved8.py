@@ -1,0 +1,352 @@
+"""Activations kept for backward in 8 bits (checkpoint8, Saved8 operands of einshard).
+
+The oracle quantises in 64 bits.  Codes must be equal, not close: every scaling
+is by a power of two.  Products are compared within the roundings of their
+output (half a step of the type), of the 16-bit intermediates (half a step of
+each factor, carried through the product of absolute values) and of the 32-bit
+accumulation (2^-23 a term at most, which the same product bounds).
+"""
+
+import pytest
+import torch
+import torch.distributed as dist
+
+import torch_einshard_b200 as es
+from torch_einshard_b200.models.tp_mlp import TPMLP
+from torch_einshard_b200.models.transformer import TPTransformer, TransformerConfig
+
+cuda = pytest.param("cuda", marks=pytest.mark.gpu)
+DEVICES = ["cpu", cuda]
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def oracle(x):
+    """(restored values in fp64, half steps) of x by the definition, block by block."""
+    x = x.detach().double().cpu()
+    flat = x.reshape(x.shape[:-1].numel(), x.shape[-1])
+    out, half = torch.zeros_like(flat), torch.zeros_like(flat)
+    for start in range(0, flat.shape[1], 32):
+        block = flat[:, start:start + 32]
+        amax = block.abs().amax(1)
+        bad = ~torch.isfinite(amax)
+        amax = torch.where(bad, 1.0, amax)
+        e = torch.floor(torch.log2(amax.clamp(min=2.0 ** -1000))) - 6  # exact in 64 bits away from powers of two
+        e = torch.where(torch.exp2(e + 7) <= amax, e + 1, e)
+        e = torch.where(torch.exp2(e + 6) > amax, e - 1, e).clamp(min=-126)
+        e = torch.where(torch.round(amax / torch.exp2(e)) > 127, e + 1, e)
+        step = torch.exp2(e)[:, None]
+        q = torch.round(block / step) * step
+        out[:, start:start + 32] = torch.where(bad[:, None], float("nan"), q)
+        half[:, start:start + 32] = step / 2
+    return out.reshape(x.shape), half.reshape(x.shape)
+
+
+def check_restore(x):
+    got = es.checkpoint8(x).restore()
+    assert got.dtype == x.dtype and got.shape == x.shape and not got.requires_grad
+    limit = torch.finfo(x.dtype).max
+    want = oracle(x)[0]
+    assert torch.equal(torch.isnan(got.cpu()), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(got.cpu().double()), torch.nan_to_num(want.clamp(-limit, limit)))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(1,), (7,), (32,), (33,), (1, 1), (3, 31), (2, 3, 64), (5, 40), (4, 1000), (2, 1001),
+                                   (1, 8200), (300, 96), (0, 64), (5, 0)])
+def test_restore_is_the_definition(device, dtype, shape):
+    gen = torch.Generator().manual_seed(3)
+    x = torch.randn(shape, generator=gen) * torch.exp(3 * torch.randn(shape, generator=gen))
+    check_restore(x.to(dtype).to(device))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [32, 50, 96])
+def test_special_values(device, dtype, width):
+    info = torch.finfo(dtype)
+    x = torch.zeros(12, width, dtype=dtype)
+    x[1, 3] = info.max
+    x[2] = info.max
+    x[3, :] = -info.max
+    x[4, 0] = float("inf")
+    x[5, width - 1] = float("nan")
+    x[6, 1] = -float("inf")
+    x[7] = info.smallest_normal
+    x[8, 2] = info.smallest_normal * info.eps  # the smallest subnormal
+    x[9, :2] = torch.tensor([1.0, 0.5])  # a tie: 63.5 steps would round either way under a scale of max / 127
+    x[10] = 127.5 / 64
+    x[11, 0] = -0.0
+    check_restore(x.to(device))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_error_is_half_a_step(device):
+    x = torch.randn(64, 257, generator=torch.Generator().manual_seed(1)).to(device)
+    s = es.checkpoint8(x)
+    _, half = oracle(x)
+    assert ((s.restore() - x).abs().cpu().double() <= half).all()
+    assert s.nbytes == 64 * 257 + 64 * 9
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_views_and_alignments(device):
+    base = torch.randn(6, 130, 70, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(device)
+    check_restore(base.transpose(1, 2))
+    check_restore(base[:, 1:, 3:67])
+    check_restore(base.flatten()[1:1 + 64 * 64].view(64, 64))
+    check_restore(base[:, :, :1].expand(6, 130, 40))
+
+
+def _case(device, dtype, b, s, c, h, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    def make(*shape, scale=1.0):
+        return (torch.randn(shape, generator=gen) * scale).to(dtype).to(device)
+    return make(b, s, c), make(h, c, scale=c ** -0.5), make(c, h, scale=h ** -0.5), make(b, s, c), make(b, s, h)
+
+
+def close(got, want, slack, dtype, terms):
+    """|got - want| within the output's rounding, `terms` half steps of 16-bit factors and the accumulation."""
+    bound = half_step(dtype) * want.abs() + (terms * half_step(dtype) + 2.0 ** -20) * 1.01 * slack
+    bound = bound + torch.finfo(dtype).smallest_normal
+    err = (got.detach().double().cpu() - want).abs()
+    assert (err <= bound).all(), float((err / bound).max())
+
+
+SHAPES = [(1, 1, 32, 8), (2, 5, 40, 48), (3, 33, 100, 72), (1, 7, 33, 31), (2, 130, 256, 520)]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("transposed", [False, True])
+def test_linear(device, dtype, shape, transposed):
+    x, w, _, _, dz = _case(device, dtype, *shape)
+    if transposed:
+        w = w.t().contiguous()
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    s = es.checkpoint8(x)
+    z = es.einshard("b s c, c h -> b s h" if transposed else "b s c, h c -> b s h", s, w)
+    dx, dw = torch.autograd.grad(z, (x, w), dz)
+    xd, zd = x.detach().double().cpu(), dz.double().cpu()
+    wd = (w.t() if transposed else w).detach().double().cpu()
+    kept = s.restore().double().cpu()
+    close(z, xd @ wd.t(), xd.abs() @ wd.abs().t(), dtype, 0)
+    close(dx, zd @ wd, zd.abs() @ wd.abs(), dtype, 0)
+    want = torch.einsum("bsh,bsc->hc", zd, kept)
+    slack = torch.einsum("bsh,bsc->hc", zd.abs(), kept.abs())
+    close(dw.t() if transposed else dw, want, slack, dtype, 0)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", SHAPES + [pytest.param((2, 2500, 128, 2048), marks=pytest.mark.gpu)])
+def test_mlp(device, dtype, shape):
+    if device == "cpu" and shape[1] > 1000:
+        pytest.skip("the wide kernel's shape")
+    x, w1, w2, dy, _ = _case(device, dtype, *shape, seed=5)
+    for t in (x, w1, w2):
+        t.requires_grad_(True)
+    s = es.checkpoint8(x)
+    a = es.einshard("b s c, h c -> b s h", s, w1, activation="silu")
+    assert isinstance(a, es.Saved8) and a.value.dtype == dtype
+    y = es.einshard("b s h, c h -> b s c", a, w2)
+    dx, dw1, dw2 = torch.autograd.grad(y, (x, w1, w2), dy)
+
+    xd, w1d, w2d, dyd = (t.detach().double().cpu() for t in (x, w1, w2, dy))
+    pre = xd @ w1d.t()
+    codes = a.codes.cpu().double().view(*pre.shape)
+    step = torch.exp2(a.exps.cpu().double().repeat_interleave(32, 1)[:, :pre.shape[-1]] - 127).view(*pre.shape)
+    kept = codes * step
+    # the pre-activation is kept from the 32-bit product: half a step off, and the accumulation
+    assert ((kept - pre).abs() <= step / 2 + 2.0 ** -20 * (xd.abs() @ w1d.abs().t())).all()
+    act = pre * torch.sigmoid(pre)
+    # the sigmoid's own error is below 2^-20 of the value; |d silu| <= 1.1 |d pre|
+    close(a.value, act, act.abs() + xd.abs() @ w1d.abs().t(), dtype, 0)
+    close(y, a.value.detach().double().cpu() @ w2d.t(), act.abs() @ w2d.abs().t() * 1.1 + 1e-6, dtype, 0)
+    sig = torch.sigmoid(kept)
+    akept = kept * sig
+    assert torch.allclose(a.restore().double().cpu(), akept, rtol=half_step(dtype) + 2.0 ** -20, atol=1e-7)
+    close(dw2, torch.einsum("bsc,bsh->ch", dyd, akept), torch.einsum("bsc,bsh->ch", dyd.abs(), akept.abs()), dtype, 1)
+    da, da_abs = dyd @ w2d, dyd.abs() @ w2d.abs()
+    slope = sig * (1 + kept * (1 - sig))
+    dh = da * slope
+    # da is rounded to the type, its product with silu' once more; the accumulation's part goes by da_abs
+    dh_err = dh.abs() * 2.01 + da_abs * slope.abs() * 2.0 ** -20 / half_step(dtype) + 1e-9
+    close(dx, dh @ w1d, (dh_err + dh.abs() * 2.0 ** -6) @ w1d.abs(), dtype, 1)
+    xk = s.restore().double().cpu()
+    close(dw1, torch.einsum("bsh,bsc->hc", dh, xk), torch.einsum("bsh,bsc->hc", dh_err + dh.abs() * 2.0 ** -6, xk.abs()),
+          dtype, 1)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_gradients_against_differences(device):
+    """Where x is on the grid of its blocks, x^ = x and gradients are those of the product: central differences of
+    a bilinear form have no error but rounding (64 bits on the CPU, whole numbers on the GPU)."""
+    dtype = torch.float64 if device == "cpu" else torch.float32
+    gen = torch.Generator().manual_seed(4)
+    x = torch.randint(-60, 61, (2, 3, 8), generator=gen).to(dtype).to(device).requires_grad_(True)
+    w = torch.randint(-4, 5, (5, 8), generator=gen).to(dtype).to(device).requires_grad_(True)
+    g = torch.randint(-4, 5, (2, 3, 5), generator=gen).to(dtype).to(device)
+
+    def f(xv, wv):
+        return (es.einshard("b s c, h c -> b s h", es.checkpoint8(xv), wv) * g).sum()
+
+    dx, dw = torch.autograd.grad(f(x, w), (x, w))
+    for t, grad, which in ((x, dx, 0), (w, dw, 1)):
+        flat = t.detach().flatten()
+        for i in range(0, flat.numel(), 3):
+            hi, lo = flat.clone(), flat.clone()
+            hi[i] += 1
+            lo[i] -= 1
+            args = [[x.detach(), w.detach()] for _ in range(2)]
+            args[0][which], args[1][which] = hi.view(t.shape), lo.view(t.shape)
+            assert float(grad.flatten()[i]) == float((f(*args[0]) - f(*args[1])) / 2)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_axis_orders_and_ellipsis(device):
+    x, w, _, _, _ = _case(device, torch.float32, 2, 6, 40, 48, seed=7)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    s = es.checkpoint8(x)
+    kept = s.restore().double().cpu()
+    wd = w.detach().double().cpu()
+    for formula, fn, batched in [
+        ("b s c, h c -> h b s", lambda a, b: torch.einsum("bsc,hc->hbs", a, b), False),
+        ("b s c, h c -> s h b", lambda a, b: torch.einsum("bsc,hc->shb", a, b), False),
+        ("... c, h c -> ... h", lambda a, b: torch.einsum("bsc,hc->bsh", a, b), False),
+    ]:
+        z = es.einshard(formula, s, w)
+        dz = torch.randn(z.shape, generator=torch.Generator().manual_seed(1)).to(device)
+        (dw,) = torch.autograd.grad(z, w, dz)
+        wr = wd.clone().requires_grad_(True)
+        (want,) = torch.autograd.grad(fn(kept, wr), wr, dz.double().cpu())
+        assert torch.allclose(dw.double().cpu(), want, rtol=1e-5, atol=1e-5)
+        a = es.einshard(formula, s, w, activation="silu")
+        assert a.restore().shape == a.value.shape
+        assert torch.allclose(a.restore(), a.value, atol=0.05)
+        (dw,) = torch.autograd.grad(a.value, w, dz)
+        pre = fn(x.detach().double().cpu(), wr)
+        (want,) = torch.autograd.grad(torch.nn.functional.silu(pre), wr, dz.double().cpu())
+        assert (dw.double().cpu() - want).norm() <= 0.02 * want.norm()  # 8-bit x and pre-activation: steps of 1/64
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["b s h", "h b s", "s h b"])
+def test_activation_layouts_16_bit(order):
+    x, w, _, _, _ = _case("cuda", torch.bfloat16, 2, 6, 40, 48, seed=8)
+    w.requires_grad_(True)
+    a = es.einshard(f"b s c, h c -> {order}", es.checkpoint8(x), w, activation="silu")
+    pre = torch.einsum(f"bsc,hc->{order.replace(' ', '')}", x.double(), w.detach().double())
+    want = pre * torch.sigmoid(pre)
+    assert ((a.value.double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-5).all()
+    dz = torch.randn_like(a.value)
+    (dw,) = torch.autograd.grad(a.value, w, dz)
+    sig = torch.sigmoid(pre)
+    dh = dz.double() * sig * (1 + pre * (1 - sig))
+    want = torch.einsum(f"{order.replace(' ', '')},bsc->hc", dh, x.double())
+    assert (dw.double() - want).norm() <= 0.02 * want.norm()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_refusals(device):
+    x = torch.randn(2, 3, 8, device=device)
+    w = torch.randn(5, 8, device=device)
+    s = es.checkpoint8(x)
+    with pytest.raises(TypeError):
+        es.checkpoint8(s)
+    with pytest.raises(TypeError):
+        es.checkpoint8([1.0])
+    with pytest.raises(TypeError):
+        es.checkpoint8(torch.ones(4, dtype=torch.int64, device=device))
+    with pytest.raises(TypeError):
+        es.checkpoint8(torch.ones(4, dtype=torch.complex64, device=device))
+    with pytest.raises(ValueError):
+        es.checkpoint8(torch.tensor(1.0, device=device))
+    with pytest.raises(TypeError, match="goes first"):
+        es.einshard("h c, b s c -> b s h", w, s)
+    with pytest.raises(TypeError, match="second operand"):
+        es.einshard("b s c -> b c s", s)
+    with pytest.raises(ValueError, match="alike"):
+        es.einshard("b s c, h c -> b s h", s, w.double())
+    with pytest.raises(ValueError, match="activation"):
+        es.einshard("b s c, h c -> b s h", s, w, activation="gelu")
+    with pytest.raises(NotImplementedError):
+        es.einshard("b s c, h -> b h", s, w[:, 0])  # s and c summed out
+    with pytest.raises(NotImplementedError):
+        es.einshard("b s (c k), h c k -> b s h", s, torch.randn(5, 4, 2, device=device), sizes={"k": 2})
+    with pytest.raises(RuntimeError):  # no second derivative through rounded codes
+        xg = x.clone().requires_grad_(True)
+        z = es.einshard("b s c, h c -> b s h", es.checkpoint8(xg), w).square().sum()
+        (dx,) = torch.autograd.grad(z, xg, create_graph=True)
+        torch.autograd.grad(dx.sum(), xg)
+
+
+@pytest.mark.gpu
+def test_capture_and_replay():
+    x, w1, w2, dy, _ = _case("cuda", torch.bfloat16, 2, 64, 64, 96, seed=9)
+
+    def step():
+        s = es.checkpoint8(x)
+        a = es.einshard("b s c, h c -> b s h", s, w1, activation="silu")
+        return es.einshard("b s h, c h -> b s c", a, w2), a.restore()
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y, kept = step()
+    x.copy_(torch.randn_like(x))
+    graph.replay()
+    want_y, want_kept = step()
+    assert torch.equal(y, want_y) and torch.equal(kept, want_kept)
+
+
+@pytest.fixture
+def one_rank_mesh(request):
+    from torch.distributed.device_mesh import init_device_mesh
+    device = request.param
+    if not dist.is_initialized():
+        dist.init_process_group("gloo" if device == "cpu" else "nccl", init_method="tcp://127.0.0.1:0", rank=0,
+                                world_size=1)
+    yield device, init_device_mesh(device, (1,), mesh_dim_names=("tp",))
+    dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("one_rank_mesh", DEVICES, indirect=True)
+def test_models_keep_their_outputs_and_gradients(one_rank_mesh):
+    """The forward pass does not change; gradients are those of activations within half a step."""
+    device, mesh = one_rank_mesh
+    dtype = torch.float32 if device == "cpu" else torch.bfloat16
+    models = [TPMLP(64, 256, mesh, dtype=dtype, device=device, std=0.1, checkpoint=c) for c in (None, "int8")]
+    x = torch.randn(2, 32, 64, generator=torch.Generator().manual_seed(0)).to(device, dtype)
+    outs = [m(x) for m in models]
+    assert (outs[0] - outs[1]).abs().max() <= 4 * half_step(dtype) * outs[0].abs().max()
+    for m, y in zip(models, outs):
+        y.float().square().sum().backward()
+    for p, q in zip(models[0].parameters(), models[1].parameters()):
+        assert (p.grad.float() - q.grad.float()).norm() <= 0.03 * p.grad.float().norm()
+
+    cfg = TransformerConfig(layers=2, d=64, heads=4, mlp=128, vocab=97, seq=16, dtype=dtype)
+    tokens = torch.randint(0, 97, (2, 16), generator=torch.Generator().manual_seed(1)).to(device)
+    losses, grads = [], []
+    for mode in (False, "int8"):
+        model = TPTransformer(cfg, mesh, device=device, checkpoint=mode)
+        loss = model(tokens, tokens.roll(-1, 1))
+        loss.backward()
+        losses.append(float(loss))
+        grads.append([p.grad.float() for p in model.parameters()])
+    assert abs(losses[0] - losses[1]) <= (1e-5 if device == "cpu" else 0.02) * abs(losses[0])
+    for p, q in zip(*grads):
+        assert (p - q).norm() <= 0.05 * p.norm() + 1e-6
+    with pytest.raises(ValueError):
+        TPMLP(64, 256, mesh, dtype=dtype, device=device, checkpoint="int4")

@@ -16,6 +16,7 @@ from .ops.einsum import einsum
 from .ops.fft import einfft
 from .ops.halo import einhalo, einwindow
 from .ops.roll import einroll
+from .ops.saved8 import Saved8, checkpoint8
 from .parallel.executor import distributed_1d
 from .parallel.mesh import CompoundDeviceMesh, wrap_mesh
 from .parallel.collectives import compute_split_shapes, compute_split_shapes_for_factors, init_process_group, resolve_split_shapes

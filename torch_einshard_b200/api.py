@@ -15,6 +15,7 @@ from .notation.parser import parse_sharding
 from .notation.spec import Axes, AxisGroup, EllipsisAxis, TensorSpec
 from .ops import gemm as _gemm
 from .ops.einsum import einsum
+from .ops.saved8 import Saved8, silu_saved
 from .parallel.executor import distributed_1d
 from .plan.policy import resolve_plan_policy
 from .plan.state import TensorState
@@ -123,10 +124,18 @@ def _run(shard, xs, mesh, shapes, sizes, policy, activation=None):
     if activation is not None:
         if getattr(shard[2], "partials", ()):
             raise ValueError("activation needs a complete output (no // partial sums)")
-        out = _gemm.silu(out) if activation == "silu" else None
-        if out is None:
+        if activation != "silu":
             raise ValueError(f"unsupported activation {activation!r} (supported: 'silu')")
+        out = silu_saved(out) if isinstance(xs[0], Saved8) else _gemm.silu(out)
     return out
+
+
+def _check_saved(shard, xs):
+    """A Saved8 operand is the first of two."""
+    if any(isinstance(x, Saved8) for x in xs[1:]):
+        raise TypeError("a Saved8 operand goes first")
+    if xs and isinstance(xs[0], Saved8) and shard[1] is None:
+        raise TypeError("a Saved8 operand needs a second operand to be contracted with")
 
 
 def einshard(shard, *xs, mesh=None, shapes=None, sizes=None, families=None, optimize=None, policy=None,
@@ -138,13 +147,19 @@ def einshard(shard, *xs, mesh=None, shapes=None, sizes=None, families=None, opti
     in the GEMM's epilogue (the wide kernel writes the pre-activation, kept for
     backward, and the activation from one pass over its accumulator); for a
     distributed one it follows the plan's last step.  An output with ``//``
-    partial sums cannot take one."""
+    partial sums cannot take one.
+
+    The first operand of a contraction may be a :class:`Saved8`
+    (:func:`checkpoint8`): backward then reads it from its 8-bit codes.  With
+    ``activation`` the result is a ``Saved8`` as well."""
     policy = resolve_plan_policy(optimize=optimize, policy=policy)
     shard, sizes = cached_expand_axis_families(shard, sizes, families)
     shard = parse_sharding(shard)
     if activation is not None and getattr(shard[2], "partials", ()):
         raise ValueError("activation needs a complete output (no // partial sums)")
-    registrations = _prepare(_operand_registrations(shard, xs, mesh))
+    _check_saved(shard, xs)
+    plain = [x.value if isinstance(x, Saved8) else x for x in xs]
+    registrations = _prepare(_operand_registrations(shard, plain, mesh))
     out = _run(shard, xs, mesh, shapes, sizes, policy, activation)
     _commit(registrations)
     return out

@@ -11,6 +11,7 @@
 #include "fft.h"
 #include "gemm.h"
 #include "act.h"
+#include "bindings_train.h"
 #include "gemm_ar.h"
 #include "gemm_nvls.h"
 #include "nvls.h"
@@ -1124,5 +1125,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("set_gemm_sleep_ns", [](int64_t v) { g_sleep_ns = static_cast<int>(v); }, "wide-kernel epilogue back-off ns");
   m.def("set_tma_l2_promotion", [](int64_t v) { es::tma_l2_promotion() = static_cast<int>(v); },
         "L2 promotion of TMA loads: 0 none, 1 64B, 2 128B, 3 256B (tuning)");
+  es::bind_training_ops(m, g_launches);
   m.def("launch_count", []() { return g_launches.load(); }, "native kernel launches so far");
 }

@@ -19,14 +19,20 @@ the reference ships no model class.
 import torch
 
 from ..api import einshard
+from ..ops.saved8 import checkpoint8
 
 __all__ = ["TPMLP", "tp_mlp_flops"]
 
 
 class TPMLP(torch.nn.Module):
     def __init__(self, c, h, mesh, *, tp_dim="tp", dtype=torch.bfloat16, device=None, std=0.02, seed=0,
-                 single_formula=True):
+                 single_formula=True, checkpoint=None):
         super().__init__()
+        # checkpoint="int8": the input and the pre-activation are kept for backward in 8 bits
+        # (ops/saved8.py); the activation is rebuilt from the pre-activation's codes
+        if checkpoint not in (None, False, "int8"):
+            raise ValueError(f"checkpoint must be None or 'int8', not {checkpoint!r}")
+        self.checkpoint = checkpoint
         # single_formula: write the row-parallel step as one formula
         # ("b n h/tp, c h/tp -> b n c"), whose plan is the same local contraction
         # followed by the same all-reduce as the two-call chain below, so the
@@ -47,6 +53,8 @@ class TPMLP(torch.nn.Module):
 
     def forward(self, x):
         t = self.tp_dim
+        if self.checkpoint == "int8" and torch.is_grad_enabled():
+            x = checkpoint8(x)
         a = einshard(f"b n c, h/{t} c -> b n h/{t}", x, self.w1, mesh=self.mesh, activation="silu")
         if self.single_formula:
             return einshard(f"b n h/{t}, c h/{t} -> b n c", a, self.w2, mesh=self.mesh)

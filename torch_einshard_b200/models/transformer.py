@@ -28,6 +28,7 @@ import torch.utils.checkpoint
 import torch.nn.functional as F
 
 from ..api import einshard
+from ..ops.saved8 import checkpoint8
 from ..params import register_parameter_layout
 
 __all__ = ["TransformerConfig", "TPTransformer", "transformer_flops_per_token"]
@@ -49,8 +50,9 @@ def transformer_flops_per_token(cfg, *, backward=True):
 
 
 class _Block(torch.nn.Module):
-    def __init__(self, cfg, tp, tp_rank, gen, device):
+    def __init__(self, cfg, tp, tp_rank, gen, device, int8=False):
         super().__init__()
+        self.int8 = int8
         d, hd = cfg.d, cfg.d // cfg.heads
         self.local_heads = cfg.heads // tp
         self.head_dim = hd
@@ -77,8 +79,16 @@ class _Block(torch.nn.Module):
         assert e == self.wq.shape[0] and f == self.w_up.shape[0]
 
     def forward(self, x, mesh):
-        b, s, _ = x.shape
-        h = einshard("b s d -> b s d // tp", self.ln1(x), mesh=mesh)
+        x = x + self.attention(self.ln1(x), mesh)
+        return x + self.mlp(self.ln2(x), mesh)
+
+    def _keep(self, t):
+        """The operand of the next contractions: kept for backward in 8 bits when the model says so."""
+        return checkpoint8(t) if self.int8 and torch.is_grad_enabled() else t
+
+    def attention(self, h, mesh):
+        b, s, _ = h.shape
+        h = self._keep(einshard("b s d -> b s d // tp", h, mesh=mesh))
         q = einshard("b s d, e/tp d -> b s e/tp", h, self.wq, mesh=mesh)
         k = einshard("b s d, e/tp d -> b s e/tp", h, self.wk, mesh=mesh)
         v = einshard("b s d, e/tp d -> b s e/tp", h, self.wv, mesh=mesh)
@@ -86,17 +96,21 @@ class _Block(torch.nn.Module):
         q, k, v = (t.reshape(shape).transpose(1, 2) for t in (q, k, v))
         attn = F.scaled_dot_product_attention(q, k, v, is_causal=True)
         attn = attn.transpose(1, 2).reshape(b, s, self.local_heads * self.head_dim)
-        x = x + einshard("b s e/tp, d e/tp -> b s d", attn, self.wo, mesh=mesh)
-        h = einshard("b s d -> b s d // tp", self.ln2(x), mesh=mesh)
+        return einshard("b s e/tp, d e/tp -> b s d", self._keep(attn), self.wo, mesh=mesh)
+
+    def mlp(self, h, mesh):
+        h = self._keep(einshard("b s d -> b s d // tp", h, mesh=mesh))
         act = einshard("b s d, f/tp d -> b s f/tp", h, self.w_up, mesh=mesh, activation="silu")
-        return x + einshard("b s f/tp, d f/tp -> b s d", act, self.w_dn, mesh=mesh)
+        return einshard("b s f/tp, d f/tp -> b s d", act, self.w_dn, mesh=mesh)
 
 
 class TPTransformer(torch.nn.Module):
     def __init__(self, cfg, mesh, *, tp_dim="tp", device=None, seed=0, checkpoint=False):
         super().__init__()
         self.cfg, self.mesh = cfg, mesh
-        self.checkpoint = checkpoint  # recompute each block in backward (activation checkpointing)
+        # "int8": keep the operands of the blocks' contractions and the MLP's pre-activation in 8 bits
+        # (ops/saved8.py); any other true value: recompute each block in backward (activation checkpointing)
+        self.checkpoint = checkpoint
         tp_mesh = mesh[tp_dim]
         tp = tp_mesh.size()
         tp_rank = tp_mesh.get_local_rank()
@@ -105,7 +119,8 @@ class TPTransformer(torch.nn.Module):
         gen = torch.Generator(device="cpu").manual_seed(seed)
         self.embed = torch.nn.Parameter(
             torch.empty(cfg.vocab, cfg.d).normal_(0.0, 0.02, generator=gen).to(device=device, dtype=cfg.dtype))
-        self.blocks = torch.nn.ModuleList(_Block(cfg, tp, tp_rank, gen, device) for _ in range(cfg.layers))
+        self.blocks = torch.nn.ModuleList(
+            _Block(cfg, tp, tp_rank, gen, device, checkpoint == "int8") for _ in range(cfg.layers))
         self.ln_f = torch.nn.LayerNorm(cfg.d, device=device, dtype=cfg.dtype)
         self._register_metadata(mesh)
 
@@ -126,7 +141,7 @@ class TPTransformer(torch.nn.Module):
     def forward(self, tokens, targets=None):
         x = F.embedding(tokens, self.embed)
         for block in self.blocks:
-            if self.checkpoint and torch.is_grad_enabled():
+            if self.checkpoint and self.checkpoint != "int8" and torch.is_grad_enabled():
                 x = torch.utils.checkpoint.checkpoint(block, x, self.mesh, use_reentrant=False)
             else:
                 x = block(x, self.mesh)

@@ -16,6 +16,7 @@ import string
 
 from ..notation.spec import AxisGroup, EllipsisAxis
 from .contraction import contract
+from .saved8 import Saved8, contract_saved
 
 __all__ = ["einsum", "expand_groups", "pack_groups"]
 
@@ -121,8 +122,12 @@ def equation_for(shard, name_only=False):
 
 def einsum(shard, *xs, name_only=False, sizes=None, activation=None):
     """Run the local contraction described by ``shard`` on ``xs``, optionally
-    followed by an elementwise ``activation`` (fused into the GEMM epilogue)."""
+    followed by an elementwise ``activation`` (fused into the GEMM epilogue).
+    The first operand may be a :class:`.saved8.Saved8`."""
     binary = shard[1] is not None
+    saved = isinstance(xs[0], Saved8)
+    if saved and any(_has_groups(spec) for spec in (shard[0], shard[2])):
+        raise NotImplementedError("Factored axes are not supported with a Saved8 operand")
     if not name_only:
         assert not getattr(shard[0], "partials", ()), "Local einsum does not support partial inputs"
         if binary:
@@ -135,5 +140,7 @@ def einsum(shard, *xs, name_only=False, sizes=None, activation=None):
     if binary:
         lhs += "," + _letters(shard[1], table, name_only)
     rhs = _letters(shard[2], table, name_only, allow_missing=False)
-    output = contract(f"{lhs}->{rhs}", *xs, activation=activation)
+    output = (contract_saved if saved else contract)(f"{lhs}->{rhs}", *xs, activation=activation)
+    if saved:
+        return output
     return output if name_only else pack_groups(output, shard[2])

@@ -28,6 +28,7 @@ import torch.distributed as dist
 
 from ..notation.spec import Axes, Axis, EllipsisAxis, TensorSpec
 from ..ops.einsum import einsum
+from ..ops.saved8 import Saved8
 from ..plan.cost import TensorRuntimeInfo, rank_alternatives
 from ..plan.policy import resolve_plan_policy
 from ..plan.state import PlanStep
@@ -131,7 +132,10 @@ class BinaryExecutor:
         self.plan = ExecutionPlan()
         self.policy = resolve_plan_policy(policy=policy)
         self.mesh, self.shapes = mesh, shapes
-        self.x0, self.y0 = x, y
+        # an operand kept for backward in 8 bits: its value goes through the plan's steps, and its codes stay its
+        # codes while those steps leave the value as it is
+        self.saved = x if isinstance(x, Saved8) else None
+        self.x0, self.y0 = x if self.saved is None else x.value, y
         self.spec0, self.spec1, self.spec_out = shard
         self.axes0 = _no_ellipsis(_axes(self.spec0))
         self.axes1 = _no_ellipsis(_axes(self.spec1))
@@ -337,6 +341,10 @@ class BinaryExecutor:
                                        tensor, self.group(dim), step_args=(dim,))
         return tensor, TensorSpec(axes, _partials(spec))
 
+    def _kept(self, steps):
+        """Whether ``steps`` hand the operand on unchanged (only its gradient differs)."""
+        return all(s.name == "identity_forward_allreduce_backward" for s in self.runtime_input_steps(steps))
+
     def _localize(self, axis):
         if self.scatter_by_dim.get(axis.shard_dim) == axis:
             axis = Axis(axis.name)
@@ -356,7 +364,7 @@ class BinaryExecutor:
                 if candidate.name == "alltoall_repartition":
                     plan.consider(candidate, status="rejected", reason="runtime split-shape validation failed")
 
-        fuse = _binary_fusion(self)
+        fuse = _binary_fusion(self) if self.saved is None else None
         deferred0 = [] if fuse is not None and fuse.kind == "dgrad_allreduce" and fuse.operand == 0 else None
         deferred1 = [] if fuse is not None and fuse.kind == "dgrad_allreduce" and fuse.operand == 1 else None
         if fuse is not None and fuse.kind == "allgather_gemm":
@@ -399,6 +407,8 @@ class BinaryExecutor:
                 x = M.identity_forward_allreduce_backward(x, deferred0[0])
             if deferred1:
                 y = M.identity_forward_allreduce_backward(y, deferred1[0])
+            if self.saved is not None and self._kept(tp.input0_steps):
+                x = self.saved.with_value(x)
             z = einsum((spec0, spec1, local_out), x, y)
 
         current = local_out_axes
