@@ -1,11 +1,12 @@
 // Torch bindings of the training-step operators around the contractions:
-// activations kept in 8 bits (quant8.h).
+// activations kept in 8 bits (quant8.h), norms with gate and residual (norm.h).
 #include "bindings_train.h"
 
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include "gemm.h"
+#include "norm.h"
 #include "quant8.h"
 
 namespace es {
@@ -95,12 +96,154 @@ at::Tensor restore8_op(const at::Tensor& codes, const at::Tensor& exps, const c1
   return out;
 }
 
+// ------------------------------------------------------------------ norms
+
+using Opt = c10::optional<at::Tensor>;
+
+void norm_param(NormParam& q, const Opt& t, const at::Tensor& x, int64_t count, const char* name) {
+  if (!t.has_value()) return;
+  TORCH_CHECK(t->device() == x.device() && t->is_contiguous() && t->numel() == count &&
+                  (t->scalar_type() == x.scalar_type() || t->scalar_type() == at::kFloat),
+              "einshard norm: ", name, " of ", count, " elements, contiguous, of the stream's type or fp32");
+  q.p = t->data_ptr();
+  q.f32 = t->scalar_type() == at::kFloat ? 1 : 0;
+}
+
+NormArgs norm_args(const at::Tensor& x, const Opt& y, const Opt& w, const Opt& b, const Opt& pw, const Opt& pb,
+                   const Opt& gate, int64_t gate_inner, int64_t gate_count, bool post, bool center, double scale,
+                   double eps) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2 && x.size(1) > 0 && (x.stride(1) == 1 || x.size(1) == 1),
+              "einshard norm: [rows, d] CUDA tensor");
+  NormArgs a;
+  a.dtype = code_of(x.scalar_type(), "norm");
+  a.rows = x.size(0);
+  a.d = x.size(1);
+  a.x = x.data_ptr();
+  a.ldx = x.stride(0);
+  if (y.has_value()) {
+    TORCH_CHECK(y->device() == x.device() && y->sizes() == x.sizes() && y->scalar_type() == x.scalar_type() &&
+                    (y->stride(1) == 1 || y->size(1) == 1),
+                "einshard norm: block output of the stream's shape and type");
+    a.y = y->data_ptr();
+    a.ldy = y->stride(0);
+  }
+  TORCH_CHECK(y.has_value() || (!post && !gate.has_value()), "einshard norm: a norm or gate of an absent block");
+  norm_param(a.w, w, x, a.d, "weight");
+  norm_param(a.b, b, x, a.d, "bias");
+  norm_param(a.pw, pw, x, a.d, "post weight");
+  norm_param(a.pb, pb, x, a.d, "post bias");
+  TORCH_CHECK(post || (!pw.has_value() && !pb.has_value()), "einshard norm: post parameters without post");
+  if (gate.has_value()) {
+    TORCH_CHECK(gate_inner > 0 && gate_count > 0 && a.rows % (gate_inner * gate_count) == 0,
+                "einshard norm: gate rows");
+    norm_param(a.gate, gate, x, gate_count * a.d, "gate");
+    a.gate_inner = gate_inner;
+    a.gate_count = gate_count;
+  }
+  a.post = post;
+  a.center = center;
+  a.scale = static_cast<float>(scale);
+  a.eps = static_cast<float>(eps);
+  a.sms = sms_of(x);
+  return a;
+}
+
+// (h, n, stats); h is undefined without a block output, stats unless kept
+std::vector<Opt> norm_forward_op(const at::Tensor& x, const Opt& y, const Opt& w, const Opt& b, const Opt& pw,
+                                 const Opt& pb, const Opt& gate, int64_t gate_inner, int64_t gate_count, bool post,
+                                 bool center, double scale, double eps, bool keep) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const NormArgs a = norm_args(x, y, w, b, pw, pb, gate, gate_inner, gate_count, post, center, scale, eps);
+  NormForward f;
+  Opt h, stats;
+  at::Tensor n = at::empty(x.sizes(), x.options());
+  f.n = n.data_ptr();
+  if (y.has_value()) {
+    h = at::empty(x.sizes(), x.options());
+    f.h = h->data_ptr();
+  }
+  if (keep) {
+    stats = at::empty({x.size(0), 4}, x.options().dtype(at::kFloat));
+    f.stats = stats->data_ptr<float>();
+  }
+  if (x.numel() > 0) counted(norm_forward(a, f, at::cuda::getCurrentCUDAStream()), "norm");
+  return {h, n, stats};
+}
+
+// Gradients of x, y, w, b, pw, pb, gate (as `want` says) for those of h and n
+std::vector<Opt> norm_backward_op(const Opt& dh, const Opt& dn, const at::Tensor& x, const Opt& y, const Opt& w,
+                                  const Opt& b, const Opt& pw, const Opt& pb, const Opt& gate, int64_t gate_inner,
+                                  int64_t gate_count, bool post, bool center, double scale, double eps,
+                                  const at::Tensor& stats, const std::vector<bool>& want) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const NormArgs a = norm_args(x, y, w, b, pw, pb, gate, gate_inner, gate_count, post, center, scale, eps);
+  TORCH_CHECK(want.size() == 7, "einshard norm: seven gradients");
+  TORCH_CHECK(stats.device() == x.device() && stats.is_contiguous() && stats.scalar_type() == at::kFloat &&
+                  stats.numel() == 4 * a.rows,
+              "einshard norm: statistics of the forward pass");
+  std::vector<Opt> out(7);
+  const Opt given[7] = {x, y, w, b, pw, pb, gate};
+  for (int i = 0; i < 7; ++i) {
+    if (!want[i] || !given[i].has_value()) continue;
+    out[i] = a.rows == 0 ? at::zeros(given[i]->sizes(), given[i]->options())
+                         : at::empty(given[i]->sizes(), given[i]->options());
+  }
+  if (a.rows == 0) return out;
+  for (const Opt& g : {dh, dn})
+    TORCH_CHECK(!g.has_value() || (g->device() == x.device() && g->sizes() == x.sizes() && g->is_contiguous() &&
+                                   g->scalar_type() == x.scalar_type()),
+                "einshard norm: gradients of the stream's shape and type, contiguous");
+  NormPlan plan = norm_plan(a);
+  NormBackward g;
+  NormSums s;
+  g.dh = dh.has_value() ? dh->data_ptr() : nullptr;
+  g.dn = dn.has_value() ? dn->data_ptr() : nullptr;
+  g.stats = stats.data_ptr<float>();
+  g.dx = out[0].has_value() ? out[0]->data_ptr() : nullptr;
+  g.dy = out[1].has_value() ? out[1]->data_ptr() : nullptr;
+  s.dw = out[2].has_value() ? out[2]->data_ptr() : nullptr;
+  s.db = out[3].has_value() ? out[3]->data_ptr() : nullptr;
+  s.dpw = out[4].has_value() ? out[4]->data_ptr() : nullptr;
+  s.dpb = out[5].has_value() ? out[5]->data_ptr() : nullptr;
+  at::Tensor products, ws, coef;
+  if (out[6].has_value()) {
+    if (plan.grouped) {
+      s.dgate = out[6]->data_ptr();
+    } else if (gate_count == a.rows) {
+      g.dgate_rows = out[6]->data_ptr();
+      g.dgate_f32 = a.gate.f32;
+    } else {
+      products = at::empty({a.rows, a.d}, x.options().dtype(at::kFloat));
+      g.dgate_rows = products.data_ptr();
+      g.dgate_f32 = 1;
+    }
+  }
+  if (s.dw || s.db || s.dpw || s.dpb || s.dgate) {
+    ws = at::empty({plan.units(), plan.sums(), a.d}, x.options().dtype(at::kFloat));
+    g.ws = ws.data_ptr<float>();
+  }
+  if (!norm_in_registers(a)) {
+    coef = at::empty({a.rows, 4}, x.options().dtype(at::kFloat));
+    g.coef = coef.data_ptr<float>();
+  }
+  int launches = 0;
+  const int rc = norm_backward(a, plan, g, s, at::cuda::getCurrentCUDAStream(), &launches);
+  counted(rc, "norm backward", launches);
+  if (products.defined()) {
+    const int64_t outer = a.rows / (gate_inner * gate_count);
+    out[6]->copy_(products.view({outer, gate_count, gate_inner, a.d}).sum(c10::IntArrayRef{0, 2}).view(out[6]->sizes()));
+  }
+  return out;
+}
+
 }  // namespace
 
 void bind_training_ops(pybind11::module_& m, std::atomic<long long>& launches) {
   g_count = &launches;
   m.def("quant8", &quant8_op, "(codes, exponents) of a [rows, d] tensor kept in 8 bits");
   m.def("quant8_silu", &quant8_silu_op, "(silu(h), codes, exponents) of an fp32 pre-activation");
+  m.def("norm_forward", &norm_forward_op, "(h, n, statistics) of the norms around a block's residual");
+  m.def("norm_backward", &norm_backward_op, "gradients of norm_forward");
   m.def("restore8", &restore8_op, "what 8-bit codes stand for, its silu, or grad * silu'");
 }
 

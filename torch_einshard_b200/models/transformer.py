@@ -28,6 +28,7 @@ import torch.utils.checkpoint
 import torch.nn.functional as F
 
 from ..api import einshard
+from ..ops.norm import einnorm
 from ..ops.saved8 import checkpoint8
 from ..params import register_parameter_layout
 
@@ -35,9 +36,14 @@ __all__ = ["TransformerConfig", "TPTransformer", "transformer_flops_per_token"]
 
 
 class TransformerConfig:
-    def __init__(self, layers=24, d=2048, heads=16, mlp=8192, vocab=32000, seq=8192, dtype=torch.bfloat16):
-        self.layers, self.d, self.heads, self.mlp, self.vocab, self.seq, self.dtype = \
-            layers, d, heads, mlp, vocab, seq, dtype
+    def __init__(self, layers=24, d=2048, heads=16, mlp=8192, vocab=32000, seq=8192, dtype=torch.bfloat16,
+                 norm="pre"):
+        # norm="sandwich": every block's output is normed too and enters the stream through a gate per channel
+        # (ops/norm.py, one pass for both norms, gate and residual)
+        if norm not in ("pre", "sandwich"):
+            raise ValueError(f"norm must be 'pre' or 'sandwich', not {norm!r}")
+        self.layers, self.d, self.heads, self.mlp, self.vocab, self.seq, self.dtype, self.norm = \
+            layers, d, heads, mlp, vocab, seq, dtype, norm
 
 
 def transformer_flops_per_token(cfg, *, backward=True):
@@ -47,6 +53,11 @@ def transformer_flops_per_token(cfg, *, backward=True):
     per_layer = dense + attention
     total = cfg.layers * per_layer + 2 * cfg.d * cfg.vocab
     return total * (3 if backward else 1)
+
+
+def _after_block(x, y, post, gate, norm):
+    return einnorm("b s d", x, y, axis="d", weight=norm.weight, bias=norm.bias, eps=norm.eps, post=True,
+                   post_weight=post.weight, post_bias=post.bias, gate=gate, gate_axes="d")
 
 
 class _Block(torch.nn.Module):
@@ -76,11 +87,24 @@ class _Block(torch.nn.Module):
         self.w_dn = shard(d, cfg.mlp, std / math.sqrt(2 * cfg.layers), dim=1)
         self.ln1 = torch.nn.LayerNorm(d, device=device, dtype=cfg.dtype)
         self.ln2 = torch.nn.LayerNorm(d, device=device, dtype=cfg.dtype)
+        self.sandwich = cfg.norm == "sandwich"
+        if self.sandwich:
+            self.post1 = torch.nn.LayerNorm(d, device=device, dtype=cfg.dtype)
+            self.post2 = torch.nn.LayerNorm(d, device=device, dtype=cfg.dtype)
+            # every block starts as a small correction of the stream
+            gate = 1.0 / math.sqrt(2 * cfg.layers)
+            self.gate1 = torch.nn.Parameter(torch.full((d,), gate, device=device, dtype=cfg.dtype))
+            self.gate2 = torch.nn.Parameter(torch.full((d,), gate, device=device, dtype=cfg.dtype))
         assert e == self.wq.shape[0] and f == self.w_up.shape[0]
 
     def forward(self, x, mesh):
         x = x + self.attention(self.ln1(x), mesh)
         return x + self.mlp(self.ln2(x), mesh)
+
+    def residual(self, x, n, mesh, next_norm):
+        """The stream and the next block's normed input, from this block's (norm="sandwich")."""
+        x, n = _after_block(x, self.attention(n, mesh), self.post1, self.gate1, self.ln2)
+        return _after_block(x, self.mlp(n, mesh), self.post2, self.gate2, next_norm)
 
     def _keep(self, t):
         """The operand of the next contractions: kept for backward in 8 bits when the model says so."""
@@ -134,18 +158,35 @@ class TPTransformer(torch.nn.Module):
             for ln in (block.ln1, block.ln2):
                 for p in ln.parameters():
                     register_parameter_layout(p, "c", mesh_dim_names=names)
+            if block.sandwich:
+                for p in (*block.post1.parameters(), *block.post2.parameters(), block.gate1, block.gate2):
+                    register_parameter_layout(p, "c", mesh_dim_names=names)
         register_parameter_layout(self.embed, "v d", mesh_dim_names=names)
         for p in self.ln_f.parameters():
             register_parameter_layout(p, "c", mesh_dim_names=names)
 
+    def _sandwich(self, x, recompute):
+        norms = [block.ln1 for block in self.blocks] + [self.ln_f]
+        x, n = einnorm("b s d", x, axis="d", weight=norms[0].weight, bias=norms[0].bias, eps=norms[0].eps)
+        for block, after in zip(self.blocks, norms[1:]):
+            if recompute:
+                x, n = torch.utils.checkpoint.checkpoint(block.residual, x, n, self.mesh, after, use_reentrant=False)
+            else:
+                x, n = block.residual(x, n, self.mesh, after)
+        return n
+
     def forward(self, tokens, targets=None):
         x = F.embedding(tokens, self.embed)
-        for block in self.blocks:
-            if self.checkpoint and self.checkpoint != "int8" and torch.is_grad_enabled():
-                x = torch.utils.checkpoint.checkpoint(block, x, self.mesh, use_reentrant=False)
-            else:
-                x = block(x, self.mesh)
-        x = self.ln_f(x)
+        recompute = self.checkpoint and self.checkpoint != "int8" and torch.is_grad_enabled()
+        if self.cfg.norm == "sandwich":
+            x = self._sandwich(x, recompute)
+        else:
+            for block in self.blocks:
+                if recompute:
+                    x = torch.utils.checkpoint.checkpoint(block, x, self.mesh, use_reentrant=False)
+                else:
+                    x = block(x, self.mesh)
+            x = self.ln_f(x)
         logits = einshard("b s d, v d -> b s v", x, self.embed)
         if targets is None:
             return logits

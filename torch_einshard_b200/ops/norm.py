@@ -1,0 +1,246 @@
+"""``einnorm``: the norms before and after a block, fused with its gate and the scaled residual stream.
+
+For a residual stream ``x`` and a block's output ``y`` over named axes,
+
+    p = norm(y) * post_weight + post_bias     (``post=True``; otherwise p = y)
+    h = scale * x + gate * p                  the new stream
+    n = norm(h) * weight + bias               the next block's input
+
+in one pass over x and y (``csrc/norm.cu``), and one for the gradients of all of
+them.  ``kind`` is "layer" (mean and variance) or "rms".  The gate has its own
+axes: a vector of the normalised axis, a row for every batch entry, one for
+every token, a scalar; its gradient is summed over the axes it lacks.  The
+statistics, h before its norm and all sums are 32-bit; h and n are rounded
+once, and n is the norm of h before that rounding.
+
+Every axis but the normalised one may be sharded (the operation is local to a
+rank; gradients of replicated parameters are reduced as those of any other
+local operation are, by the registered hooks).  CUDA tensors of 16 and 32 bits
+run natively, everything else on torch.  An extension of this framework.
+"""
+
+import math
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ..notation.families import cached_expand_axis_families
+from ..notation.parser import parse_sharding
+from ..notation.spec import AxisGroup, EllipsisAxis
+from . import _native
+
+__all__ = ["einnorm"]
+
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _axes(formula, families, label):
+    formula, _ = cached_expand_axis_families(formula, families=families)
+    spec = parse_sharding(f"{formula} -> {formula}")[0]
+    if getattr(spec, "partials", ()):
+        raise ValueError(f"einnorm does not take partial sums in {label}")
+    names = set()
+    for axis in spec.axes:
+        if isinstance(axis, AxisGroup):
+            raise NotImplementedError(f"einnorm does not support factored axes in {label}")
+        if axis.name in names:
+            raise ValueError(f"Axis {axis.name!r} appears more than once in {label}")
+        names.add(axis.name)
+    return list(spec.axes)
+
+
+def _written_out(axes, rank):
+    """Axis keys with the ellipsis replaced by one key per dimension it covers."""
+    width = rank - sum(1 for a in axes if not isinstance(a, EllipsisAxis))
+    out = []
+    for a in axes:
+        if isinstance(a, EllipsisAxis):
+            out.extend(("...", i) for i in range(max(width, 0)))
+        else:
+            out.append(a)
+    return out
+
+
+def _check_like(t, x, name):
+    if t.shape != x.shape or t.dtype != x.dtype or t.device != x.device:
+        raise ValueError(f"{name} must have the stream's shape, dtype and device: {tuple(t.shape)}, {t.dtype} on "
+                         f"{t.device} for {tuple(x.shape)}, {x.dtype} on {x.device}")
+
+
+def _check_vector(t, x, d, name):
+    if t is None:
+        return
+    if t.shape != (d,):
+        raise ValueError(f"{name} must have the normalised axis alone ({d}), not {tuple(t.shape)}")
+    _check_param(t, x, name)
+
+
+def _check_param(t, x, name):
+    if t.device != x.device or t.dtype not in (x.dtype, torch.float32):
+        raise ValueError(f"{name} must be {x.dtype} or float32 on {x.device}, not {t.dtype} on {t.device}")
+
+
+def _gate_rows(gate, gate_keys, lead, shape, norm_key, d):
+    """The gate as [count, d] with its row for a stream row r at (r // inner) % count.
+
+    ``lead`` are the stream's other axes in order, ``shape`` their lengths.  Axes
+    the gate has must cover a run of them; where they do not, it is expanded to
+    the run around them (the gradient sums again, by autograd)."""
+    if norm_key not in gate_keys:
+        gate = gate.unsqueeze(-1).expand(*gate.shape, d)
+        gate_keys = gate_keys + [norm_key]
+    order = [k for k in lead if k in gate_keys] + [norm_key]
+    gate = gate.permute([gate_keys.index(k) for k in order])
+    # axes of length one change nothing: drop them
+    keep = [i for i, k in enumerate(order[:-1]) if gate.shape[i] != 1]
+    present = [order[i] for i in keep]
+    gate = gate.reshape([gate.shape[i] for i in keep] + [d])
+    if not present:
+        return gate.reshape(1, d), math.prod(shape), 1
+    places = [lead.index(k) for k in present]
+    low, high = places[0], places[-1] + 1
+    run = list(shape[low:high])
+    view = [s if lead[low + i] in present else 1 for i, s in enumerate(run)]
+    gate = gate.reshape(view + [d]).expand(run + [d])
+    return gate.reshape(math.prod(run), d), math.prod(shape[high:]), math.prod(run)
+
+
+def _rows(t):
+    t = t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
+
+
+class _NativeNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, y, w, b, pw, pb, gate, conf):
+        h, n, stats = _native.require().norm_forward(x, y, w, b, pw, pb, gate, *conf, any(ctx.needs_input_grad))
+        ctx.conf = conf
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, y, w, b, pw, pb, gate, stats)
+        return (h, n) if y is not None else n
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        *tensors, stats = ctx.saved_tensors
+        dh, dn = grads if len(grads) == 2 else (None, grads[0])
+        if dh is None and dn is None:
+            return (None,) * 8
+        dh, dn = (None if g is None else g.contiguous() for g in (dh, dn))
+        out = _native.require().norm_backward(dh, dn, *tensors, *ctx.conf, stats, list(ctx.needs_input_grad[:7]))
+        return (*out, None)
+
+
+def _torch_norm(x, y, w, b, pw, pb, gate, conf):
+    inner, count, post, center, scale, eps = conf
+    dtype = x.dtype
+    wide = torch.promote_types(dtype, torch.float32)
+
+    def normed(t, weight, bias):
+        if center:
+            t = t - t.mean(-1, keepdim=True)
+        t = t / torch.sqrt(t.square().mean(-1, keepdim=True) + eps)
+        t = t if weight is None else t * weight.to(wide)
+        return t if bias is None else t + bias.to(wide)
+
+    h = x.to(wide)
+    if y is not None:
+        p = y.to(wide)
+        if post:
+            p = normed(p, pw, pb)
+        if gate is not None:
+            rows = torch.arange(x.shape[0], device=x.device) // inner % count
+            p = p * gate.to(wide)[rows]
+        h = scale * h + p
+    n = normed(h, w, b).to(dtype)
+    return n if y is None else (h.to(dtype), n)
+
+
+def _on_kernels(x):
+    if not x.is_cuda or x.dtype not in _TYPES:
+        return False
+    if _native.available():
+        return True
+    if _native.allow_fallback():
+        return False
+    _native.require()  # raises: native extension missing on a CUDA machine
+    return False
+
+
+def einnorm(shard, x, y=None, *, axis, weight=None, bias=None, kind="layer", eps=1e-5, post=False, post_weight=None,
+            post_bias=None, gate=None, gate_axes=None, scale=1.0, families=None):
+    """Residual stream and next input ``(h, n)`` after a block (see the module docstring).
+
+    ``shard`` names the axes of ``x`` and ``y`` ("b s d"), ``axis`` the one that
+    is normalised, ``gate_axes`` those of ``gate`` ("d", "b d", "b s d", "b", ...).
+    Without ``y`` there is no block yet: ``h`` is ``x`` and ``n`` its norm.
+    Parameters and gate are of the stream's type or fp32."""
+    axes = _axes(shard, families, "the stream")
+    if x.dtype not in (*_TYPES, torch.float64):
+        raise TypeError(f"einnorm takes floating-point tensors, not {x.dtype}")
+    keys = _written_out(axes, x.dim())
+    if len(keys) != x.dim():
+        raise ValueError(f"The stream has {x.dim()} dimensions, {shard!r} names {len(axes)} axes")
+    found = [k for k in keys if not isinstance(k, tuple) and k.name == axis]
+    if not found:
+        raise ValueError(f"Axis {axis!r} is not among the stream's axes")
+    norm_key = found[0]
+    if not norm_key.local():
+        raise NotImplementedError(f"einnorm needs the normalised axis {axis!r} whole on every rank")
+    place = keys.index(norm_key)
+    d = x.shape[place]
+    if d == 0:
+        raise ValueError(f"The normalised axis {axis!r} is empty")
+    if kind not in ("layer", "rms"):
+        raise ValueError(f"kind must be 'layer' or 'rms', not {kind!r}")
+    if not (math.isfinite(eps) and eps >= 0):
+        raise ValueError(f"eps must be finite and not negative, not {eps}")
+    if not math.isfinite(scale):
+        raise ValueError(f"scale must be finite, not {scale}")
+    if y is None and (post or gate is not None or scale != 1.0):
+        raise ValueError("post, gate and scale belong to a block's output y")
+    if not post and (post_weight is not None or post_bias is not None):
+        raise ValueError("post_weight and post_bias need post=True")
+    if y is not None:
+        _check_like(y, x, "y")
+    for t, name in ((weight, "weight"), (bias, "bias"), (post_weight, "post_weight"), (post_bias, "post_bias")):
+        _check_vector(t, x, d, name)
+
+    lead = keys[:place] + keys[place + 1:]
+    shape = list(x.shape[:place]) + list(x.shape[place + 1:])
+    inner = count = 1
+    if gate is not None:
+        if gate_axes is None:
+            raise ValueError("gate needs gate_axes")
+        width = x.dim() - sum(1 for a in axes if not isinstance(a, EllipsisAxis))
+        named = _axes(gate_axes, families, "the gate") if gate_axes.strip() else []  # "": a scalar
+        gate_keys = _written_out(named, len(named) - 1 + width if any(isinstance(a, EllipsisAxis) for a in named)
+                                 else len(named))
+        if len(gate_keys) != gate.dim():
+            raise ValueError(f"The gate has {gate.dim()} dimensions, {gate_axes!r} names {len(gate_keys)} axes")
+        for k, size in zip(gate_keys, gate.shape):
+            if k not in keys:
+                raise ValueError(f"The gate's axis {k} is not one of the stream's")
+            if size != x.shape[keys.index(k)]:
+                raise ValueError(f"The gate's axis {k} has length {size}, the stream's {x.shape[keys.index(k)]}")
+        _check_param(gate, x, "gate")
+        if x.numel():
+            gate, inner, count = _gate_rows(gate, gate_keys, lead, shape, norm_key, d)
+        else:
+            gate = gate.sum().expand(1, d)  # no row to weigh: in the graph, with a gradient of zero
+            inner = 1
+    elif gate_axes is not None:
+        raise ValueError("gate_axes without a gate")
+
+    conf = (inner, count, bool(post), kind == "layer", float(scale), float(eps))
+    args = [_rows(x.movedim(place, -1)), None if y is None else _rows(y.movedim(place, -1))]
+    params = [None if t is None else t.contiguous() for t in (weight, bias, post_weight, post_bias, gate)]
+    if _on_kernels(x):
+        out = _NativeNorm.apply(*args, *params, conf)
+    else:
+        out = _torch_norm(*args, *params, conf)
+
+    def back(t):
+        return t.reshape(*shape, d).movedim(-1, place)
+
+    return (x, back(out)) if y is None else (back(out[0]), back(out[1]))
