@@ -16,6 +16,7 @@ from .ops.einsum import einsum
 from .ops.fft import einfft
 from .ops.halo import einhalo, einwindow
 from .ops.norm import einnorm
+from .ops.policy import PolicyLoss, einpolicy
 from .ops.roll import einroll
 from .ops.saved8 import Saved8, checkpoint8
 from .parallel.executor import distributed_1d

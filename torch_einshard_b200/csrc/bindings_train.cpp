@@ -1,5 +1,6 @@
 // Torch bindings of the training-step operators around the contractions:
-// activations kept in 8 bits (quant8.h), norms with gate and residual (norm.h).
+// activations kept in 8 bits (quant8.h), norms with gate and residual (norm.h),
+// the policy loss (policy.h).
 #include "bindings_train.h"
 
 #include <ATen/cuda/CUDAContext.h>
@@ -7,6 +8,7 @@
 
 #include "gemm.h"
 #include "norm.h"
+#include "policy.h"
 #include "quant8.h"
 
 namespace es {
@@ -236,6 +238,104 @@ std::vector<Opt> norm_backward_op(const Opt& dh, const Opt& dn, const at::Tensor
   return out;
 }
 
+// ------------------------------------------------------------------ policy loss
+
+void per_token(const Opt& t, const at::Tensor& logits, int64_t count, at::ScalarType type, const char* name) {
+  if (!t.has_value()) return;
+  TORCH_CHECK(t->device() == logits.device() && t->is_contiguous() && t->numel() == count && t->scalar_type() == type,
+              "einshard policy loss: ", name, " of ", count, " elements, contiguous, ", type);
+}
+
+PolicyArgs policy_args(const at::Tensor& logits, const at::Tensor& ids, const Opt& mask, const Opt& old,
+                       const Opt& ref, const at::Tensor& adv, int64_t length, double lo, double hi, double kl,
+                       double temperature, int64_t reduction, double weight) {
+  TORCH_CHECK(logits.is_cuda() && logits.dim() == 2 && logits.size(1) > 0 &&
+                  (logits.stride(1) == 1 || logits.size(1) == 1),
+              "einshard policy loss: [tokens, vocabulary] CUDA logits");
+  PolicyArgs a;
+  a.dtype = code_of(logits.scalar_type(), "policy loss");
+  a.logits = logits.data_ptr();
+  a.tokens = logits.size(0);
+  a.vocab = logits.size(1);
+  a.ld = logits.stride(0);
+  TORCH_CHECK(length > 0 && a.tokens % length == 0, "einshard policy loss: sequence length");
+  a.length = length;
+  per_token(ids, logits, a.tokens, at::kLong, "ids");
+  per_token(mask, logits, a.tokens, at::kBool, "mask");
+  per_token(old, logits, a.tokens, at::kFloat, "old log-probabilities");
+  per_token(ref, logits, a.tokens, at::kFloat, "reference log-probabilities");
+  const bool per_sequence = adv.numel() != a.tokens;
+  per_token(adv, logits, per_sequence ? a.tokens / length : a.tokens, at::kFloat, "advantages");
+  a.ids = ids.data_ptr<int64_t>();
+  a.mask = mask.has_value() ? mask->data_ptr<bool>() : nullptr;
+  a.old = old.has_value() ? old->data_ptr<float>() : nullptr;
+  a.ref = ref.has_value() ? ref->data_ptr<float>() : nullptr;
+  a.adv = adv.data_ptr<float>();
+  a.adv_per_sequence = per_sequence;
+  a.lo = static_cast<float>(lo);
+  a.hi = static_cast<float>(hi);
+  a.kl = static_cast<float>(kl);
+  a.inv_temp = static_cast<float>(1.0 / temperature);
+  a.reduction = static_cast<int>(reduction);
+  a.weight = static_cast<float>(weight);
+  a.sms = sms_of(logits);
+  return a;
+}
+
+PolicyState policy_state(const at::Tensor& logp, const at::Tensor& terms, const at::Tensor& norm,
+                         const at::Tensor& weight) {
+  PolicyState s;
+  s.logp = logp.data_ptr<float>();
+  s.terms = reinterpret_cast<float4*>(terms.data_ptr<float>());
+  s.norm = reinterpret_cast<float2*>(norm.data_ptr<float>());
+  s.weight = weight.data_ptr<float>();
+  return s;
+}
+
+// (loss, KL, clipped share, logp, terms, norm, weight)
+std::vector<at::Tensor> policy_forward_op(const at::Tensor& logits, const at::Tensor& ids, const Opt& mask,
+                                          const Opt& old, const Opt& ref, const at::Tensor& adv, int64_t length,
+                                          double lo, double hi, double kl, double temperature, int64_t reduction,
+                                          double weight) {
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const PolicyArgs a = policy_args(logits, ids, mask, old, ref, adv, length, lo, hi, kl, temperature, reduction, weight);
+  const auto f32 = logits.options().dtype(at::kFloat);
+  const int64_t sequences = a.tokens / length;
+  TORCH_CHECK(a.tokens > 0, "einshard policy loss: no tokens");
+  at::Tensor loss = at::empty({}, f32), kl_out = at::empty({}, f32), clipped = at::empty({}, f32);
+  at::Tensor logp = at::empty({a.tokens}, f32), terms = at::empty({a.tokens, 4}, f32);
+  at::Tensor norm = at::empty({a.tokens, 2}, f32), weights = at::empty({sequences}, f32);
+  at::Tensor sums = at::empty({sequences, 4}, f32);
+  PolicyState s = policy_state(logp, terms, norm, weights);
+  s.sums = reinterpret_cast<float4*>(sums.data_ptr<float>());
+  s.loss = loss.data_ptr<float>();
+  s.kl = kl_out.data_ptr<float>();
+  s.clipped = clipped.data_ptr<float>();
+  int launches = 0;
+  counted(policy_forward(a, s, at::cuda::getCurrentCUDAStream(), &launches), "policy loss", 0);
+  g_count->fetch_add(launches, std::memory_order_relaxed);
+  return {loss, kl_out, clipped, logp, terms, norm, weights};
+}
+
+at::Tensor policy_backward_op(const at::Tensor& grad, const at::Tensor& logits, const at::Tensor& ids,
+                              const Opt& mask, const Opt& old, const Opt& ref, const at::Tensor& adv, int64_t length,
+                              double lo, double hi, double kl, double temperature, int64_t reduction, double weight_factor,
+                              const at::Tensor& terms, const at::Tensor& norm, const at::Tensor& weight) {
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const PolicyArgs a = policy_args(logits, ids, mask, old, ref, adv, length, lo, hi, kl, temperature, reduction, weight_factor);
+  TORCH_CHECK(grad.device() == logits.device() && grad.numel() == 1 && grad.scalar_type() == at::kFloat,
+              "einshard policy loss: fp32 gradient of the loss");
+  per_token(terms, logits, 4 * a.tokens, at::kFloat, "terms");
+  per_token(norm, logits, 2 * a.tokens, at::kFloat, "norms");
+  per_token(weight, logits, a.tokens / length, at::kFloat, "weights");
+  TORCH_CHECK(a.tokens > 0, "einshard policy loss: no tokens");
+  at::Tensor out = at::empty(logits.sizes(), logits.options());
+  const PolicyState s = policy_state(terms, terms, norm, weight);
+  counted(policy_backward(a, s, grad.data_ptr<float>(), out.data_ptr(), at::cuda::getCurrentCUDAStream()),
+          "policy loss backward");
+  return out;
+}
+
 }  // namespace
 
 void bind_training_ops(pybind11::module_& m, std::atomic<long long>& launches) {
@@ -244,6 +344,8 @@ void bind_training_ops(pybind11::module_& m, std::atomic<long long>& launches) {
   m.def("quant8_silu", &quant8_silu_op, "(silu(h), codes, exponents) of an fp32 pre-activation");
   m.def("norm_forward", &norm_forward_op, "(h, n, statistics) of the norms around a block's residual");
   m.def("norm_backward", &norm_backward_op, "gradients of norm_forward");
+  m.def("policy_forward", &policy_forward_op, "clipped policy loss of token logits, with what its gradient needs");
+  m.def("policy_backward", &policy_backward_op, "gradient of policy_forward by the logits");
   m.def("restore8", &restore8_op, "what 8-bit codes stand for, its silu, or grad * silu'");
 }
 

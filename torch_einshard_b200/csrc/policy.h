@@ -1,0 +1,43 @@
+// Clipped policy loss with a KL term from logits (policy.cu).  dtype codes as in gemm.h.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace es {
+
+enum PolicyReduction : int { kReduceMean = 0, kReduceSequence = 1, kReduceSum = 2 };
+
+struct PolicyArgs {
+  int dtype = 0;
+  const void* logits = nullptr;  // [tokens, vocab], row pitch ld
+  long long ld = 0, tokens = 0, vocab = 0;
+  long long length = 1;            // tokens of a sequence (tokens = sequences * length)
+  const int64_t* ids = nullptr;    // [tokens]
+  const bool* mask = nullptr;      // [tokens]; null: every token counts
+  const float* old = nullptr;      // [tokens]; null: the log-probabilities themselves
+  const float* ref = nullptr;      // [tokens]; null: no KL term
+  const float* adv = nullptr;      // [tokens], or one a sequence
+  int adv_per_sequence = 0;
+  float lo = 0.2f, hi = 0.2f, kl = 0.0f, inv_temp = 1.0f;
+  float weight = 1.0f;             // factor of the loss
+  int reduction = kReduceMean;
+  int sms = 148;
+};
+
+struct PolicyState {
+  float* logp = nullptr;    // [tokens] output: log-probability of the token, 0 where masked
+  float4* terms = nullptr;  // [tokens] loss, KL, clipped, derivative of the loss by logp (without weights)
+  float2* norm = nullptr;   // [tokens] largest logit and log2 of the sum of exponentials
+  float* weight = nullptr;  // [sequences] weight of a token's loss
+  float4* sums = nullptr;   // [sequences] scratch
+  float* loss = nullptr;    // scalars
+  float* kl = nullptr;
+  float* clipped = nullptr;
+};
+
+int policy_forward(const PolicyArgs& a, const PolicyState& s, cudaStream_t stream, int* launches);
+// dlogits [tokens, vocab] contiguous, for the gradient *grad of the loss
+int policy_backward(const PolicyArgs& a, const PolicyState& s, const float* grad, void* dlogits, cudaStream_t stream);
+
+}  // namespace es

@@ -29,6 +29,7 @@ import torch.nn.functional as F
 
 from ..api import einshard
 from ..ops.norm import einnorm
+from ..ops.policy import einpolicy
 from ..ops.saved8 import checkpoint8
 from ..params import register_parameter_layout
 
@@ -191,3 +192,9 @@ class TPTransformer(torch.nn.Module):
         if targets is None:
             return logits
         return F.cross_entropy(logits.float().flatten(0, 1), targets.flatten())
+
+    def policy_loss(self, tokens, *, advantages, mask=None, **options):
+        """Clipped policy loss (ops/policy.py:einpolicy, which takes ``options``) of the tokens from the second on,
+        each predicted from those before it; ``mask`` and the log-probabilities have one entry for each of these."""
+        logits = self(tokens[:, :-1])
+        return einpolicy("b s v", logits, tokens[:, 1:], axis="v", advantages=advantages, mask=mask, **options)
