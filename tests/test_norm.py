@@ -150,7 +150,7 @@ def test_forward_and_gradients(device, dtype, kind, shape):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("kind", ["layer", "rms"])
-@pytest.mark.parametrize("d", [4104, 8192, 8191, 8200, 10001])
+@pytest.mark.parametrize("d", [4104, 8192, 8191, 8200, 10001, 16384, 32776, 65536, 65544])
 @pytest.mark.parametrize("gate", ["channel", "token"])
 def test_wide_rows(dtype, kind, d, gate):
     check(*make("cuda", dtype, (2, 21, d), kind=kind, gate=gate))

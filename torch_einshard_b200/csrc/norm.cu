@@ -18,103 +18,165 @@
 // dependent ones.  h is formed again from x and y in 32 bits, never read back
 // rounded.
 //
-// The kernels are bound by memory (8 bytes a 16-bit element forward, 12
-// backward).  A block of d / 8 threads holds a row in registers, eight elements
-// a thread; the column sums of the parameters' gradients stay in registers
-// (in shared memory above 4096 columns, where registers run out) over the
-// block's rows, go to a workspace once a block, and a second kernel adds them
-// in a fixed order.  A gate that is constant over the block's rows leaves its
-// own sum and dpw's: S1 = sum D yh gives dgate = pw S1 + pb S0 and gate S1.
-//
-// Rows wider than 8192 take several passes over the row through the caches.
+// Memory is the bound (8 bytes a 16-bit element forward, 12 backward), and a
+// row's fixed work (reductions, addresses) comes next: a thread holds 16
+// elements, arithmetic is in fp32 pairs, and rows come through shared memory by
+// asynchronous copies, up to three ahead of the one at work.  The column sums of
+// the parameters' gradients stay in registers (in shared memory above 4096
+// columns a block) over a block's rows, go to a workspace once a block, and a
+// second kernel adds them in a fixed order.  A gate that is constant over the
+// block's rows leaves its own sum and dpw's: S1 = sum D yh gives
+// dgate = pw S1 + pb S0 and gate S1.  Rows too wide for a block are shared by a
+// cluster, still wider ones take several passes through the caches.
 #include "norm.h"
 
 #include "gemm.h"
+#include "ptx.cuh"
 #include "vec.cuh"
 
 namespace es {
 namespace {
 
-constexpr int kE = 8;             // elements of a row a thread holds
-constexpr long long kMaxD = 8192; // 1024 threads
-constexpr long long kRegSums = 4096;
+// A thread holds 2 kP columns of a row, as kP pairs.
+constexpr int kThreads = 512;       // most threads a block has
+constexpr int kRowPairs = 8;
+constexpr int kRegSums = 4096;      // columns whose sums stay in registers
+constexpr int kMaxCluster = 8;
+constexpr int kWideThreads = 512;   // block of the several-pass kernels
 constexpr long long kMinGroup = 16;
-constexpr int kWideThreads = 512; // block of the several-pass kernels
+constexpr int kMaxStages = 4;       // rows in flight
+
+// How a block reads a row: every thread runs of eight columns (kExact), the last threads fewer (kVec), or
+// strided columns of a row without alignment (kAny).
+enum Access : int { kAny = 0, kVec = 1, kExact = 2 };
 
 // ------------------------------------------------------------------ element access
 
-// The thread's eight elements of a row: consecutive with kVec, else strided by the block.
-template <bool kVec>
-__device__ __forceinline__ long long column(int i) {
-  return kVec ? static_cast<long long>(threadIdx.x) * kE + i : static_cast<long long>(i) * blockDim.x + threadIdx.x;
+// The block's part of a row: columns [c0, c0 + n); a row's blocks take `per` each, the last ones what is left.
+struct Span {
+  int d, per, c0, n;
+  __device__ __forceinline__ int columns_of(int rank) const {
+    const int left = d - rank * per;
+    return left < per ? (left > 0 ? left : 0) : per;
+  }
+};
+
+__host__ __device__ __forceinline__ int columns_per_block(long long d, int blocks) {
+  return static_cast<int>(((d + blocks - 1) / blocks + 7) / 8 * 8);
 }
 
-template <typename T, bool kVec>
-struct Elems {
-  Raw8<T> raw;
-  T e[kVec ? 1 : kE];
-  __device__ __forceinline__ void load(const T* row, long long d) {
-    if (kVec) {
-      if (column<true>(0) < d) raw = load8_stream(row + column<true>(0));
-    } else {
+__device__ __forceinline__ Span span_of(const NormArgs& a, int rank, int blocks) {
+  Span s;
+  s.d = static_cast<int>(a.d);
+  s.per = columns_per_block(a.d, blocks);
+  s.c0 = rank * s.per;
+  s.n = s.columns_of(rank);
+  return s;
+}
+
+// First column of the thread's run r of eight (kVec, kExact).
+__device__ __forceinline__ int run_of(int r) {
+  return (r * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x)) * 8;
+}
+
+// Column of the thread's element i.
+template <int kA>
+__device__ __forceinline__ int column(int i) {
+  return kA != kAny ? run_of(i / 8) + i % 8 : i * static_cast<int>(blockDim.x) + static_cast<int>(threadIdx.x);
+}
+
+template <int kA>
+__device__ __forceinline__ bool has(int i, const Span& s) {
+  return kA == kExact || (kA == kVec ? run_of(i / 8) : column<kAny>(i)) < s.n;
+}
+
+// Pair i of a thread's values where its columns exist, else zero.
+template <int kA>
+__device__ __forceinline__ Pair only(Pair v, int i, const Span& s) {
+  if (kA == kExact) return v;
+  if (kA == kVec) return has<kVec>(2 * i, s) ? v : 0ull;
+  const float2 f = both(v);
+  return pair(has<kAny>(2 * i, s) ? f.x : 0.0f, has<kAny>(2 * i + 1, s) ? f.y : 0.0f);
+}
+
+// A stream's rows on their way through shared memory.  With runs of eight a
+// thread copies its own 16 (32) bytes to its own place and needs no barrier to
+// read them.  Otherwise the block copies the aligned 16-byte words that cover its
+// columns, and a barrier comes before the read; nothing behind the row's end is read.
+template <typename T, int kA, int kP>
+struct Stream {
+  static constexpr int kW = static_cast<int>(sizeof(T) / 2);  // 16-byte words of a run
+  static constexpr int kRuns = kP / 4;
+  const T* base;
+  long long ld;
+  uint4* slots;  // [stages][words]
+  int words;
+  __device__ __forceinline__ static int words_of(int n) {
+    return kA != kAny ? static_cast<int>(blockDim.x) * kRuns * kW
+                      : (n * static_cast<int>(sizeof(T)) + 15) / 16 + 1;
+  }
+  __device__ __forceinline__ void fetch(long long row, int stage, const Span& s) const {
+    const T* src = base + row * ld + s.c0;
+    uint4* dst = slots + stage * words;
+    if (kA != kAny) {
 #pragma unroll
-      for (int i = 0; i < kE; ++i)
-        if (column<false>(i) < d) e[kVec ? 0 : i] = row[column<false>(i)];
+      for (int r = 0; r < kRuns; ++r) {
+        if (!has<kA>(8 * r, s)) continue;
+#pragma unroll
+        for (int i = 0; i < kW; ++i)
+          copy16_async(dst + (r * kW + i) * blockDim.x + threadIdx.x,
+                       reinterpret_cast<const uint4*>(src + run_of(r)) + i);
+      }
+    } else {
+      const uintptr_t first = reinterpret_cast<uintptr_t>(src) & ~static_cast<uintptr_t>(15);
+      const uintptr_t end = reinterpret_cast<uintptr_t>(src + s.n);
+      for (uintptr_t p = first + 16 * threadIdx.x; p < end; p += 16 * blockDim.x) {
+        const int bytes = end - p < 16 ? static_cast<int>(end - p) : 16;
+        copy16_async(dst + (p - first) / 16, reinterpret_cast<const void*>(p), bytes);
+      }
     }
   }
-  __device__ __forceinline__ void get(float (&f)[kE], long long d) const {
-    if (kVec) {
-      if (column<true>(0) < d) {
-        unpack8(raw, f);
-        return;
+  __device__ __forceinline__ void read(long long row, int stage, const Span& s, Pair (&f)[kP]) const {
+    const uint4* src = slots + stage * words;
+    if (kA != kAny) {
+#pragma unroll
+      for (int r = 0; r < kRuns; ++r) {
+        Raw8<T> raw;
+#pragma unroll
+        for (int i = 0; i < kW; ++i) raw.w[i] = src[(r * kW + i) * blockDim.x + threadIdx.x];
+        unpack8(raw, f + 4 * r);
       }
-#pragma unroll
-      for (int i = 0; i < kE; ++i) f[i] = 0.0f;
     } else {
+      const int off = static_cast<int>((reinterpret_cast<uintptr_t>(base + row * ld + s.c0) & 15) / sizeof(T));
+      const T* e = reinterpret_cast<const T*>(src) + off;
 #pragma unroll
-      for (int i = 0; i < kE; ++i) f[i] = column<false>(i) < d ? to_float<T>(e[kVec ? 0 : i]) : 0.0f;
+      for (int i = 0; i < kP; ++i)
+        f[i] = pair(has<kAny>(2 * i, s) ? to_float<T>(e[column<kAny>(2 * i)]) : 0.0f,
+                    has<kAny>(2 * i + 1, s) ? to_float<T>(e[column<kAny>(2 * i + 1)]) : 0.0f);
     }
   }
 };
 
-template <typename T, bool kVec>
-__device__ __forceinline__ void put(T* row, const float (&f)[kE], long long d) {
-  if (kVec) {
-    if (column<true>(0) < d) store8(row + column<true>(0), f);
+template <typename T, int kA, int kP>
+__device__ __forceinline__ void put(T* row, const Pair (&f)[kP], const Span& s) {
+  T* out = row + s.c0;
+  if (kA != kAny) {
+#pragma unroll
+    for (int r = 0; r < kP / 4; ++r)
+      if (has<kA>(8 * r, s)) store8(out + run_of(r), f + 4 * r);
   } else {
 #pragma unroll
-    for (int i = 0; i < kE; ++i)
-      if (column<false>(i) < d) row[column<false>(i)] = from_float<T>(f[i]);
+    for (int i = 0; i < kP; ++i) {
+      if (has<kAny>(2 * i, s)) out[column<kAny>(2 * i)] = from_float<T>(lo_of(f[i]));
+      if (has<kAny>(2 * i + 1, s)) out[column<kAny>(2 * i + 1)] = from_float<T>(hi_of(f[i]));
+    }
   }
 }
 
-// A column vector's elements in fp32 (`other` where it is absent).
-template <typename T, bool kVec>
-__device__ __forceinline__ void param(const NormParam& q, long long offset, float other, float (&f)[kE], long long d) {
-  if (q.p == nullptr) {
+template <int kP>
+__device__ __forceinline__ void fill(Pair (&f)[kP], float v) {
 #pragma unroll
-    for (int i = 0; i < kE; ++i) f[i] = other;
-    return;
-  }
-  if (kVec) {
-    const long long c = column<true>(0);
-    if (c >= d) {
-#pragma unroll
-      for (int i = 0; i < kE; ++i) f[i] = 0.0f;
-    } else if (q.f32) {
-      unpack8(load8(static_cast<const float*>(q.p) + offset + c), f);
-    } else {
-      unpack8(load8(static_cast<const T*>(q.p) + offset + c), f);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < kE; ++i) {
-      const long long c = column<false>(i);
-      f[i] = c >= d ? 0.0f
-                    : (q.f32 ? static_cast<const float*>(q.p)[offset + c]
-                             : to_float<T>(static_cast<const T*>(q.p)[offset + c]));
-    }
-  }
+  for (int i = 0; i < kP; ++i) f[i] = pair(v);
 }
 
 template <typename T>
@@ -123,21 +185,77 @@ __device__ __forceinline__ float param1(const NormParam& q, long long i, float o
   return q.f32 ? static_cast<const float*>(q.p)[i] : to_float<T>(static_cast<const T*>(q.p)[i]);
 }
 
-__device__ __forceinline__ long long gate_row(const NormArgs& a, long long row) {
-  return a.gate.p == nullptr ? 0 : (row / a.gate_inner) % a.gate_count;
+// A column vector's elements in fp32, `other` where there is none.
+template <typename T, int kA, int kP>
+__device__ __forceinline__ void param(const NormParam& q, long long offset, float other, Pair (&f)[kP],
+                                      const Span& s) {
+  if (q.p == nullptr) {
+    fill(f, other);
+  } else if (kA != kAny) {
+#pragma unroll
+    for (int r = 0; r < kP / 4; ++r) {
+      const long long c = offset + s.c0 + run_of(r);
+      if (!has<kA>(8 * r, s)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[4 * r + i] = 0ull;
+      } else if (q.f32) {
+        unpack8(load8(static_cast<const float*>(q.p) + c), f + 4 * r);
+      } else {
+        unpack8(load8(static_cast<const T*>(q.p) + c), f + 4 * r);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kP; ++i) {
+      float v[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int k = column<kAny>(2 * i + h);
+        v[h] = k < s.n ? param1<T>(q, offset + s.c0 + k, other) : 0.0f;
+      }
+      f[i] = pair(v[0], v[1]);
+    }
+  }
 }
 
-// ------------------------------------------------------------------ block reductions
+// f times a column vector, where there is one.
+template <typename T, int kA, int kP>
+__device__ __forceinline__ void times(const NormParam& q, long long offset, Pair (&f)[kP], const Span& s) {
+  if (q.p == nullptr) return;
+  Pair v[kP];
+  param<T, kA>(q, offset, 1.0f, v, s);
+#pragma unroll
+  for (int i = 0; i < kP; ++i) f[i] = mul2(f[i], v[i]);
+}
 
-// Sum over the block, in every thread.  `red` holds two sets of 32 words used in
-// turn: one barrier a reduction is enough.
+// All copies but those of the rows behind the next one have landed.
+__device__ __forceinline__ void wait_row(int stages) {
+  if (stages >= 4)
+    copy_wait<2>();
+  else if (stages == 3)
+    copy_wait<1>();
+  else
+    copy_wait<0>();
+}
+
+__device__ __forceinline__ long long gate_row(const NormArgs& a, long long row) {
+  if (a.gate_count == 1) return 0;
+  if (a.gate_count == a.rows) return row;
+  if (a.rows < (1ll << 31))
+    return static_cast<uint32_t>(row) / static_cast<uint32_t>(a.gate_inner) % static_cast<uint32_t>(a.gate_count);
+  return (row / a.gate_inner) % a.gate_count;
+}
+
+// ------------------------------------------------------------------ reductions over a row
+
+// Sum over the block, in every thread, for the several-pass kernels.  `red` holds
+// two sets of 32 words used in turn: one barrier a reduction is enough.
 struct Reducer {
   float* red;
   int turn = 0;
   __device__ __forceinline__ float sum(float v) {
     v = warp_sum(v);
     const int warps = blockDim.x >> 5;
-    if (warps == 1) return v;
     float* set = red + (turn & 1) * 32;
     ++turn;
     if ((threadIdx.x & 31) == 0) set[threadIdx.x >> 5] = v;
@@ -147,10 +265,114 @@ struct Reducer {
   }
 };
 
-// kN sums at once (kN a power of two up to 8): a warp halves the number of
-// values a lane carries with every exchange, so eight sums take nine shuffles.
+// Words of the warps of a row's blocks: a warp's words are stored in every block
+// of the cluster, one barrier later every thread adds them all in the same
+// order.  Two sets in turn: a block writes a set again only behind the next
+// barrier, which every reader of it has passed.
+constexpr int kMaxWarps = kThreads / 32;
+
+template <int kWords>
+struct Exchange {
+  float* mem;  // [2][kMaxCluster x kMaxWarps][kWords], at the same place in every block
+  int rank, blocks, warps, turn = 0;
+  static constexpr int kSet = kMaxCluster * kMaxWarps * kWords;
+  // lane l of a warp stores word l of its kWords
+  __device__ __forceinline__ const float* share(float word, int lane) {
+    float* set = mem + (turn & 1) * kSet;
+    ++turn;
+    float* at = set + (rank * warps + static_cast<int>(threadIdx.x >> 5)) * kWords + lane;
+    if (blocks == 1) {
+      if (lane < kWords) *at = word;
+      __syncthreads();
+    } else {
+      if (lane < kWords)
+        for (int b = 0; b < blocks; ++b) st_cluster_f32(map_to_cta(at, b), word);
+      cluster_sync();
+    }
+    return set;
+  }
+};
+
+__host__ __device__ constexpr int exchange_bytes(int words) { return 2 * kMaxCluster * kMaxWarps * words * 4; }
+
+// Mean and sum of squared differences from it (center), or 0 and the sum of
+// squares, over a row: the warp's own mean and differences first, then the warps' are
+// joined, M2 = sum M2_w + n_w (m_w - m)^2; no difference of large sums is taken.
+template <int kA, int kP>
+__device__ __forceinline__ void row_stats(const Pair (&v)[kP], const Span& s, const NormArgs& a, float inv_d,
+                                          Exchange<2>& ex, float* mean, float* m2) {
+  const int lane = threadIdx.x & 31;
+  // columns of warp w of block b: counted over the runs or strided passes
+  auto count = [&](int b, int w) {
+    if (kA == kExact) return 64 * kP;
+    const int all = s.columns_of(b);
+    int n = 0;
+    constexpr int kPasses = kA == kVec ? kP / 4 : 2 * kP, kStep = kA == kVec ? 8 : 1;
+#pragma unroll
+    for (int i = 0; i < kPasses; ++i) {
+      const int left = all - (i * static_cast<int>(blockDim.x) + w * 32) * kStep;
+      n += left < 0 ? 0 : (left < 32 * kStep ? left : 32 * kStep);
+    }
+    return n;
+  };
+  Pair t = 0ull;
+  float mw = 0.0f;
+  if (a.center) {
+#pragma unroll
+    for (int i = 0; i < kP; ++i) t = add2(t, v[i]);
+    const int n = count(ex.rank, threadIdx.x >> 5);
+    mw = warp_sum(lo_of(t) + hi_of(t)) *
+         (kA == kExact ? 1.0f / (64 * kP) : __fdividef(1.0f, static_cast<float>(n > 0 ? n : 1)));
+    t = 0ull;
+  }
+  const Pair off = pair(-mw);
+#pragma unroll
+  for (int i = 0; i < kP; ++i) {
+    const Pair e = only<kA>(add2(v[i], off), i, s);
+    t = fma2(e, e, t);
+  }
+  const float sq = warp_sum(lo_of(t) + hi_of(t));
+  const int entries = ex.warps * ex.blocks;
+  if (entries == 1) {
+    *mean = mw;
+    *m2 = sq;
+    return;
+  }
+  const float2* set = reinterpret_cast<const float2*>(ex.share(lane == 0 ? mw : sq, lane));
+  float m = 0.0f, q = 0.0f;
+  if (entries <= 4) {
+    // few words: every thread adds them all
+    for (int e = 0; e < entries; ++e) {
+      const float2 w = set[e];
+      m += w.x * count(e / ex.warps, e % ex.warps);
+      q += w.y;
+    }
+    m *= inv_d;
+    if (a.center)
+      for (int e = 0; e < entries; ++e) {
+        const float off = set[e].x - m;
+        q += off * off * count(e / ex.warps, e % ex.warps);
+      }
+  } else if (!a.center) {
+    for (int e = lane; e < entries; e += 32) q += set[e].y;
+    q = warp_sum(q);
+  } else {
+    for (int e = lane; e < entries; e += 32) m += set[e].x * count(e / ex.warps, e % ex.warps);
+    m = warp_sum(m) * inv_d;
+    for (int e = lane; e < entries; e += 32) {
+      const float2 w = set[e];
+      q += w.y + (w.x - m) * (w.x - m) * count(e / ex.warps, e % ex.warps);
+    }
+    q = warp_sum(q);
+  }
+  *mean = m;
+  *m2 = q;
+}
+
+// kN sums at once (kN 4 or 8): a warp halves the number of values a lane carries
+// with every exchange, so eight sums take nine shuffles instead of forty.
 template <int kN>
-__device__ __forceinline__ float warp_sums(float (&v)[kN]) {
+__device__ __forceinline__ void row_sums(float (&v)[kN], Exchange<kN>& ex) {
   const int lane = threadIdx.x & 31;
   int off = 16;
 #pragma unroll
@@ -163,111 +385,113 @@ __device__ __forceinline__ float warp_sums(float (&v)[kN]) {
       v[i] = keep + __shfl_xor_sync(0xffffffffu, give, off);
     }
   }
-  float r = v[0];
-  for (; off > 0; off >>= 1) r += __shfl_xor_sync(0xffffffffu, r, off);
-  return r;  // lane l holds the sum whose index is its top log2(kN) bits
-}
-
-// The kN sums of the block in every thread; red: 2 x 32 x kN words, in turn.
-template <int kN>
-__device__ __forceinline__ void block_sums(float (&v)[kN], float* red, int& turn) {
-  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  constexpr int kSpan = 32 / kN;  // lanes that hold one sum
-  const float mine = warp_sums<kN>(v);
-  if (warps == 1) {
+  float mine = v[0];
 #pragma unroll
-    for (int i = 0; i < kN; ++i) v[i] = __shfl_sync(0xffffffffu, mine, i * kSpan);
-    return;
+  for (int o = 16 / kN; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  // lane l holds the sum whose number is its top log2(kN) bits: bring sum k to lane k
+  mine = __shfl_sync(0xffffffffu, mine, (lane % kN) * (32 / kN));
+  const int entries = ex.warps * ex.blocks;
+  if (entries > 1) {
+    const float* set = ex.share(mine, lane);
+    float s = 0.0f;
+    for (int e = lane / kN; e < entries; e += 32 / kN) s += set[e * kN + lane % kN];
+#pragma unroll
+    for (int o = kN; o < 32; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    mine = s;
   }
-  float* set = red + (turn & 1) * 32 * kN;
-  ++turn;
-  if (lane % kSpan == 0) set[(threadIdx.x >> 5) * kN + lane / kSpan] = mine;
-  __syncthreads();
-  // warp w's sum i at set[w kN + i]: every lane adds one index over some warps, then exchanges
-  const int i = lane % kN;
-  float s = 0.0f;
-  for (int w = lane / kN; w < warps; w += kSpan) s += set[w * kN + i];
 #pragma unroll
-  for (int off = kN; off < 32; off <<= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
-#pragma unroll
-  for (int k = 0; k < kN; ++k) v[k] = __shfl_sync(0xffffffffu, s, k);
+  for (int k = 0; k < kN; ++k) v[k] = __shfl_sync(0xffffffffu, mine, k);
 }
 
 // ------------------------------------------------------------------ forward
 
-template <typename T, bool kVec, bool kPost>
-__global__ void __launch_bounds__(1024) norm_forward_kernel(const NormArgs a, const NormForward o) {
-  __shared__ float red[64];
-  Reducer r{red};
+// Dynamic shared memory: exchange words, then the streams' slots.
+template <typename T, int kA, bool kPost>
+__global__ void __launch_bounds__(kThreads)
+    norm_forward_kernel(const NormArgs a, const NormForward o, const int blocks, const int stages) {
+  extern __shared__ __align__(16) unsigned char shared[];
+  constexpr int kP = kRowPairs;
+  using Rows = Stream<T, kA, kP>;
+  const int rank = blocks == 1 ? 0 : static_cast<int>(cluster_ctarank());
+  const Span s = span_of(a, rank, blocks);
+  Exchange<2> ex{reinterpret_cast<float*>(shared), rank, blocks, static_cast<int>(blockDim.x >> 5)};
+  const int words = Rows::words_of(s.columns_of(0));
+  uint4* slots = reinterpret_cast<uint4*>(shared + exchange_bytes(2));
+  const Rows sx{static_cast<const T*>(a.x), a.ldx, slots, words};
+  const Rows sy{static_cast<const T*>(a.y), a.ldy, slots + stages * words, words};
   const float inv_d = 1.0f / static_cast<float>(a.d);
-  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    Elems<T, kVec> ex, ey;
-    ex.load(static_cast<const T*>(a.x) + row * a.ldx, a.d);
-    if (a.y != nullptr) ey.load(static_cast<const T*>(a.y) + row * a.ldy, a.d);
-    float h[kE], q[kE];
-    ex.get(h, a.d);
-    float my = 0.0f, ry = 1.0f;
+  const long long first = blockIdx.x / blocks, step = gridDim.x / blocks;
+  const int ahead = stages - 1;
+  auto fetch = [&](long long row, int stage) {
+    if (row < a.rows) {
+      sx.fetch(row, stage, s);
+      if (a.y != nullptr) sy.fetch(row, stage, s);
+    }
+    copy_commit();
+  };
+  for (int k = 0; k < ahead; ++k) fetch(first + k * step, k);
+  // column vectors in registers: t = gate pw, u = gate pb (t = gate without post), formed anew where the gate's
+  // row changes
+  Pair t[kP], u[kP], w[kP], b[kP];
+  param<T, kA>(a.w, 0, 1.0f, w, s);
+  param<T, kA>(a.b, 0, 0.0f, b, s);
+  long long gate_at = -1;
+  if (blocks > 1) cluster_sync();  // every block runs before one writes another's words
+  int stage = 0;
+  for (long long row = first; row < a.rows; row += step) {
     if (a.y != nullptr) {
-      float p[kE];
-      ey.get(p, a.d);
+      const long long g = gate_row(a, row);
+      if (g != gate_at) {
+        gate_at = g;
+        param<T, kA>(a.gate, g * a.d, 1.0f, t, s);
+        if (kPost) {
+          param<T, kA>(a.pb, 0, 0.0f, u, s);
+#pragma unroll
+          for (int i = 0; i < kP; ++i) u[i] = mul2(u[i], t[i]);
+          times<T, kA>(a.pw, 0, t, s);
+        }
+      }
+    }
+    wait_row(stages);
+    if (kA == kAny) __syncthreads();
+    Pair h[kP], p[kP];
+    sx.read(row, stage, s, h);
+    float my = 0.0f, ry = 1.0f, m2;
+    if (a.y != nullptr) sy.read(row, stage, s, p);
+    // the slot read a row ago; with kAny every thread has read it before the barrier above
+    fetch(row + ahead * step, stage == 0 ? ahead : stage - 1);
+    if (a.y != nullptr) {
+      const Pair scale = pair(a.scale);
       if (kPost) {
-        if (a.center) {
-          float s = 0.0f;
 #pragma unroll
-          for (int i = 0; i < kE; ++i) s += p[i];
-          my = r.sum(s) * inv_d;
-        }
-        float s = 0.0f;
+        for (int i = 0; i < kP; ++i) p[i] = only<kA>(p[i], i, s);
+        row_stats<kA>(p, s, a, inv_d, ex, &my, &m2);
+        ry = rsqrtf(m2 * inv_d + a.eps);
+        const Pair off = pair(-my), unit = pair(ry);
 #pragma unroll
-        for (int i = 0; i < kE; ++i) {
-          p[i] = column<kVec>(i) < a.d ? p[i] - my : 0.0f;
-          s += p[i] * p[i];
-        }
-        ry = 1.0f / sqrtf(r.sum(s) * inv_d + a.eps);
-        param<T, kVec>(a.pw, 0, 1.0f, q, a.d);
+        for (int i = 0; i < kP; ++i)
+          h[i] = fma2(scale, h[i], fma2(mul2(add2(p[i], off), unit), t[i], u[i]));
+      } else {
 #pragma unroll
-        for (int i = 0; i < kE; ++i) p[i] = p[i] * ry * q[i];
-        if (a.pb.p != nullptr) {
-          param<T, kVec>(a.pb, 0, 0.0f, q, a.d);
-#pragma unroll
-          for (int i = 0; i < kE; ++i) p[i] += q[i];
-        }
+        for (int i = 0; i < kP; ++i) h[i] = fma2(scale, h[i], mul2(p[i], t[i]));
       }
-      if (a.gate.p != nullptr) {
-        param<T, kVec>(a.gate, gate_row(a, row) * a.d, 1.0f, q, a.d);
-#pragma unroll
-        for (int i = 0; i < kE; ++i) p[i] *= q[i];
-      }
-#pragma unroll
-      for (int i = 0; i < kE; ++i) h[i] = a.scale * h[i] + p[i];
-      put<T, kVec>(static_cast<T*>(o.h) + row * a.d, h, a.d);
+      put<T, kA>(static_cast<T*>(o.h) + row * a.d, h, s);
     }
-    float mh = 0.0f;
-    if (a.center) {
-      float s = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kE; ++i) s += column<kVec>(i) < a.d ? h[i] : 0.0f;
-      mh = r.sum(s) * inv_d;
-    }
-    float s = 0.0f;
+    for (int i = 0; i < kP; ++i) h[i] = only<kA>(h[i], i, s);
+    float mh;
+    row_stats<kA>(h, s, a, inv_d, ex, &mh, &m2);
+    const float rh = rsqrtf(m2 * inv_d + a.eps);
+    const Pair off = pair(-mh), unit = pair(rh);
 #pragma unroll
-    for (int i = 0; i < kE; ++i) {
-      h[i] = column<kVec>(i) < a.d ? h[i] - mh : 0.0f;
-      s += h[i] * h[i];
-    }
-    const float rh = 1.0f / sqrtf(r.sum(s) * inv_d + a.eps);
-    param<T, kVec>(a.w, 0, 1.0f, q, a.d);
-#pragma unroll
-    for (int i = 0; i < kE; ++i) h[i] = h[i] * rh * q[i];
-    if (a.b.p != nullptr) {
-      param<T, kVec>(a.b, 0, 0.0f, q, a.d);
-#pragma unroll
-      for (int i = 0; i < kE; ++i) h[i] += q[i];
-    }
-    put<T, kVec>(static_cast<T*>(o.n) + row * a.d, h, a.d);
-    if (o.stats != nullptr && threadIdx.x == 0)
+    for (int i = 0; i < kP; ++i) h[i] = fma2(mul2(add2(h[i], off), unit), w[i], b[i]);
+    put<T, kA>(static_cast<T*>(o.n) + row * a.d, h, s);
+    if (o.stats != nullptr && threadIdx.x == 0 && rank == 0)
       reinterpret_cast<float4*>(o.stats)[row] = make_float4(my, ry, mh, rh);
+    stage = stage == ahead ? 0 : stage + 1;
   }
+  copy_wait<0>();
+  if (blocks > 1) cluster_sync();  // no block leaves while another may still write its words
 }
 
 // Row of any width: several passes through the caches.
@@ -333,227 +557,264 @@ __device__ __forceinline__ void unit_rows(const NormArgs& a, const NormPlan& p, 
   *last = slice * p.len + p.len < per ? *first + p.len : (group + 1) * per;
 }
 
-// Column sums of a thread: kFull 0: S1 (of D yh), W1 (of dn hh); 1: S0, W0 as well.
-// In registers, or in shared memory [sum][column].
-template <int kSums, bool kShared>
+// A thread's column sums in registers, or in shared memory [sum][two pairs][thread].
+template <int kSums, int kP, bool kShared>
 struct Sums {
-  float acc[kShared ? 1 : kSums][kE];
-  float* mem;
-  long long d;
-  __device__ __forceinline__ void init(float* shared, long long d_) {
-    mem = shared;
-    d = d_;
-    if (kShared) {
-      for (long long i = threadIdx.x; i < kSums * d; i += blockDim.x) mem[i] = 0.0f;
-      __syncthreads();
-    } else {
-#pragma unroll
-      for (int k = 0; k < kSums; ++k)
-#pragma unroll
-        for (int i = 0; i < kE; ++i) acc[kShared ? 0 : k][i] = 0.0f;
-    }
+  Pair acc[kShared ? 1 : kSums][kP];
+  ulonglong2* mem;
+  __device__ __forceinline__ ulonglong2* at(int k, int q) const {
+    return mem + (k * (kP / 2) + q) * blockDim.x + threadIdx.x;
   }
-  template <bool kVec>
-  __device__ __forceinline__ void add(int k, const float (&v)[kE]) {
-    if (!kShared) {
-#pragma unroll
-      for (int i = 0; i < kE; ++i) acc[kShared ? 0 : k][i] += v[i];
-    } else if (kVec) {
-      const long long c = column<true>(0);
-      if (c < d) {
-        float4* m = reinterpret_cast<float4*>(mem + k * d + c);
-        float4 u = m[0], w = m[1];
-        u.x += v[0], u.y += v[1], u.z += v[2], u.w += v[3];
-        w.x += v[4], w.y += v[5], w.z += v[6], w.w += v[7];
-        m[0] = u;
-        m[1] = w;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kE; ++i)
-        if (column<false>(i) < d) mem[k * d + column<false>(i)] += v[i];
-    }
-  }
-  template <bool kVec>
-  __device__ __forceinline__ void flush(float* ws) {
+  __device__ __forceinline__ void init(void* shared) {
+    mem = static_cast<ulonglong2*>(shared);
 #pragma unroll
     for (int k = 0; k < kSums; ++k) {
       if (kShared) {
 #pragma unroll
-        for (int i = 0; i < kE; ++i)
-          if (column<kVec>(i) < d) ws[k * d + column<kVec>(i)] = mem[k * d + column<kVec>(i)];
+        for (int q = 0; q < kP / 2; ++q) *at(k, q) = make_ulonglong2(0ull, 0ull);
       } else {
-        put<float, kVec>(ws + k * d, acc[kShared ? 0 : k], d);
+#pragma unroll
+        for (int i = 0; i < kP; ++i) acc[kShared ? 0 : k][i] = 0ull;
       }
+    }
+  }
+  // sum k += v w
+  __device__ __forceinline__ void add(int k, const Pair (&v)[kP], const Pair (&w)[kP]) {
+    if (kShared) {
+#pragma unroll
+      for (int q = 0; q < kP / 2; ++q) {
+        const ulonglong2 m = *at(k, q);
+        *at(k, q) = make_ulonglong2(fma2(v[2 * q], w[2 * q], m.x), fma2(v[2 * q + 1], w[2 * q + 1], m.y));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kP; ++i) acc[kShared ? 0 : k][i] = fma2(v[i], w[i], acc[kShared ? 0 : k][i]);
+    }
+  }
+  __device__ __forceinline__ void add(int k, const Pair (&v)[kP]) {
+    if (kShared) {
+#pragma unroll
+      for (int q = 0; q < kP / 2; ++q) {
+        const ulonglong2 m = *at(k, q);
+        *at(k, q) = make_ulonglong2(add2(v[2 * q], m.x), add2(v[2 * q + 1], m.y));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kP; ++i) acc[kShared ? 0 : k][i] = add2(v[i], acc[kShared ? 0 : k][i]);
+    }
+  }
+  template <int kA>
+  __device__ __forceinline__ void flush(float* ws, long long d, const Span& s) const {
+#pragma unroll
+    for (int k = 0; k < kSums; ++k) {
+      Pair v[kP];
+#pragma unroll
+      for (int q = 0; q < kP / 2; ++q) {
+        if (kShared) {
+          const ulonglong2 m = *at(k, q);
+          v[2 * q] = m.x;
+          v[2 * q + 1] = m.y;
+        } else {
+          v[2 * q] = acc[kShared ? 0 : k][2 * q];
+          v[2 * q + 1] = acc[kShared ? 0 : k][2 * q + 1];
+        }
+      }
+      put<float, kA>(ws + k * d, v, s);
     }
   }
 };
 
-template <typename T, bool kVec, bool kPost, bool kFull, bool kShared>
-__global__ void __launch_bounds__(kShared ? 1024 : kRegSums / kE)
-    norm_backward_kernel(const NormArgs a, const NormPlan plan, const NormBackward o) {
-  extern __shared__ float shared[];
+// Sums: 0 S1 (of D yh, or of gate D yh), 1 W1 (dn hh); kFull: 2 S0, 3 W0 as well.
+// kShared: twice the columns a thread, and their sums in shared memory.
+template <typename T, int kA, bool kPost, bool kFull, bool kShared>
+__global__ void __launch_bounds__(kThreads)
+    norm_backward_kernel(const NormArgs a, const NormPlan plan, const NormBackward o, const int blocks,
+                         const int stages) {
+  extern __shared__ __align__(16) unsigned char shared[];
   constexpr int kN = kFull ? 8 : 4;
   constexpr int kSums = kFull ? 4 : 2;
-  float* red = shared;  // 2 x 32 x kN
-  Sums<kSums, kShared> sums;
-  sums.init(shared + 64 * kN, a.d);
-  const bool want = o.ws != nullptr;
-  int turn = 0;
+  constexpr int kP = kShared ? kRowPairs : kRowPairs / 2;
+  using Rows = Stream<T, kA, kP>;
+  const int rank = blocks == 1 ? 0 : static_cast<int>(cluster_ctarank());
+  const Span s = span_of(a, rank, blocks);
+  Exchange<kN> ex{reinterpret_cast<float*>(shared), rank, blocks, static_cast<int>(blockDim.x >> 5)};
+  Sums<kSums, kP, kShared> sums;
+  sums.init(shared + exchange_bytes(kN));
+  const int words = Rows::words_of(s.columns_of(0));
+  uint4* slots = reinterpret_cast<uint4*>(shared + exchange_bytes(kN)) + (kShared ? kSums * (kP / 2) * blockDim.x : 0);
+  const Rows sx{static_cast<const T*>(a.x), a.ldx, slots, words};
+  const Rows sy{static_cast<const T*>(a.y), a.ldy, slots + stages * words, words};
+  const Rows sh{static_cast<const T*>(o.dh), a.d, slots + 2 * stages * words, words};
+  const Rows sn{static_cast<const T*>(o.dn), a.d, slots + 3 * stages * words, words};
   const float inv_d = 1.0f / static_cast<float>(a.d);
+  const long long unit = blockIdx.x / blocks;
   long long first, last;
-  unit_rows(a, plan, blockIdx.x, &first, &last);
-  for (long long row = first; row < last; ++row) {
-    Elems<T, kVec> ex, ey, eh, en;
-    ex.load(static_cast<const T*>(a.x) + row * a.ldx, a.d);
-    if (a.y != nullptr) ey.load(static_cast<const T*>(a.y) + row * a.ldy, a.d);
-    if (o.dh != nullptr) eh.load(static_cast<const T*>(o.dh) + row * a.d, a.d);
-    if (o.dn != nullptr) en.load(static_cast<const T*>(o.dn) + row * a.d, a.d);
-    const float4 st = reinterpret_cast<const float4*>(o.stats)[row];
-    float x[kE], yh[kE], g[kE], t[kE], u[kE], q[kE];
-    ex.get(x, a.d);
-#pragma unroll
-    for (int i = 0; i < kE; ++i) yh[i] = 0.0f;
-    param<T, kVec>(a.gate, gate_row(a, row) * a.d, 1.0f, g, a.d);
-    // x becomes hh; t = gate pw
-#pragma unroll
-    for (int i = 0; i < kE; ++i) t[i] = g[i];
-    if (a.y != nullptr) {
-      ey.get(yh, a.d);
-      float p[kE];
-      if (kPost) {
-        param<T, kVec>(a.pw, 0, 1.0f, q, a.d);
-#pragma unroll
-        for (int i = 0; i < kE; ++i) {
-          yh[i] = column<kVec>(i) < a.d ? (yh[i] - st.x) * st.y : 0.0f;
-          t[i] *= q[i];
-          p[i] = yh[i] * q[i];
-        }
-        if (kFull && a.pb.p != nullptr) {
-          param<T, kVec>(a.pb, 0, 0.0f, q, a.d);
-#pragma unroll
-          for (int i = 0; i < kE; ++i) p[i] += q[i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < kE; ++i) p[i] = yh[i];
-      }
-#pragma unroll
-      for (int i = 0; i < kE; ++i) x[i] = a.scale * x[i] + g[i] * p[i];
+  unit_rows(a, plan, unit, &first, &last);
+  auto fetch = [&](long long row, int stage) {
+    if (row < last) {
+      sx.fetch(row, stage, s);
+      if (a.y != nullptr) sy.fetch(row, stage, s);
+      if (o.dh != nullptr) sh.fetch(row, stage, s);
+      if (o.dn != nullptr) sn.fetch(row, stage, s);
     }
+    copy_commit();
+  };
+  // with one stage the next row goes to the slot just read
+  const int ahead = stages > 1 ? stages - 1 : 1;
+  for (int k = 0; k < ahead; ++k) fetch(first + k, k);
+  const Pair scale = pair(a.scale);
+  if (blocks > 1) cluster_sync();  // every block runs before one writes another's words
+  int stage = 0;
+  for (long long row = first; row < last; ++row) {
+    const float4 st = reinterpret_cast<const float4*>(o.stats)[row];
+    const long long g0 = gate_row(a, row) * a.d;
+    wait_row(stages);
+    if (kA == kAny) __syncthreads();
+    Pair hh[kP], yh[kP], t[kP], u[kP];
+    Pair v[kN];
 #pragma unroll
-    for (int i = 0; i < kE; ++i) x[i] = column<kVec>(i) < a.d ? (x[i] - st.z) * st.w : 0.0f;
-    // u = dh + r_h gn; q = gn
-    if (o.dn != nullptr) {
-      float dn[kE];
-      en.get(dn, a.d);
-      param<T, kVec>(a.w, 0, 1.0f, q, a.d);
-      if (want) {
-        if (kFull) sums.template add<kVec>(3, dn);
+    for (int k = 0; k < kN; ++k) v[k] = 0ull;
+    sx.read(row, stage, s, hh);
+    param<T, kA>(a.gate, g0, 1.0f, t, s);  // t: the gate; with kPost times pw
+    if (a.y != nullptr) {
+      sy.read(row, stage, s, yh);
 #pragma unroll
-        for (int i = 0; i < kE; ++i) u[i] = dn[i] * x[i];
-        sums.template add<kVec>(1, u);
+      for (int i = 0; i < kP; ++i) hh[i] = mul2(hh[i], scale);
+      if (kPost) {
+        if (kFull && a.pb.p != nullptr) {
+          param<T, kA>(a.pb, 0, 0.0f, u, s);
+#pragma unroll
+          for (int i = 0; i < kP; ++i) hh[i] = fma2(t[i], u[i], hh[i]);
+        }
+        times<T, kA>(a.pw, 0, t, s);
+        const Pair off = pair(-st.x), unit_y = pair(st.y);
+#pragma unroll
+        for (int i = 0; i < kP; ++i) yh[i] = only<kA>(mul2(add2(yh[i], off), unit_y), i, s);
       }
 #pragma unroll
-      for (int i = 0; i < kE; ++i) q[i] *= dn[i];
+      for (int i = 0; i < kP; ++i) hh[i] = fma2(t[i], yh[i], hh[i]);
     } else {
+      fill(yh, 0.0f);
+    }
+    const Pair rh = pair(st.w);
+    {
+      const Pair off = pair(-st.z);
 #pragma unroll
-      for (int i = 0; i < kE; ++i) q[i] = 0.0f;
+      for (int i = 0; i < kP; ++i) hh[i] = only<kA>(mul2(add2(hh[i], off), rh), i, s);
     }
     if (o.dh != nullptr) {
-      eh.get(u, a.d);
+      sh.read(row, stage, s, u);
+#pragma unroll
+      for (int i = 0; i < kP; ++i) u[i] = only<kA>(u[i], i, s);
     } else {
-#pragma unroll
-      for (int i = 0; i < kE; ++i) u[i] = 0.0f;
+      fill(u, 0.0f);
     }
-    float v[kN];
+    if (o.dn != nullptr) {
+      Pair dn[kP];
+      sn.read(row, stage, s, dn);
 #pragma unroll
-    for (int k = 0; k < kN; ++k) v[k] = 0.0f;
+      for (int i = 0; i < kP; ++i) dn[i] = only<kA>(dn[i], i, s);
+      sums.add(1, dn, hh);
+      if constexpr (kFull) sums.add(3, dn);
+      times<T, kA>(a.w, 0, dn, s);
 #pragma unroll
-    for (int i = 0; i < kE; ++i) {
-      u[i] += st.w * q[i];
-      v[0] += q[i] * x[i];
-      if (kPost) {
-        const float A = t[i] * u[i], B = t[i] * st.w;
-        v[1] += A * yh[i];
-        v[2] += B * x[i] * yh[i];
+      for (int i = 0; i < kP; ++i) {
+        u[i] = fma2(rh, dn[i], u[i]);  // dh + r_h gn
+        v[0] = fma2(dn[i], hh[i], v[0]);
+        if constexpr (kFull) v[3] = add2(v[3], dn[i]);
+      }
+    }
+    if (kA == kAny && stages == 1) __syncthreads();  // every thread has read the slot
+    // the slot read a row ago (a barrier lies between, or it is the thread's own); one stage: this row's, read above
+    fetch(row + ahead, stages == 1 ? 0 : (stage == 0 ? ahead : stage - 1));
+    if (kPost) {
+#pragma unroll
+      for (int i = 0; i < kP; ++i) {
+        const Pair A = mul2(t[i], u[i]), B = only<kA>(mul2(t[i], rh), i, s), C = mul2(B, hh[i]);
+        v[1] = fma2(A, yh[i], v[1]);
+        v[2] = fma2(C, yh[i], v[2]);
         if constexpr (kFull) {
-          v[4] += A;
-          v[5] += B;
-          v[6] += B * x[i];
-          v[7] += B * yh[i];
+          v[4] = add2(v[4], A);
+          v[5] = add2(v[5], B);
+          v[6] = add2(v[6], C);
+          v[7] = fma2(B, yh[i], v[7]);
         }
       }
-      if constexpr (kFull) v[3] += q[i];
     }
-    block_sums<kN>(v, red, turn);
-    const float m2 = v[0] * inv_d;
-    const float m1 = kFull && a.center ? v[3] * inv_d : 0.0f;
-    // u becomes D
+    float e[kN];
 #pragma unroll
-    for (int i = 0; i < kE; ++i) u[i] = column<kVec>(i) < a.d ? u[i] - st.w * (m1 + m2 * x[i]) : 0.0f;
+    for (int k = 0; k < kN; ++k) e[k] = lo_of(v[k]) + hi_of(v[k]);
+    row_sums<kN>(e, ex);
+#pragma unroll
+    for (int k = 0; k < kN; ++k) e[k] *= inv_d;
+    const float m2 = e[0];
+    float m1 = 0.0f;
+    if constexpr (kFull) m1 = a.center ? e[3] : 0.0f;
+    // u becomes D
+    {
+      const Pair c1 = pair(-st.w * m1), c2 = pair(-st.w * m2);
+#pragma unroll
+      for (int i = 0; i < kP; ++i) u[i] = only<kA>(fma2(c2, hh[i], add2(u[i], c1)), i, s);
+    }
     if (o.dx != nullptr) {
 #pragma unroll
-      for (int i = 0; i < kE; ++i) q[i] = a.scale * u[i];
-      put<T, kVec>(static_cast<T*>(o.dx) + row * a.d, q, a.d);
+      for (int i = 0; i < kP; ++i) hh[i] = mul2(scale, u[i]);
+      put<T, kA>(static_cast<T*>(o.dx) + row * a.d, hh, s);
     }
-    if (a.y == nullptr) continue;
-    if (want) {
-      if (plan.grouped) {
-        if (kFull) sums.template add<kVec>(2, u);
+    if (a.y != nullptr) {
+      if (plan.grouped || a.gate.p == nullptr) {
+        sums.add(0, u, yh);
+        if constexpr (kFull) sums.add(2, u);
+      } else if (kPost) {
+        Pair gd[kP];
 #pragma unroll
-        for (int i = 0; i < kE; ++i) q[i] = u[i] * yh[i];
-        sums.template add<kVec>(0, q);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kE; ++i) q[i] = u[i] * g[i];
-        if (kFull) sums.template add<kVec>(2, q);
-#pragma unroll
-        for (int i = 0; i < kE; ++i) q[i] *= yh[i];
-        sums.template add<kVec>(0, q);
+        for (int i = 0; i < kP; ++i) gd[i] = u[i];
+        times<T, kA>(a.gate, g0, gd, s);
+        sums.add(0, gd, yh);
+        if constexpr (kFull) sums.add(2, gd);
       }
-    }
-    if (o.dgate_rows != nullptr) {
-      // D p, with p formed again
+      if (o.dgate_rows != nullptr) {
 #pragma unroll
-      for (int i = 0; i < kE; ++i) q[i] = yh[i];
-      if (kPost) {
-        float pw[kE];
-        param<T, kVec>(a.pw, 0, 1.0f, pw, a.d);
+        for (int i = 0; i < kP; ++i) hh[i] = yh[i];
+        if (kPost) {
+          times<T, kA>(a.pw, 0, hh, s);
+          if (kFull && a.pb.p != nullptr) {
+            Pair c[kP];
+            param<T, kA>(a.pb, 0, 0.0f, c, s);
 #pragma unroll
-        for (int i = 0; i < kE; ++i) q[i] *= pw[i];
-        if (kFull && a.pb.p != nullptr) {
-          param<T, kVec>(a.pb, 0, 0.0f, pw, a.d);
-#pragma unroll
-          for (int i = 0; i < kE; ++i) q[i] += pw[i];
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < kE; ++i) q[i] *= u[i];
-      if (o.dgate_f32)
-        put<float, kVec>(static_cast<float*>(o.dgate_rows) + row * a.d, q, a.d);
-      else
-        put<T, kVec>(static_cast<T*>(o.dgate_rows) + row * a.d, q, a.d);
-    }
-    if (o.dy != nullptr) {
-      if (kPost) {
-        float e2 = (v[1] - m2 * v[2]) * inv_d, e1 = 0.0f;
-        if constexpr (kFull) {
-          if (a.center) {
-            e2 -= m1 * v[7] * inv_d;
-            e1 = (v[4] - m1 * v[5] - m2 * v[6]) * inv_d;
+            for (int i = 0; i < kP; ++i) hh[i] = add2(hh[i], c[i]);
           }
         }
 #pragma unroll
-        for (int i = 0; i < kE; ++i) q[i] = st.y * (t[i] * u[i] - e1 - yh[i] * e2);
-      } else {
-#pragma unroll
-        for (int i = 0; i < kE; ++i) q[i] = g[i] * u[i];
+        for (int i = 0; i < kP; ++i) hh[i] = mul2(hh[i], u[i]);
+        if (o.dgate_f32)
+          put<float, kA>(static_cast<float*>(o.dgate_rows) + row * a.d, hh, s);
+        else
+          put<T, kA>(static_cast<T*>(o.dgate_rows) + row * a.d, hh, s);
       }
-      put<T, kVec>(static_cast<T*>(o.dy) + row * a.d, q, a.d);
+      if (o.dy != nullptr) {
+#pragma unroll
+        for (int i = 0; i < kP; ++i) u[i] = mul2(t[i], u[i]);
+        if (kPost) {
+          float e2 = e[1] - m2 * e[2], e1 = 0.0f;
+          if constexpr (kFull) {
+            if (a.center) {
+              e2 -= m1 * e[7];
+              e1 = e[4] - m1 * e[5] - m2 * e[6];
+            }
+          }
+          const Pair c1 = pair(-e1), c2 = pair(-e2), unit_y = pair(st.y);
+#pragma unroll
+          for (int i = 0; i < kP; ++i) u[i] = mul2(unit_y, fma2(c2, yh[i], add2(u[i], c1)));
+        }
+        put<T, kA>(static_cast<T*>(o.dy) + row * a.d, u, s);
+      }
     }
+    if (stages > 1) stage = stage == ahead ? 0 : stage + 1;
   }
-  if (want) sums.template flush<kVec>(o.ws + blockIdx.x * static_cast<long long>(kSums) * a.d);
+  if (o.ws != nullptr) sums.template flush<kA>(o.ws + unit * static_cast<long long>(kSums) * a.d, a.d, s);
+  copy_wait<0>();
+  if (blocks > 1) cluster_sync();  // no block leaves while another may still write its words
 }
 
 // Terms of one element, for the several-pass kernels.
@@ -651,9 +912,6 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// The units' sums to gradients: block (tile of 32 columns, y): y = 0 the
-// parameters, y = 1 + group the gate's row.  32 threads walk the columns, 32 the
-// units; fixed order.
 __device__ __forceinline__ void put1(void* p, int f32, int dtype, long long i, float v) {
   if (f32)
     static_cast<float*>(p)[i] = v;
@@ -665,58 +923,90 @@ __device__ __forceinline__ void put1(void* p, int f32, int dtype, long long i, f
     static_cast<float*>(p)[i] = v;
 }
 
+// The units' sums to gradients: block (tile of 32 columns, job).  Job 0: the
+// parameters, and the gate's row where it has one; then a job a gate row.  Eight
+// threads walk the columns four at a time, 128 the units; the order is fixed.
 template <typename T>
 __global__ void __launch_bounds__(1024)
-    norm_finish_kernel(const NormArgs a, const NormPlan plan, const float* ws, const NormSums o) {
+    norm_finish_kernel(const NormArgs a, const NormPlan plan, const float* __restrict__ ws, const NormSums o) {
   __shared__ float part[4][32][33];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int quad = lane & 7;                       // columns 4 quad .. 4 quad + 3 of the tile
+  const int walker = w * 4 + (lane >> 3);
+  const long long c4 = blockIdx.x * 32ll + quad * 4;
   const long long c = blockIdx.x * 32ll + lane;
   const int n = plan.sums();
-  for (long long job = blockIdx.y; job <= (o.dgate != nullptr ? plan.groups : 0); job += gridDim.y) {
+  const bool vec = a.d % 4 == 0;
+  const long long jobs = o.dgate != nullptr && plan.groups > 1 ? 1 + plan.groups : 1;
+  for (long long job = blockIdx.y; job < jobs; job += gridDim.y) {
     const long long first = job == 0 ? 0 : (job - 1) * plan.slices;
     const long long last = job == 0 ? plan.units() : job * plan.slices;
-    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (c < a.d) {
-      for (long long unit = first + w; unit < last; unit += 32) {
-        const float* u = ws + unit * n * a.d + c;
-        const float g = job == 0 && plan.grouped ? param1<T>(a.gate, unit / plan.slices * a.d + c, 1.0f) : 1.0f;
-        s[0] += g * u[0];
-        s[1] += u[a.d];
-        if (n == 4) {
-          s[2] += g * u[2 * a.d];
-          s[3] += u[3 * a.d];
+    const bool weigh = job == 0 && plan.grouped && plan.groups > 1;  // with the gate of the unit's group
+    float s[4][4] = {};
+#pragma unroll 2
+    for (long long unit = first + walker; unit < last; unit += 128) {
+      float g[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+      if (weigh)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (c4 + j < a.d) g[j] = param1<T>(a.gate, unit / plan.slices * a.d + c4 + j, 1.0f);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (k >= n) break;
+        const float* u = ws + (unit * n + k) * a.d + c4;
+        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (vec) {
+          if (c4 < a.d) {
+            const float4 f = *reinterpret_cast<const float4*>(u);
+            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (c4 + j < a.d) v[j] = u[j];
         }
+        const bool gated = k == 0 || k == 2;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[k][j] += gated ? g[j] * v[j] : v[j];
       }
     }
     __syncthreads();  // the previous job's sums are read
 #pragma unroll
-    for (int k = 0; k < 4; ++k) part[k][w][lane] = s[k];
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float v = s[k][j];
+        v += __shfl_xor_sync(0xffffffffu, v, 8);
+        v += __shfl_xor_sync(0xffffffffu, v, 16);
+        if (lane < 8) part[k][w][quad * 4 + j] = v;
+      }
     __syncthreads();
     if (w < 4) {
       float v = 0.0f;
-#pragma unroll 8
+#pragma unroll
       for (int i = 0; i < 32; ++i) v += part[w][i][lane];
-      part[w][0][lane] = v;  // read and written by this warp alone
+      part[w][0][lane] = v;  // read and written by this thread alone
     }
     __syncthreads();
     if (w == 0 && c < a.d) {
       const float s1 = part[0][0][lane], w1 = part[1][0][lane], s0 = part[2][0][lane], w0 = part[3][0][lane];
       if (job == 0) {
+        // one group: the sums of D become those of gate D here
+        const float g = plan.grouped && plan.groups == 1 ? param1<T>(a.gate, c, 1.0f) : 1.0f;
         if (o.dw != nullptr) put1(o.dw, a.w.f32, a.dtype, c, w1);
         if (o.db != nullptr) put1(o.db, a.b.f32, a.dtype, c, w0);
-        if (o.dpw != nullptr) put1(o.dpw, a.pw.f32, a.dtype, c, s1);
-        if (o.dpb != nullptr) put1(o.dpb, a.pb.f32, a.dtype, c, s0);
-      } else {
+        if (o.dpw != nullptr) put1(o.dpw, a.pw.f32, a.dtype, c, g * s1);
+        if (o.dpb != nullptr) put1(o.dpb, a.pb.f32, a.dtype, c, g * s0);
+      }
+      if (o.dgate != nullptr && (job > 0 || plan.groups == 1)) {
         const float v = a.post ? param1<T>(a.pw, c, 1.0f) * s1 + (n == 4 ? param1<T>(a.pb, c, 0.0f) * s0 : 0.0f) : s1;
-        put1(o.dgate, a.gate.f32, a.dtype, (job - 1) * a.d + c, v);
+        put1(o.dgate, a.gate.f32, a.dtype, (job > 0 ? job - 1 : 0) * a.d + c, v);
       }
     }
   }
 }
 
 // ------------------------------------------------------------------ launches
-
-int threads_for(long long d) { return static_cast<int>(((d + kE - 1) / kE + 31) / 32 * 32); }
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
@@ -726,19 +1016,112 @@ bool vector_rows(const NormArgs& a) {
          aligned(a.b.p) && aligned(a.pw.p) && aligned(a.pb.p) && aligned(a.gate.p);
 }
 
-int sum_bytes(const NormArgs& a, const NormPlan& plan) {
-  return a.d > kRegSums ? static_cast<int>(plan.sums() * a.d * sizeof(float)) : 0;
+// Columns a block holds: 512 threads' of a 16-bit type; of fp32, whose rows take twice the shared memory beside
+// the shared sums, those with sums in registers.
+long long block_columns(const NormArgs& a) { return a.dtype == kDtypeF32 ? kRegSums : 2 * kRowPairs * kThreads; }
+
+// Blocks that share a row: one, or a cluster.
+int blocks_for(const NormArgs& a) { return static_cast<int>((a.d + block_columns(a) - 1) / block_columns(a)); }
+
+int threads_for(const NormArgs& a, int pairs) {
+  const int columns = columns_per_block(a.d, blocks_for(a));
+  return ((columns + 2 * pairs - 1) / (2 * pairs) + 31) / 32 * 32;
 }
 
-template <typename T, bool kVec, bool kPost>
+// Sums in registers up to 512 threads of four pairs.
+bool shared_sums(const NormArgs& a) { return columns_per_block(a.d, blocks_for(a)) > kRegSums; }
+int backward_pairs(const NormArgs& a) { return shared_sums(a) ? kRowPairs : kRowPairs / 2; }
+
+Access access_of(const NormArgs& a, int pairs, bool others_aligned) {
+  if (!vector_rows(a) || !others_aligned) return kAny;
+  return a.d == 2ll * pairs * threads_for(a, pairs) * blocks_for(a) ? kExact : kVec;
+}
+
+// Bytes of a row's slots in `streams` streams.
+int slot_bytes(const NormArgs& a, int pairs, bool vec, int streams) {
+  const int size = a.dtype == kDtypeF32 ? 4 : 2;
+  const long long per = columns_per_block(a.d, blocks_for(a));
+  const long long n = per < a.d ? per : a.d;
+  const long long words = vec ? static_cast<long long>(threads_for(a, pairs)) * (pairs / 4) * (size / 2) : (n * size + 15) / 16 + 1;
+  return static_cast<int>(streams * words * 16);
+}
+
+constexpr int kSharedBytes = 227 * 1024;
+
+// What the row kernels launch with.
+struct Launch {
+  int threads;
+  int fixed;      // bytes of the exchange words and shared sums
+  int stages;
+  int bytes;
+  long long resident;  // blocks an SM holds, about
+};
+
+Launch backward_launch(const NormArgs& a, const NormPlan& plan, bool vec) {
+  Launch l;
+  const bool shared = shared_sums(a);
+  const int pairs = backward_pairs(a);
+  const int threads = l.threads = threads_for(a, pairs);
+  l.fixed = exchange_bytes(plan.full ? 8 : 4) + (shared ? plan.sums() * pairs * 8 * threads : 0);
+  const int slot = slot_bytes(a, pairs, vec, 4);
+  const long long regs = plan.full || shared ? 128 : 112;
+  l.resident = 65536 / (regs * threads);
+  if (l.resident > 12) l.resident = 12;
+  if (l.resident < 1) l.resident = 1;
+  // as many rows in flight as an SM's shared memory allows its resident blocks, two at least where one block can
+  for (;; --l.resident) {
+    l.stages = static_cast<int>((kSharedBytes / l.resident - 1024 - l.fixed) / slot);
+    if (l.stages >= 2 || l.resident == 1) break;
+  }
+  if (l.stages > kMaxStages) l.stages = kMaxStages;
+  l.bytes = l.fixed + l.stages * slot;
+  return l;
+}
+
+Launch forward_launch(const NormArgs& a, bool vec) {
+  Launch l;
+  l.fixed = exchange_bytes(2);
+  const int slot = slot_bytes(a, kRowPairs, vec, 2);
+  const int threads = l.threads = threads_for(a, kRowPairs);
+  l.resident = 65536 / (128ll * threads);
+  if (l.resident < 1) l.resident = 1;
+  for (;; --l.resident) {
+    l.stages = static_cast<int>((kSharedBytes / l.resident - 1024 - l.fixed) / slot);
+    if (l.stages >= 3 || l.resident == 1) break;
+  }
+  if (l.stages > kMaxStages) l.stages = kMaxStages;
+  l.bytes = l.fixed + l.stages * slot;
+  return l;
+}
+
+template <class Kernel, class... Args>
+int launch_rows(Kernel kernel, long long units, const NormArgs& a, const Launch& l, cudaStream_t stream,
+                Args... args) {
+  cudaError_t e = cudaSuccess;
+  const int bytes = l.bytes;
+  if (bytes > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return static_cast<int>(e);
+  const int blocks = blocks_for(a);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(units * blocks));
+  cfg.blockDim = dim3(static_cast<unsigned>(l.threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(blocks);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = blocks > 1 ? 1 : 0;
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, a, args..., blocks, l.stages));
+}
+
+template <typename T, int kA, bool kPost>
 int forward_rows(const NormArgs& a, const NormForward& f, cudaStream_t stream) {
-  const int threads = threads_for(a.d);
-  // enough blocks to fill the SMs' 2048 threads (at most 32 blocks an SM), rows in turn
-  const long long per_sm = 2048 / threads < 32 ? 2048 / threads : 32;
-  const long long cap = a.sms * per_sm;
-  const int grid = static_cast<int>(a.rows < cap ? a.rows : cap);
-  norm_forward_kernel<T, kVec, kPost><<<grid, threads, 0, stream>>>(a, f);
-  return static_cast<int>(cudaGetLastError());
+  const Launch l = forward_launch(a, kA != kAny);
+  const long long cap = a.sms * l.resident / blocks_for(a);
+  return launch_rows(norm_forward_kernel<T, kA, kPost>, a.rows < cap ? a.rows : cap, a, l, stream, f);
 }
 
 template <typename T>
@@ -748,30 +1131,26 @@ int forward_type(const NormArgs& a, const NormForward& f, cudaStream_t stream) {
     norm_forward_wide_kernel<T><<<static_cast<int>(a.rows < cap ? a.rows : cap), kWideThreads, 0, stream>>>(a, f);
     return static_cast<int>(cudaGetLastError());
   }
-  const bool vec = vector_rows(a) && aligned(f.h) && aligned(f.n);
-  if (vec) return a.post ? forward_rows<T, true, true>(a, f, stream) : forward_rows<T, true, false>(a, f, stream);
-  return a.post ? forward_rows<T, false, true>(a, f, stream) : forward_rows<T, false, false>(a, f, stream);
-}
-
-template <typename T, bool kVec, bool kPost, bool kFull, bool kShared>
-int backward_rows(const NormArgs& a, const NormPlan& plan, const NormBackward& b, cudaStream_t stream) {
-  auto kernel = norm_backward_kernel<T, kVec, kPost, kFull, kShared>;
-  const int bytes = 64 * (kFull ? 8 : 4) * static_cast<int>(sizeof(float)) + (kShared ? sum_bytes(a, plan) : 0);
-  if (bytes > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e != cudaSuccess) return static_cast<int>(e);
+  switch (access_of(a, kRowPairs, aligned(f.h) && aligned(f.n))) {
+    case kExact:
+      return a.post ? forward_rows<T, kExact, true>(a, f, stream) : forward_rows<T, kExact, false>(a, f, stream);
+    case kVec:
+      return a.post ? forward_rows<T, kVec, true>(a, f, stream) : forward_rows<T, kVec, false>(a, f, stream);
+    default:
+      return a.post ? forward_rows<T, kAny, true>(a, f, stream) : forward_rows<T, kAny, false>(a, f, stream);
   }
-  kernel<<<static_cast<unsigned>(plan.units()), threads_for(a.d), bytes, stream>>>(a, plan, b);
-  return static_cast<int>(cudaGetLastError());
 }
 
-template <typename T, bool kVec, bool kPost>
+template <typename T, int kA, bool kPost>
 int backward_sums(const NormArgs& a, const NormPlan& plan, const NormBackward& b, cudaStream_t stream) {
-  if (a.d > kRegSums)
-    return plan.full ? backward_rows<T, kVec, kPost, true, true>(a, plan, b, stream)
-                     : backward_rows<T, kVec, kPost, false, true>(a, plan, b, stream);
-  return plan.full ? backward_rows<T, kVec, kPost, true, false>(a, plan, b, stream)
-                   : backward_rows<T, kVec, kPost, false, false>(a, plan, b, stream);
+  const Launch l = backward_launch(a, plan, kA != kAny);
+  const long long units = plan.units();
+  if (shared_sums(a))
+    return plan.full
+               ? launch_rows(norm_backward_kernel<T, kA, kPost, true, true>, units, a, l, stream, plan, b)
+               : launch_rows(norm_backward_kernel<T, kA, kPost, false, true>, units, a, l, stream, plan, b);
+  return plan.full ? launch_rows(norm_backward_kernel<T, kA, kPost, true, false>, units, a, l, stream, plan, b)
+                   : launch_rows(norm_backward_kernel<T, kA, kPost, false, false>, units, a, l, stream, plan, b);
 }
 
 template <typename T>
@@ -780,13 +1159,18 @@ int backward_type(const NormArgs& a, const NormPlan& plan, const NormBackward& b
   *launches = 1;
   int rc;
   if (norm_in_registers(a)) {
-    const bool vec = vector_rows(a) && aligned(b.dh) && aligned(b.dn) && aligned(b.dx) && aligned(b.dy) &&
-                     aligned(b.dgate_rows) && aligned(b.ws);
-    if (vec)
-      rc = a.post ? backward_sums<T, true, true>(a, plan, b, stream) : backward_sums<T, true, false>(a, plan, b, stream);
-    else
-      rc = a.post ? backward_sums<T, false, true>(a, plan, b, stream)
-                  : backward_sums<T, false, false>(a, plan, b, stream);
+    switch (access_of(a, backward_pairs(a), aligned(b.dh) && aligned(b.dn) && aligned(b.dx) && aligned(b.dy) &&
+                             aligned(b.dgate_rows) && aligned(b.ws))) {
+      case kExact:
+        rc = a.post ? backward_sums<T, kExact, true>(a, plan, b, stream)
+                    : backward_sums<T, kExact, false>(a, plan, b, stream);
+        break;
+      case kVec:
+        rc = a.post ? backward_sums<T, kVec, true>(a, plan, b, stream) : backward_sums<T, kVec, false>(a, plan, b, stream);
+        break;
+      default:
+        rc = a.post ? backward_sums<T, kAny, true>(a, plan, b, stream) : backward_sums<T, kAny, false>(a, plan, b, stream);
+    }
   } else {
     const long long cap = a.sms * 4ll;
     norm_backward_wide_kernel<T><<<static_cast<int>(a.rows < cap ? a.rows : cap), kWideThreads, 0, stream>>>(a, b);
@@ -800,7 +1184,7 @@ int backward_type(const NormArgs& a, const NormPlan& plan, const NormBackward& b
     }
   }
   if (rc != 0 || b.ws == nullptr) return rc;
-  const long long jobs = 1 + (s.dgate != nullptr ? plan.groups : 0);
+  const long long jobs = s.dgate != nullptr && plan.groups > 1 ? 1 + plan.groups : 1;
   const dim3 grid(static_cast<unsigned>((a.d + 31) / 32), static_cast<unsigned>(jobs < 65535 ? jobs : 65535));
   norm_finish_kernel<T><<<grid, 1024, 0, stream>>>(a, plan, b.ws, s);
   ++*launches;
@@ -809,7 +1193,7 @@ int backward_type(const NormArgs& a, const NormPlan& plan, const NormBackward& b
 
 }  // namespace
 
-bool norm_in_registers(const NormArgs& a) { return a.d <= kMaxD; }
+bool norm_in_registers(const NormArgs& a) { return a.d <= block_columns(a) * kMaxCluster; }
 
 NormPlan norm_plan(const NormArgs& a) {
   NormPlan p;
@@ -819,12 +1203,10 @@ NormPlan norm_plan(const NormArgs& a) {
   p.grouped = a.gate.p != nullptr && a.gate_inner * a.gate_count == a.rows && a.gate_inner >= kMinGroup;
   p.groups = p.grouped ? a.gate_count : 1;
   const long long per = a.rows / p.groups;
-  // resident blocks: about 96 registers a thread, or the shared sums' bytes
-  const int threads = a.d <= kMaxD ? threads_for(a.d) : kWideThreads;
-  long long per_sm = 65536 / (96ll * threads);
-  if (a.d > kRegSums) per_sm = 1;
-  if (per_sm > 16) per_sm = 16;
-  long long slices = a.sms * per_sm / p.groups;
+  // a unit a resident block (or cluster)
+  long long all = a.sms * 4ll;
+  if (norm_in_registers(a)) all = a.sms * backward_launch(a, p, vector_rows(a)).resident / blocks_for(a);
+  long long slices = all / p.groups;
   if (slices > per) slices = per;
   if (slices < 1) slices = 1;
   p.len = (per + slices - 1) / slices;

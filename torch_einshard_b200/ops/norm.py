@@ -20,6 +20,8 @@ run natively, everything else on torch.  An extension of this framework.
 """
 
 import math
+from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -32,10 +34,10 @@ from . import _native
 __all__ = ["einnorm"]
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_FLOATS = (*_TYPES, torch.float64)
 
 
-def _axes(formula, families, label):
-    formula, _ = cached_expand_axis_families(formula, families=families)
+def _axes(formula, label):
     spec = parse_sharding(f"{formula} -> {formula}")[0]
     if getattr(spec, "partials", ()):
         raise ValueError(f"einnorm does not take partial sums in {label}")
@@ -49,16 +51,78 @@ def _axes(formula, families, label):
     return list(spec.axes)
 
 
-def _written_out(axes, rank):
-    """Axis keys with the ellipsis replaced by one key per dimension it covers."""
-    width = rank - sum(1 for a in axes if not isinstance(a, EllipsisAxis))
+def _written_out(axes, width):
+    """Axis keys with the ellipsis replaced by one key for each of the ``width`` dimensions it covers."""
     out = []
     for a in axes:
         if isinstance(a, EllipsisAxis):
-            out.extend(("...", i) for i in range(max(width, 0)))
+            out.extend(("...", i) for i in range(width))
         else:
             out.append(a)
     return out
+
+
+@dataclass(frozen=True)
+class _Plan:
+    """What the formula and the shapes alone decide."""
+
+    place: int       # the normalised dimension
+    d: int
+    lead: tuple      # lengths of the others, in order
+    # the gate as [count, d], its row for a stream row r at (r // inner) % count: spread over d first
+    # (it lacks the axis), permuted, viewed and expanded to the run of axes it covers (None where not needed)
+    spread: bool = False
+    order: tuple = None
+    view: tuple = None
+    run: tuple = None
+    inner: int = 1
+    count: int = 1
+
+
+@lru_cache(maxsize=1024)
+def _plan(shard, axis, gate_axes, shape, gate_shape):
+    axes = _axes(shard, "the stream")
+    width = max(len(shape) - sum(1 for a in axes if not isinstance(a, EllipsisAxis)), 0)
+    keys = _written_out(axes, width)
+    if len(keys) != len(shape):
+        raise ValueError(f"The stream has {len(shape)} dimensions, {shard!r} names {len(axes)} axes")
+    found = [k for k in keys if not isinstance(k, tuple) and k.name == axis]
+    if not found:
+        raise ValueError(f"Axis {axis!r} is not among the stream's axes")
+    norm_key = found[0]
+    if not norm_key.local():
+        raise NotImplementedError(f"einnorm needs the normalised axis {axis!r} whole on every rank")
+    place = keys.index(norm_key)
+    d = shape[place]
+    if d == 0:
+        raise ValueError(f"The normalised axis {axis!r} is empty")
+    lead_keys, lead = keys[:place] + keys[place + 1:], shape[:place] + shape[place + 1:]
+    if gate_shape is None:
+        if gate_axes is not None:
+            raise ValueError("gate_axes without a gate")
+        return _Plan(place, d, lead)
+    if gate_axes is None:
+        raise ValueError("gate needs gate_axes")
+    gate_keys = _written_out(_axes(gate_axes, "the gate"), width) if gate_axes.strip() else []  # "": a scalar
+    if len(gate_keys) != len(gate_shape):
+        raise ValueError(f"The gate has {len(gate_shape)} dimensions, {gate_axes!r} names {len(gate_keys)} axes")
+    for k, size in zip(gate_keys, gate_shape):
+        if k not in keys:
+            raise ValueError(f"The gate's axis {k} is not one of the stream's")
+        if size != shape[keys.index(k)]:
+            raise ValueError(f"The gate's axis {k} has length {size}, the stream's {shape[keys.index(k)]}")
+    spread = norm_key not in gate_keys
+    if spread:
+        gate_keys = gate_keys + [norm_key]
+    order = tuple(gate_keys.index(k) for k in [k for k in lead_keys if k in gate_keys] + [norm_key])
+    # axes of length one change nothing; the others must cover a run of the stream's axes
+    places = [i for i, k in enumerate(lead_keys) if k in gate_keys and lead[i] != 1]
+    low, high = (places[0], places[-1] + 1) if places else (0, 0)
+    run = lead[low:high]
+    view = tuple(s if low + i in places else 1 for i, s in enumerate(run))
+    inner = math.prod(lead[high:]) if places else math.prod(lead)
+    return _Plan(place, d, lead, spread, None if order == tuple(range(len(order))) else order, view,
+                 None if view == run else run, inner, math.prod(run))
 
 
 def _check_like(t, x, name):
@@ -80,33 +144,21 @@ def _check_param(t, x, name):
         raise ValueError(f"{name} must be {x.dtype} or float32 on {x.device}, not {t.dtype} on {t.device}")
 
 
-def _gate_rows(gate, gate_keys, lead, shape, norm_key, d):
-    """The gate as [count, d] with its row for a stream row r at (r // inner) % count.
-
-    ``lead`` are the stream's other axes in order, ``shape`` their lengths.  Axes
-    the gate has must cover a run of them; where they do not, it is expanded to
-    the run around them (the gradient sums again, by autograd)."""
-    if norm_key not in gate_keys:
-        gate = gate.unsqueeze(-1).expand(*gate.shape, d)
-        gate_keys = gate_keys + [norm_key]
-    order = [k for k in lead if k in gate_keys] + [norm_key]
-    gate = gate.permute([gate_keys.index(k) for k in order])
-    # axes of length one change nothing: drop them
-    keep = [i for i, k in enumerate(order[:-1]) if gate.shape[i] != 1]
-    present = [order[i] for i in keep]
-    gate = gate.reshape([gate.shape[i] for i in keep] + [d])
-    if not present:
-        return gate.reshape(1, d), math.prod(shape), 1
-    places = [lead.index(k) for k in present]
-    low, high = places[0], places[-1] + 1
-    run = list(shape[low:high])
-    view = [s if lead[low + i] in present else 1 for i, s in enumerate(run)]
-    gate = gate.reshape(view + [d]).expand(run + [d])
-    return gate.reshape(math.prod(run), d), math.prod(shape[high:]), math.prod(run)
+def _gate_rows(gate, plan):
+    if plan.spread:
+        gate = gate.unsqueeze(-1).expand(*gate.shape, plan.d)
+    if plan.order is not None:
+        gate = gate.permute(plan.order)
+    if plan.run is not None:
+        # rows between the gate's own axes: written out (its gradient sums over them again, by autograd)
+        gate = gate.reshape(*plan.view, plan.d).expand(*plan.run, plan.d)
+    return gate.reshape(plan.count, plan.d)
 
 
-def _rows(t):
-    t = t.reshape(math.prod(t.shape[:-1]), t.shape[-1])
+def _rows(t, plan):
+    if plan.place != t.dim() - 1:
+        t = t.movedim(plan.place, -1)
+    t = t.reshape(math.prod(plan.lead), plan.d)
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
@@ -175,22 +227,13 @@ def einnorm(shard, x, y=None, *, axis, weight=None, bias=None, kind="layer", eps
     is normalised, ``gate_axes`` those of ``gate`` ("d", "b d", "b s d", "b", ...).
     Without ``y`` there is no block yet: ``h`` is ``x`` and ``n`` its norm.
     Parameters and gate are of the stream's type or fp32."""
-    axes = _axes(shard, families, "the stream")
-    if x.dtype not in (*_TYPES, torch.float64):
+    if families is not None:
+        shard, _ = cached_expand_axis_families(shard, families=families)
+        if gate_axes is not None:
+            gate_axes, _ = cached_expand_axis_families(gate_axes, families=families)
+    if x.dtype not in _FLOATS:
         raise TypeError(f"einnorm takes floating-point tensors, not {x.dtype}")
-    keys = _written_out(axes, x.dim())
-    if len(keys) != x.dim():
-        raise ValueError(f"The stream has {x.dim()} dimensions, {shard!r} names {len(axes)} axes")
-    found = [k for k in keys if not isinstance(k, tuple) and k.name == axis]
-    if not found:
-        raise ValueError(f"Axis {axis!r} is not among the stream's axes")
-    norm_key = found[0]
-    if not norm_key.local():
-        raise NotImplementedError(f"einnorm needs the normalised axis {axis!r} whole on every rank")
-    place = keys.index(norm_key)
-    d = x.shape[place]
-    if d == 0:
-        raise ValueError(f"The normalised axis {axis!r} is empty")
+    plan = _plan(shard, axis, gate_axes, tuple(x.shape), None if gate is None else tuple(gate.shape))
     if kind not in ("layer", "rms"):
         raise ValueError(f"kind must be 'layer' or 'rms', not {kind!r}")
     if not (math.isfinite(eps) and eps >= 0):
@@ -203,44 +246,32 @@ def einnorm(shard, x, y=None, *, axis, weight=None, bias=None, kind="layer", eps
         raise ValueError("post_weight and post_bias need post=True")
     if y is not None:
         _check_like(y, x, "y")
-    for t, name in ((weight, "weight"), (bias, "bias"), (post_weight, "post_weight"), (post_bias, "post_bias")):
-        _check_vector(t, x, d, name)
-
-    lead = keys[:place] + keys[place + 1:]
-    shape = list(x.shape[:place]) + list(x.shape[place + 1:])
-    inner = count = 1
+    _check_vector(weight, x, plan.d, "weight")
+    _check_vector(bias, x, plan.d, "bias")
+    _check_vector(post_weight, x, plan.d, "post_weight")
+    _check_vector(post_bias, x, plan.d, "post_bias")
+    inner, count = plan.inner, plan.count
     if gate is not None:
-        if gate_axes is None:
-            raise ValueError("gate needs gate_axes")
-        width = x.dim() - sum(1 for a in axes if not isinstance(a, EllipsisAxis))
-        named = _axes(gate_axes, families, "the gate") if gate_axes.strip() else []  # "": a scalar
-        gate_keys = _written_out(named, len(named) - 1 + width if any(isinstance(a, EllipsisAxis) for a in named)
-                                 else len(named))
-        if len(gate_keys) != gate.dim():
-            raise ValueError(f"The gate has {gate.dim()} dimensions, {gate_axes!r} names {len(gate_keys)} axes")
-        for k, size in zip(gate_keys, gate.shape):
-            if k not in keys:
-                raise ValueError(f"The gate's axis {k} is not one of the stream's")
-            if size != x.shape[keys.index(k)]:
-                raise ValueError(f"The gate's axis {k} has length {size}, the stream's {x.shape[keys.index(k)]}")
         _check_param(gate, x, "gate")
         if x.numel():
-            gate, inner, count = _gate_rows(gate, gate_keys, lead, shape, norm_key, d)
+            gate = _gate_rows(gate, plan)
         else:
-            gate = gate.sum().expand(1, d)  # no row to weigh: in the graph, with a gradient of zero
-            inner = 1
-    elif gate_axes is not None:
-        raise ValueError("gate_axes without a gate")
+            gate, inner, count = gate.sum().expand(1, plan.d), 1, 1  # no row to weigh: a gradient of zero
 
     conf = (inner, count, bool(post), kind == "layer", float(scale), float(eps))
-    args = [_rows(x.movedim(place, -1)), None if y is None else _rows(y.movedim(place, -1))]
-    params = [None if t is None else t.contiguous() for t in (weight, bias, post_weight, post_bias, gate)]
-    if _on_kernels(x):
-        out = _NativeNorm.apply(*args, *params, conf)
+    args = [_rows(x, plan), None if y is None else _rows(y, plan)]
+    args += [None if t is None else t.contiguous() for t in (weight, bias, post_weight, post_bias, gate)]
+    if not _on_kernels(x):
+        out = _torch_norm(*args, conf)
+    elif torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+        out = _NativeNorm.apply(*args, conf)
     else:
-        out = _torch_norm(*args, *params, conf)
+        h, n, _ = _native.require().norm_forward(*args, *conf, False)
+        out = n if y is None else (h, n)
 
     def back(t):
-        return t.reshape(*shape, d).movedim(-1, place)
+        if plan.place == len(plan.lead):
+            return t.view(x.shape)
+        return t.view(*plan.lead, plan.d).movedim(-1, plan.place)
 
     return (x, back(out)) if y is None else (back(out[0]), back(out[1]))

@@ -18,6 +18,7 @@ extension of this framework.
 """
 
 import math
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
@@ -31,6 +32,7 @@ from . import _native
 __all__ = ["PolicyLoss", "einpolicy"]
 
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_FLOATS = (*_TYPES, torch.float64)
 _REDUCTIONS = {"mean": 0, "sequence": 1, "sum": 2}
 
 
@@ -60,6 +62,7 @@ class _NativePolicy(torch.autograd.Function):
     def forward(ctx, logits, ids, mask, old, ref, adv, conf):
         loss, kl, clipped, logp, *state = _native.require().policy_forward(logits, ids, mask, old, ref, adv, *conf)
         ctx.conf = conf
+        ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, ids, mask, old, ref, adv, *state)
         ctx.mark_non_differentiable(logp, kl, clipped)
         return loss, logp, kl, clipped
@@ -67,6 +70,8 @@ class _NativePolicy(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad, *_):
+        if grad is None:
+            return (None,) * 7
         *inputs, terms, norm, weight = ctx.saved_tensors
         dlogits = _native.require().policy_backward(grad.contiguous(), *inputs, *ctx.conf, terms, norm, weight)
         return (dlogits,) + (None,) * 6
@@ -110,6 +115,28 @@ def _torch_policy(logits, ids, mask, old, ref, adv, conf):
     return loss, kept(lp).detach(), reduced(kl).detach(), reduced(clipped).detach()
 
 
+@lru_cache(maxsize=1024)
+def _vocabulary(shard, axis, rank):
+    """The vocabulary's dimension."""
+    spec = parse_sharding(f"{shard} -> {shard}")[0]
+    if getattr(spec, "partials", ()):
+        raise ValueError("einpolicy does not take partial sums")
+    names = []
+    for a in spec.axes:
+        if isinstance(a, (AxisGroup, EllipsisAxis)):
+            raise NotImplementedError("einpolicy needs every axis named, none factored")
+        if not a.local():
+            raise NotImplementedError(f"einpolicy needs axis {a.name!r} whole on every rank")
+        if a.name in names:
+            raise ValueError(f"Axis {a.name!r} appears more than once")
+        names.append(a.name)
+    if rank != len(names):
+        raise ValueError(f"The logits have {rank} dimensions, {shard!r} names {len(names)} axes")
+    if axis not in names:
+        raise ValueError(f"Axis {axis!r} is not among the logits' axes")
+    return names.index(axis)
+
+
 def _token_input(t, name, shapes, logits):
     """A constant of the loss as contiguous fp32 (fp64 beside fp64 logits)."""
     if t.device != logits.device or not t.is_floating_point():
@@ -118,7 +145,12 @@ def _token_input(t, name, shapes, logits):
         raise ValueError(f"{name} must have the shape {' or '.join(str(s) for s in shapes)}, not {tuple(t.shape)}")
     if t.requires_grad:
         raise ValueError(f"{name} is a constant of the loss: detach it")
-    return t.to(torch.float64 if logits.dtype == torch.float64 else torch.float32).reshape(-1).contiguous()
+    return _flat(t.to(torch.float64 if logits.dtype == torch.float64 else torch.float32))
+
+
+def _flat(t):
+    """One contiguous row."""
+    return t.reshape(-1).contiguous()
 
 
 def einpolicy(shard, logits, ids, *, axis, advantages, old_logp=None, ref_logp=None, mask=None, clip=0.2, kl=0.0,
@@ -136,26 +168,11 @@ def einpolicy(shard, logits, ids, *, axis, advantages, old_logp=None, ref_logp=N
     no kept token at all gives 0.  ``weight`` multiplies the loss (a share of
     accumulated steps): here it is free, where a factor outside costs backward
     another pass over the logits."""
-    formula, _ = cached_expand_axis_families(shard, families=families)
-    spec = parse_sharding(f"{formula} -> {formula}")[0]
-    if getattr(spec, "partials", ()):
-        raise ValueError("einpolicy does not take partial sums")
-    names = []
-    for a in spec.axes:
-        if isinstance(a, (AxisGroup, EllipsisAxis)):
-            raise NotImplementedError("einpolicy needs every axis named, none factored")
-        if not a.local():
-            raise NotImplementedError(f"einpolicy needs axis {a.name!r} whole on every rank")
-        if a.name in names:
-            raise ValueError(f"Axis {a.name!r} appears more than once")
-        names.append(a.name)
-    if logits.dim() != len(names):
-        raise ValueError(f"The logits have {logits.dim()} dimensions, {shard!r} names {len(names)} axes")
-    if axis not in names:
-        raise ValueError(f"Axis {axis!r} is not among the logits' axes")
-    if logits.dtype not in (*_TYPES, torch.float64):
+    if families is not None:
+        shard, _ = cached_expand_axis_families(shard, families=families)
+    if logits.dtype not in _FLOATS:
         raise TypeError(f"einpolicy takes floating-point logits, not {logits.dtype}")
-    place = names.index(axis)
+    place = _vocabulary(shard, axis, logits.dim())
     shape = tuple(logits.shape[:place]) + tuple(logits.shape[place + 1:])
     vocab = logits.shape[place]
     if vocab == 0:
@@ -187,13 +204,18 @@ def einpolicy(shard, logits, ids, *, axis, advantages, old_logp=None, ref_logp=N
     if tokens == 0:
         zero = logits.detach().new_zeros((), dtype=torch.promote_types(logits.dtype, torch.float32))
         return PolicyLoss(logits.sum(dtype=zero.dtype), zero.expand(shape), zero, zero)
-    rows = logits.movedim(place, -1).reshape(tokens, vocab)
+    rows = logits if place == len(shape) else logits.movedim(place, -1)
+    rows = rows.reshape(tokens, vocab)
     if rows.stride(1) != 1 and vocab > 1:
         rows = rows.contiguous()
-    if mask is not None:
-        mask = mask.reshape(-1).contiguous()
+    mask = None if mask is None else _flat(mask)
     conf = (max(shape[-1], 1) if shape else 1, float(low), float(high), float(kl), float(temperature),
             _REDUCTIONS[reduction], float(weight))
-    args = (rows, ids.reshape(-1).long().contiguous(), mask, old, ref, adv, conf)
-    loss, logp, kl_value, clipped = _NativePolicy.apply(*args) if _on_kernels(logits) else _torch_policy(*args)
+    args = (rows, _flat(ids.long()), mask, old, ref, adv, conf)
+    if not _on_kernels(logits):
+        loss, logp, kl_value, clipped = _torch_policy(*args)
+    elif torch.is_grad_enabled() and rows.requires_grad:
+        loss, logp, kl_value, clipped = _NativePolicy.apply(*args)
+    else:
+        loss, kl_value, clipped, logp, *_ = _native.require().policy_forward(*args[:-1], *conf)
     return PolicyLoss(loss, logp.view(shape), kl_value, clipped)

@@ -236,6 +236,7 @@ class _SavedContraction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, y, equation, plan, codes, exps, meta, layout):
+        ctx.set_materialize_grads(False)
         ctx.equation, ctx.meta, ctx.layout = equation, meta, layout
         if layout is None:
             ctx.save_for_backward(y, codes, exps)
@@ -248,6 +249,8 @@ class _SavedContraction(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad, *_):
+        if grad is None:
+            return (None,) * 8
         y, codes, exps = ctx.saved_tensors[:3]
         if ctx.layout is not None:
             grad = _silu_grad(grad, *ctx.saved_tensors[3:], ctx.layout)
@@ -298,6 +301,7 @@ class _SiluSaved(torch.autograd.Function):
     @staticmethod
     def forward(ctx, h):
         wide = torch.promote_types(h.dtype, torch.float32)
+        ctx.set_materialize_grads(False)
         a, codes, exps = _silu_forward((_rows(h) if h.dim() else h.view(1, 1)).to(wide), h.dtype)
         ctx.save_for_backward(codes, exps)
         ctx.mark_non_differentiable(codes, exps)
@@ -306,7 +310,7 @@ class _SiluSaved(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad, *_):
-        return _silu_grad(grad, *ctx.saved_tensors, (False, None, None))
+        return None if grad is None else _silu_grad(grad, *ctx.saved_tensors, (False, None, None))
 
 
 def silu_saved(h):
