@@ -40,7 +40,7 @@ namespace {
 // A thread holds 2 kP columns of a row, as kP pairs.
 constexpr int kThreads = 512;       // most threads a block has
 constexpr int kRowPairs = 8;
-constexpr int kRegSums = 4096;      // columns whose sums stay in registers
+constexpr int kNarrow = kThreads * kRowPairs;  // columns of a block whose threads hold half as many
 constexpr int kMaxCluster = 8;
 constexpr int kWideThreads = 512;   // block of the several-pass kernels
 constexpr long long kMinGroup = 16;
@@ -625,15 +625,17 @@ struct Sums {
 };
 
 // Sums: 0 S1 (of D yh, or of gate D yh), 1 W1 (dn hh); kFull: 2 S0, 3 W0 as well.
-// kShared: twice the columns a thread, and their sums in shared memory.
-template <typename T, int kA, bool kPost, bool kFull, bool kShared>
+// kWide: twice the columns a thread.  Its four sums do not fit the registers, and in shared memory they leave no
+// room for the column vectors, which then come from the caches row by row.
+template <typename T, int kA, bool kPost, bool kFull, bool kWide>
 __global__ void __launch_bounds__(kThreads)
     norm_backward_kernel(const NormArgs a, const NormPlan plan, const NormBackward o, const int blocks,
                          const int stages) {
   extern __shared__ __align__(16) unsigned char shared[];
   constexpr int kN = kFull ? 8 : 4;
   constexpr int kSums = kFull ? 4 : 2;
-  constexpr int kP = kShared ? kRowPairs : kRowPairs / 2;
+  constexpr int kP = kWide ? kRowPairs : kRowPairs / 2;
+  constexpr bool kShared = kWide && kFull;
   using Rows = Stream<T, kA, kP>;
   const int rank = blocks == 1 ? 0 : static_cast<int>(cluster_ctarank());
   const Span s = span_of(a, rank, blocks);
@@ -663,30 +665,75 @@ __global__ void __launch_bounds__(kThreads)
   const int ahead = stages > 1 ? stages - 1 : 1;
   for (int k = 0; k < ahead; ++k) fetch(first + k, k);
   const Pair scale = pair(a.scale);
+  // column vectors in shared memory, a thread's own: w, t = gate pw (gate without post) and gate pb, these two
+  // formed anew where the gate's row changes
+  constexpr int kVectors = kFull ? 3 : 2;
+  ulonglong2* vectors = reinterpret_cast<ulonglong2*>(slots + 4 * stages * words);
+  auto keep = [&](int k, const Pair (&f)[kP]) {
+#pragma unroll
+    for (int q = 0; q < kP / 2; ++q)
+      vectors[(k * (kP / 2) + q) * blockDim.x + threadIdx.x] = make_ulonglong2(f[2 * q], f[2 * q + 1]);
+  };
+  long long g0 = 0;  // the gate's row
+  auto kept = [&](int k, Pair (&f)[kP]) {
+    if (kShared) {
+      param<T, kA>(k == 0 ? a.w : a.gate, k == 0 ? 0 : g0, 1.0f, f, s);
+      if (k == 1 && kPost) times<T, kA>(a.pw, 0, f, s);
+      if (k == 2) times<T, kA>(a.pb, 0, f, s);
+      return;
+    }
+#pragma unroll
+    for (int q = 0; q < kP / 2; ++q) {
+      const ulonglong2 v = vectors[(k * (kP / 2) + q) * blockDim.x + threadIdx.x];
+      f[2 * q] = v.x;
+      f[2 * q + 1] = v.y;
+    }
+  };
+  if (!kShared) {
+    Pair f[kP];
+    param<T, kA>(a.w, 0, 1.0f, f, s);
+    keep(0, f);
+  }
+  long long gate_at = -1;
   if (blocks > 1) cluster_sync();  // every block runs before one writes another's words
   int stage = 0;
   for (long long row = first; row < last; ++row) {
     const float4 st = reinterpret_cast<const float4*>(o.stats)[row];
-    const long long g0 = gate_row(a, row) * a.d;
+    const long long g = gate_row(a, row);
+    g0 = g * a.d;
+    Pair hh[kP], yh[kP], t[kP], u[kP];
+    if (!kShared && a.y != nullptr && g != gate_at) {
+      gate_at = g;
+      param<T, kA>(a.gate, g0, 1.0f, t, s);
+      if (kPost) {
+        if constexpr (kFull) {
+          param<T, kA>(a.pb, 0, 0.0f, u, s);
+#pragma unroll
+          for (int i = 0; i < kP; ++i) u[i] = mul2(u[i], t[i]);
+          keep(2, u);
+        }
+        times<T, kA>(a.pw, 0, t, s);
+      }
+      keep(1, t);
+    }
     wait_row(stages);
     if (kA == kAny) __syncthreads();
-    Pair hh[kP], yh[kP], t[kP], u[kP];
     Pair v[kN];
 #pragma unroll
     for (int k = 0; k < kN; ++k) v[k] = 0ull;
     sx.read(row, stage, s, hh);
-    param<T, kA>(a.gate, g0, 1.0f, t, s);  // t: the gate; with kPost times pw
     if (a.y != nullptr) {
+      kept(1, t);
       sy.read(row, stage, s, yh);
+      if (kPost && kFull && a.pb.p != nullptr) {
+        kept(kVectors - 1, u);
 #pragma unroll
-      for (int i = 0; i < kP; ++i) hh[i] = mul2(hh[i], scale);
+        for (int i = 0; i < kP; ++i) hh[i] = fma2(hh[i], scale, u[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kP; ++i) hh[i] = mul2(hh[i], scale);
+      }
       if (kPost) {
-        if (kFull && a.pb.p != nullptr) {
-          param<T, kA>(a.pb, 0, 0.0f, u, s);
-#pragma unroll
-          for (int i = 0; i < kP; ++i) hh[i] = fma2(t[i], u[i], hh[i]);
-        }
-        times<T, kA>(a.pw, 0, t, s);
         const Pair off = pair(-st.x), unit_y = pair(st.y);
 #pragma unroll
         for (int i = 0; i < kP; ++i) yh[i] = only<kA>(mul2(add2(yh[i], off), unit_y), i, s);
@@ -716,9 +763,10 @@ __global__ void __launch_bounds__(kThreads)
       for (int i = 0; i < kP; ++i) dn[i] = only<kA>(dn[i], i, s);
       sums.add(1, dn, hh);
       if constexpr (kFull) sums.add(3, dn);
-      times<T, kA>(a.w, 0, dn, s);
+      kept(0, t);
 #pragma unroll
       for (int i = 0; i < kP; ++i) {
+        dn[i] = mul2(dn[i], t[i]);
         u[i] = fma2(rh, dn[i], u[i]);  // dh + r_h gn
         v[0] = fma2(dn[i], hh[i], v[0]);
         if constexpr (kFull) v[3] = add2(v[3], dn[i]);
@@ -727,17 +775,19 @@ __global__ void __launch_bounds__(kThreads)
     if (kA == kAny && stages == 1) __syncthreads();  // every thread has read the slot
     // the slot read a row ago (a barrier lies between, or it is the thread's own); one stage: this row's, read above
     fetch(row + ahead, stages == 1 ? 0 : (stage == 0 ? ahead : stage - 1));
+    if (a.y != nullptr) kept(1, t);
     if (kPost) {
+      // B and C without their factor r_h
 #pragma unroll
       for (int i = 0; i < kP; ++i) {
-        const Pair A = mul2(t[i], u[i]), B = only<kA>(mul2(t[i], rh), i, s), C = mul2(B, hh[i]);
+        const Pair A = mul2(t[i], u[i]), C = mul2(t[i], hh[i]);
         v[1] = fma2(A, yh[i], v[1]);
         v[2] = fma2(C, yh[i], v[2]);
         if constexpr (kFull) {
           v[4] = add2(v[4], A);
-          v[5] = add2(v[5], B);
+          v[5] = add2(v[5], t[i]);
           v[6] = add2(v[6], C);
-          v[7] = fma2(B, yh[i], v[7]);
+          v[7] = fma2(t[i], yh[i], v[7]);
         }
       }
     }
@@ -796,11 +846,11 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int i = 0; i < kP; ++i) u[i] = mul2(t[i], u[i]);
         if (kPost) {
-          float e2 = e[1] - m2 * e[2], e1 = 0.0f;
+          float e2 = e[1] - st.w * m2 * e[2], e1 = 0.0f;
           if constexpr (kFull) {
             if (a.center) {
-              e2 -= m1 * e[7];
-              e1 = e[4] - m1 * e[5] - m2 * e[6];
+              e2 -= st.w * m1 * e[7];
+              e1 = e[4] - st.w * (m1 * e[5] + m2 * e[6]);
             }
           }
           const Pair c1 = pair(-e1), c2 = pair(-e2), unit_y = pair(st.y);
@@ -923,18 +973,20 @@ __device__ __forceinline__ void put1(void* p, int f32, int dtype, long long i, f
     static_cast<float*>(p)[i] = v;
 }
 
-// The units' sums to gradients: block (tile of 32 columns, job).  Job 0: the
-// parameters, and the gate's row where it has one; then a job a gate row.  Eight
-// threads walk the columns four at a time, 128 the units; the order is fixed.
+// The units' sums to gradients: block (tile of 16 columns, job).  Job 0: the
+// parameters, and the gate's row where it has one; then a job a gate row.  Four
+// threads walk the columns four at a time, 64 the units; the order is fixed.
+constexpr int kFinishThreads = 256;
+
 template <typename T>
-__global__ void __launch_bounds__(1024)
+__global__ void __launch_bounds__(kFinishThreads)
     norm_finish_kernel(const NormArgs a, const NormPlan plan, const float* __restrict__ ws, const NormSums o) {
-  __shared__ float part[4][32][33];
+  __shared__ float part[4][kFinishThreads / 32][16];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int quad = lane & 7;                       // columns 4 quad .. 4 quad + 3 of the tile
-  const int walker = w * 4 + (lane >> 3);
-  const long long c4 = blockIdx.x * 32ll + quad * 4;
-  const long long c = blockIdx.x * 32ll + lane;
+  const int quad = lane & 3;                       // columns 4 quad .. 4 quad + 3 of the tile
+  const int walker = w * 8 + (lane >> 2);
+  const long long c4 = blockIdx.x * 16ll + quad * 4;
+  const long long c = blockIdx.x * 16ll + (threadIdx.x & 15);
   const int n = plan.sums();
   const bool vec = a.d % 4 == 0;
   const long long jobs = o.dgate != nullptr && plan.groups > 1 ? 1 + plan.groups : 1;
@@ -943,13 +995,13 @@ __global__ void __launch_bounds__(1024)
     const long long last = job == 0 ? plan.units() : job * plan.slices;
     const bool weigh = job == 0 && plan.grouped && plan.groups > 1;  // with the gate of the unit's group
     float s[4][4] = {};
-#pragma unroll 2
-    for (long long unit = first + walker; unit < last; unit += 128) {
+#pragma unroll 4
+    for (long long unit = first + walker; unit < last; unit += kFinishThreads / 4) {
       float g[4] = {1.0f, 1.0f, 1.0f, 1.0f};
       if (weigh)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (c4 + j < a.d) g[j] = param1<T>(a.gate, unit / plan.slices * a.d + c4 + j, 1.0f);
+          if (c4 + j < a.d) g[j] = param1<T>(a.gate, static_cast<uint32_t>(unit) / static_cast<uint32_t>(plan.slices) * a.d + c4 + j, 1.0f);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (k >= n) break;
@@ -976,20 +1028,21 @@ __global__ void __launch_bounds__(1024)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float v = s[k][j];
+        v += __shfl_xor_sync(0xffffffffu, v, 4);
         v += __shfl_xor_sync(0xffffffffu, v, 8);
         v += __shfl_xor_sync(0xffffffffu, v, 16);
-        if (lane < 8) part[k][w][quad * 4 + j] = v;
+        if (lane < 4) part[k][w][quad * 4 + j] = v;
       }
     __syncthreads();
-    if (w < 4) {
-      float v = 0.0f;
+    if (threadIdx.x < 16 && c < a.d) {
+      float e[4];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v += part[w][i][lane];
-      part[w][0][lane] = v;  // read and written by this thread alone
-    }
-    __syncthreads();
-    if (w == 0 && c < a.d) {
-      const float s1 = part[0][0][lane], w1 = part[1][0][lane], s0 = part[2][0][lane], w0 = part[3][0][lane];
+      for (int k = 0; k < 4; ++k) {
+        e[k] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kFinishThreads / 32; ++i) e[k] += part[k][i][threadIdx.x];
+      }
+      const float s1 = e[0], w1 = e[1], s0 = e[2], w0 = e[3];
       if (job == 0) {
         // one group: the sums of D become those of gate D here
         const float g = plan.grouped && plan.groups == 1 ? param1<T>(a.gate, c, 1.0f) : 1.0f;
@@ -1016,9 +1069,9 @@ bool vector_rows(const NormArgs& a) {
          aligned(a.b.p) && aligned(a.pw.p) && aligned(a.pb.p) && aligned(a.gate.p);
 }
 
-// Columns a block holds: 512 threads' of a 16-bit type; of fp32, whose rows take twice the shared memory beside
-// the shared sums, those with sums in registers.
-long long block_columns(const NormArgs& a) { return a.dtype == kDtypeF32 ? kRegSums : 2 * kRowPairs * kThreads; }
+// Columns a block holds: 512 threads' of a 16-bit type, half of them of fp32, whose rows take twice the shared
+// memory.
+long long block_columns(const NormArgs& a) { return a.dtype == kDtypeF32 ? kNarrow : 2 * kRowPairs * kThreads; }
 
 // Blocks that share a row: one, or a cluster.
 int blocks_for(const NormArgs& a) { return static_cast<int>((a.d + block_columns(a) - 1) / block_columns(a)); }
@@ -1028,9 +1081,9 @@ int threads_for(const NormArgs& a, int pairs) {
   return ((columns + 2 * pairs - 1) / (2 * pairs) + 31) / 32 * 32;
 }
 
-// Sums in registers up to 512 threads of four pairs.
-bool shared_sums(const NormArgs& a) { return columns_per_block(a.d, blocks_for(a)) > kRegSums; }
-int backward_pairs(const NormArgs& a) { return shared_sums(a) ? kRowPairs : kRowPairs / 2; }
+// Backward: 512 threads of four pairs, or of eight.
+bool wide_rows(const NormArgs& a) { return columns_per_block(a.d, blocks_for(a)) > kNarrow; }
+int backward_pairs(const NormArgs& a) { return wide_rows(a) ? kRowPairs : kRowPairs / 2; }
 
 Access access_of(const NormArgs& a, int pairs, bool others_aligned) {
   if (!vector_rows(a) || !others_aligned) return kAny;
@@ -1052,6 +1105,7 @@ constexpr int kSharedBytes = 227 * 1024;
 struct Launch {
   int threads;
   int fixed;      // bytes of the exchange words and shared sums
+  int vectors = 0;  // bytes of the column vectors behind the slots
   int stages;
   int bytes;
   long long resident;  // blocks an SM holds, about
@@ -1059,22 +1113,23 @@ struct Launch {
 
 Launch backward_launch(const NormArgs& a, const NormPlan& plan, bool vec) {
   Launch l;
-  const bool shared = shared_sums(a);
+  const bool shared = wide_rows(a) && plan.full;
   const int pairs = backward_pairs(a);
   const int threads = l.threads = threads_for(a, pairs);
   l.fixed = exchange_bytes(plan.full ? 8 : 4) + (shared ? plan.sums() * pairs * 8 * threads : 0);
+  l.vectors = shared ? 0 : (plan.full ? 3 : 2) * pairs * 8 * threads;
   const int slot = slot_bytes(a, pairs, vec, 4);
-  const long long regs = plan.full || shared ? 128 : 112;
+  const long long regs = plan.full || wide_rows(a) ? 128 : 112;
   l.resident = 65536 / (regs * threads);
   if (l.resident > 12) l.resident = 12;
   if (l.resident < 1) l.resident = 1;
   // as many rows in flight as an SM's shared memory allows its resident blocks, two at least where one block can
   for (;; --l.resident) {
-    l.stages = static_cast<int>((kSharedBytes / l.resident - 1024 - l.fixed) / slot);
+    l.stages = static_cast<int>((kSharedBytes / l.resident - 1024 - l.fixed - l.vectors) / slot);
     if (l.stages >= 2 || l.resident == 1) break;
   }
   if (l.stages > kMaxStages) l.stages = kMaxStages;
-  l.bytes = l.fixed + l.stages * slot;
+  l.bytes = l.fixed + l.vectors + l.stages * slot;
   return l;
 }
 
@@ -1145,7 +1200,7 @@ template <typename T, int kA, bool kPost>
 int backward_sums(const NormArgs& a, const NormPlan& plan, const NormBackward& b, cudaStream_t stream) {
   const Launch l = backward_launch(a, plan, kA != kAny);
   const long long units = plan.units();
-  if (shared_sums(a))
+  if (wide_rows(a))
     return plan.full
                ? launch_rows(norm_backward_kernel<T, kA, kPost, true, true>, units, a, l, stream, plan, b)
                : launch_rows(norm_backward_kernel<T, kA, kPost, false, true>, units, a, l, stream, plan, b);
@@ -1185,8 +1240,8 @@ int backward_type(const NormArgs& a, const NormPlan& plan, const NormBackward& b
   }
   if (rc != 0 || b.ws == nullptr) return rc;
   const long long jobs = s.dgate != nullptr && plan.groups > 1 ? 1 + plan.groups : 1;
-  const dim3 grid(static_cast<unsigned>((a.d + 31) / 32), static_cast<unsigned>(jobs < 65535 ? jobs : 65535));
-  norm_finish_kernel<T><<<grid, 1024, 0, stream>>>(a, plan, b.ws, s);
+  const dim3 grid(static_cast<unsigned>((a.d + 15) / 16), static_cast<unsigned>(jobs < 65535 ? jobs : 65535));
+  norm_finish_kernel<T><<<grid, kFinishThreads, 0, stream>>>(a, plan, b.ws, s);
   ++*launches;
   return static_cast<int>(cudaGetLastError());
 }
