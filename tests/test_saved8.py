@@ -145,18 +145,36 @@ def test_linear(device, dtype, shape, transposed):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("shape", SHAPES + [pytest.param((2, 2500, 128, 2048), marks=pytest.mark.gpu)])
-def test_mlp(device, dtype, shape):
-    if device == "cpu" and shape[1] > 1000:
-        pytest.skip("the wide kernel's shape")
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("transposed", [False, True])
+def test_mlp(device, dtype, shape, transposed):
+    check_mlp(device, dtype, shape, transposed)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("shape", [(2, 2500, 128, 2048), (1, 5003, 200, 1040), (3, 1111, 72, 4112), (1, 4736, 64, 256),
+                                   (1, 2400, 96, 1000), (1, 2400, 96, 1032)])
+def test_mlp_in_the_product(dtype, transposed, shape):
+    """Shapes whose pre-activation is quantised, and whose gradient takes silu', in the products' epilogues (16-byte
+    rows of codes; the last two are not), with ragged edges."""
+    check_mlp("cuda", dtype, shape, transposed)
+
+
+def check_mlp(device, dtype, shape, transposed):
     x, w1, w2, dy, _ = _case(device, dtype, *shape, seed=5)
+    if transposed:
+        w1, w2 = w1.t().contiguous(), w2.t().contiguous()
     for t in (x, w1, w2):
         t.requires_grad_(True)
     s = es.checkpoint8(x)
-    a = es.einshard("b s c, h c -> b s h", s, w1, activation="silu")
+    a = es.einshard("b s c, c h -> b s h" if transposed else "b s c, h c -> b s h", s, w1, activation="silu")
     assert isinstance(a, es.Saved8) and a.value.dtype == dtype
-    y = es.einshard("b s h, c h -> b s c", a, w2)
+    y = es.einshard("b s h, h c -> b s c" if transposed else "b s h, c h -> b s c", a, w2)
     dx, dw1, dw2 = torch.autograd.grad(y, (x, w1, w2), dy)
+    if transposed:
+        w1, w2, dw1, dw2 = w1.t(), w2.t(), dw1.t(), dw2.t()
 
     xd, w1d, w2d, dyd = (t.detach().double().cpu() for t in (x, w1, w2, dy))
     pre = xd @ w1d.t()
@@ -286,6 +304,22 @@ def test_refusals(device):
         z = es.einshard("b s c, h c -> b s h", es.checkpoint8(xg), w).square().sum()
         (dx,) = torch.autograd.grad(z, xg, create_graph=True)
         torch.autograd.grad(dx.sum(), xg)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_activation_used_twice(device):
+    """The activation's value, and two products that read it, send their gradients to one pre-activation."""
+    x, w1, w2, dy, da = _case(device, torch.float32, 2, 6, 40, 48, seed=11)
+    w1.requires_grad_(True)
+    a = es.einshard("b s c, h c -> b s h", es.checkpoint8(x), w1, activation="silu")
+    y1 = es.einshard("b s h, c h -> b s c", a, w2)
+    y2 = es.einshard("b s h, c h -> s b c", a, 2 * w2)
+    parts = [torch.autograd.grad(y1, w1, dy, retain_graph=True)[0],
+             torch.autograd.grad(y2, w1, dy.transpose(0, 1), retain_graph=True)[0],
+             torch.autograd.grad(a.value, w1, da, retain_graph=True)[0]]
+    (both,) = torch.autograd.grad((y1, y2, a.value), w1, (dy, dy.transpose(0, 1), da))
+    assert torch.allclose(both, sum(parts), rtol=1e-4, atol=1e-4)
+    assert torch.allclose(parts[1], 2 * parts[0], rtol=1e-4, atol=1e-4)
 
 
 @pytest.mark.gpu

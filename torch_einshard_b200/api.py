@@ -9,13 +9,15 @@ registration without running anything.  Contract of
 ``src/torch_einshard/__init__.py:82-372``.
 """
 
+from functools import lru_cache
+
 from . import params as _params
 from .notation.families import cached_expand_axis_families
 from .notation.parser import parse_sharding
 from .notation.spec import Axes, AxisGroup, EllipsisAxis, TensorSpec
 from .ops import gemm as _gemm
-from .ops.einsum import einsum
-from .ops.saved8 import Saved8, silu_saved
+from .ops.einsum import einsum, equation_for
+from .ops.saved8 import Saved8, contract_saved, silu_saved
 from .parallel.executor import distributed_1d
 from .plan.policy import resolve_plan_policy
 from .plan.state import TensorState
@@ -138,6 +140,17 @@ def _check_saved(shard, xs):
         raise TypeError("a Saved8 operand needs a second operand to be contracted with")
 
 
+@lru_cache(maxsize=1024)
+def _saved_equation(formula):
+    """The local contraction's letters when ``formula`` is nothing else (no groups, no annotations), or None."""
+    shard = parse_sharding(formula)
+    if shard[1] is None or not local_operation(shard):
+        return None
+    if any(_has_groups(spec) or getattr(getattr(spec, "annotation", None), "is_param", False) for spec in shard):
+        return None
+    return equation_for(shard)
+
+
 def einshard(shard, *xs, mesh=None, shapes=None, sizes=None, families=None, optimize=None, policy=None,
              activation=None):
     """Run an einshard expression on ``xs`` (see module docstring).
@@ -154,6 +167,14 @@ def einshard(shard, *xs, mesh=None, shapes=None, sizes=None, families=None, opti
     ``activation`` the result is a ``Saved8`` as well."""
     policy = resolve_plan_policy(optimize=optimize, policy=policy)
     shard, sizes = cached_expand_axis_families(shard, sizes, families)
+    if len(xs) == 2 and isinstance(xs[0], Saved8) and not isinstance(xs[1], Saved8):
+        equation = _saved_equation(shard)
+        if equation is not None:
+            plan = ExecutionPlan()
+            out = contract_saved(equation, *xs, activation=activation)
+            plan.add("rank_local_einsum")
+            set_last_plan(plan)
+            return out
     shard = parse_sharding(shard)
     if activation is not None and getattr(shard[2], "partials", ()):
         raise ValueError("activation needs a complete output (no // partial sums)")

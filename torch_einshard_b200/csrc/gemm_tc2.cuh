@@ -42,10 +42,14 @@ struct SharedState2 {
   int epi[32];
 };
 
+// The kernel body; tmD: a second output map for epilogues that write two tensors
+// (EpiTile.tmw).  Those have a second staging buffer per epilogue warp behind the
+// first ones (kSmem2DualBytes).
+constexpr int kSmem2DualBytes = kSmem2Bytes + 4 * kStage2Out;
+
 template <class Epi>
-__global__ void __launch_bounds__(kThreads, 1)
-    gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                    const __grid_constant__ CUtensorMap tmC, const GemmShape shp, Epi epi) {
+__device__ __forceinline__ void gemm_tc2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmC,
+                                              const CUtensorMap& tmD, const GemmShape& shp, Epi& epi) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -199,6 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       et.q = q;
       et.lane = lane;
       et.tmc = &tmC;
+      et.tmw = &tmD;
       et.stage = out_stage + q * kStage2Out;
       const bool ok = epi.tile(et, shp, abort_flag);
       tc_fence_before();
@@ -220,6 +225,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, kTmemCols);
   }
+}
+
+template <class Epi>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ CUtensorMap tmC, const GemmShape shp, Epi epi) {
+  gemm_tc2_body(tmA, tmB, tmC, tmC, shp, epi);
+}
+
+// Two outputs.
+template <class Epi>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_tc2_dual_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                         const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmD,
+                         const GemmShape shp, Epi epi) {
+  gemm_tc2_body(tmA, tmB, tmC, tmD, shp, epi);
 }
 
 }  // namespace es

@@ -21,40 +21,13 @@
 #include "quant8.h"
 
 #include "gemm.h"
-#include "vec.cuh"
+#include "quant8.cuh"
 
 namespace es {
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kUnroll = 4;
-
-struct Step {
-  float inv;  // 2^-e
-  int byte;   // e + 127, or kQuantNan
-};
-
-// amax_bits: the largest |x| of the block as fp32 bits (NaN and infinity sort above every finite value).
-__device__ __forceinline__ Step step_of(uint32_t amax_bits) {
-  int e = static_cast<int>(amax_bits >> 23) - 127 - 6;
-  if (e < -126) e = -126;
-  float inv = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-  if (rintf(__uint_as_float(amax_bits) * inv) > 127.0f) {
-    ++e;
-    inv *= 0.5f;
-  }
-  if (amax_bits >= 0x7f800000u) return {0.0f, kQuantNan};
-  return {inv, e + 127};
-}
-
-// 2^e of an exponent byte; NaN for kQuantNan.
-__device__ __forceinline__ float scale_of(int byte) {
-  return byte == kQuantNan ? __uint_as_float(0x7fc00000u) : __uint_as_float(static_cast<uint32_t>(byte) << 23);
-}
-
-__device__ __forceinline__ int code_of(float x, const Step& s) {
-  return s.byte == kQuantNan ? 0 : __float2int_rn(x * s.inv);
-}
 
 template <typename T>
 struct Limit;
@@ -71,25 +44,36 @@ struct Limit<__half> {
   static constexpr float value = 65504.0f;
 };
 
-template <typename T>
-__device__ __forceinline__ float sigmoid_of(float x) {
-  return 1.0f / (1.0f + (sizeof(T) == 4 ? expf(-x) : __expf(-x)));
-}
-
 // A code's value; next to the type's largest value it may round past it: clamped, still within half a step.
 template <typename T>
-__device__ __forceinline__ float value_of(int q, float scale) {
-  const float v = static_cast<float>(q) * scale;
+__device__ __forceinline__ float value_of(float code, float scale) {
+  const float v = code * scale;
   return v > Limit<T>::value ? Limit<T>::value : (v < -Limit<T>::value ? -Limit<T>::value : v);  // NaN stays
 }
 
+// Two values through kMode.
 template <typename T, int kMode>
-__device__ __forceinline__ float restored(int q, float scale, float g) {
-  if (kMode == kRestoreValue) return value_of<T>(q, scale);
-  const float x = value_of<float>(q, scale);  // a pre-activation: kept from 32 bits
-  const float s = sigmoid_of<T>(x);
-  if (kMode == kRestoreSilu) return x * s;
-  return g * s * (1.0f + x * (1.0f - s));
+__device__ __forceinline__ void restored2(float& x1, float& x2, float g1, float g2) {
+  if (kMode == kRestoreValue) return;
+  float s1, s2;
+  if constexpr (sizeof(T) == 4) {
+    s1 = 1.0f / (1.0f + expf(-x1));
+    s2 = 1.0f / (1.0f + expf(-x2));
+  } else {
+    sigmoid_pair(x1, x2, s1, s2);
+  }
+  if (kMode == kRestoreSilu) {
+    x1 *= s1;
+    x2 *= s2;
+  } else {
+    x1 = g1 * silu_slope(x1, s1);
+    x2 = g2 * silu_slope(x2, s2);
+  }
+}
+
+template <typename T, int kMode>
+__device__ __forceinline__ float decoded(float code, float scale) {
+  return kMode == kRestoreValue ? value_of<T>(code, scale) : value_of<float>(code, scale);  // pre-activations: 32 bits
 }
 
 // Work of a warp in the vector kernels: kUnroll groups of 32 chunks of eight
@@ -149,15 +133,13 @@ __global__ void __launch_bounds__(kThreads) quant8_kernel(const T* __restrict__ 
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
       if (pl[u].elem < 0) continue;
-      const Step s = step_of(m);
-      uint32_t q[2] = {0, 0};
-#pragma unroll
-      for (int i = 0; i < 8; ++i) q[i >> 2] |= static_cast<uint32_t>(code_of(f[i], s) & 0xff) << (8 * (i & 3));
-      *reinterpret_cast<uint2*>(codes + pl[u].elem) = make_uint2(q[0], q[1]);
+      const Step8 s = step8_of(m);
+      *reinterpret_cast<uint2*>(codes + pl[u].elem) =
+          make_uint2(codes8_of(f[0], f[1], f[2], f[3], s), codes8_of(f[4], f[5], f[6], f[7], s));
       if ((lane & 3) == 0) exps[pl[u].block] = static_cast<uint8_t>(s.byte);
       if (kSilu) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] *= sigmoid_of<OutT>(f[i]);
+        for (int i = 0; i < 8; i += 2) restored2<OutT, kRestoreSilu>(f[i], f[i + 1], 0.0f, 0.0f);
         store8(out + pl[u].elem, f);
       }
     }
@@ -189,10 +171,14 @@ __global__ void __launch_bounds__(kThreads) quant8_any_kernel(const T* __restric
       const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(f[u]) & 0x7fffffffu);
       const long long c = (b0 + u) * kQuantBlock + lane;
       if (b0 + u >= nb) break;  // uniform
-      const Step s = step_of(m);
+      const Step8 s = step8_of(m);
       if (c < d) {
-        codes[row * d + c] = static_cast<int8_t>(code_of(f[u], s));
-        if (kSilu) out[row * d + c] = from_float<OutT>(f[u] * sigmoid_of<OutT>(f[u]));
+        codes[row * d + c] = static_cast<int8_t>(codes8_of(f[u], 0.0f, 0.0f, 0.0f, s));
+        if (kSilu) {
+          float none = 0.0f;
+          restored2<OutT, kRestoreSilu>(f[u], none, 0.0f, 0.0f);
+          out[row * d + c] = from_float<OutT>(f[u]);
+        }
       }
       if (lane == 0) exps[row * nb + b0 + u] = static_cast<uint8_t>(s.byte);
     }
@@ -218,7 +204,7 @@ __global__ void __launch_bounds__(kThreads) restore8_kernel(const int8_t* __rest
       pl[u] = walk.at(unit, u, lane);
       if (pl[u].elem < 0) continue;
       q[u] = __ldcs(reinterpret_cast<const uint2*>(codes + pl[u].elem));
-      scale[u] = scale_of(exps[pl[u].block]);
+      scale[u] = scale8_of(exps[pl[u].block]);
       if (kMode == kRestoreSiluGrad) g[u] = load8_stream(grad + pl[u].elem);
     }
 #pragma unroll
@@ -228,10 +214,11 @@ __global__ void __launch_bounds__(kThreads) restore8_kernel(const int8_t* __rest
       if (kMode == kRestoreSiluGrad) unpack8(g[u], gf);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const uint32_t w = i < 4 ? q[u].x : q[u].y;
-        const int code = static_cast<int8_t>(w >> (8 * (i & 3)));
-        f[i] = restored<T, kMode>(code, scale[u], kMode == kRestoreSiluGrad ? gf[i] : 0.0f);
+        if (kMode != kRestoreSiluGrad) gf[i] = 0.0f;
+        f[i] = decoded<T, kMode>(code8_at(i < 4 ? q[u].x : q[u].y, i & 3), scale[u]);
       }
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) restored2<T, kMode>(f[i], f[i + 1], gf[i], gf[i + 1]);
       store8(out + pl[u].elem, f);
     }
   }
@@ -254,9 +241,11 @@ __global__ void __launch_bounds__(kThreads) restore8_any_kernel(const int8_t* __
     for (int u = 0; u < kUnroll; ++u) {
       const long long c = (b0 + u) * kQuantBlock + lane;
       if (c >= d) break;
-      const float scale = scale_of(exps[row * nb + b0 + u]);
+      const float scale = scale8_of(exps[row * nb + b0 + u]);
       const float g = kMode == kRestoreSiluGrad ? to_float<T>(grad[row * d + c]) : 0.0f;
-      out[row * d + c] = from_float<T>(restored<T, kMode>(codes[row * d + c], scale, g));
+      float x = decoded<T, kMode>(static_cast<float>(codes[row * d + c]), scale), none = 0.0f;
+      restored2<T, kMode>(x, none, g, 0.0f);
+      out[row * d + c] = from_float<T>(x);
     }
   }
 }

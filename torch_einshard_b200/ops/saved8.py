@@ -29,7 +29,10 @@ torch with the same results.  An extension of this framework: the reference
 keeps activations whole or recomputes them.
 """
 
+import math
 import string
+from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -103,13 +106,14 @@ class Saved8:
     kept.  ``restore()`` gives the values that backward sees.
     """
 
-    __slots__ = ("value", "codes", "exps", "_act", "_base", "_order")
+    __slots__ = ("value", "codes", "exps", "_act", "_base", "_order", "_pre")
 
-    def __init__(self, value, codes, exps, act=False, base=None, order=None):
+    def __init__(self, value, codes, exps, act=False, base=None, order=None, pre=None):
         self.value, self.codes, self.exps = value, codes, exps
         self._act = act  # the codes are a pre-activation: the operand is its silu
         self._base = tuple(value.shape) if base is None else base  # shape of the tensor that was quantised
         self._order = order  # permutation from there to the value's axes
+        self._pre = pre  # the pre-activation's place in the graph (a tensor without values of its own)
 
     @property
     def shape(self):
@@ -134,7 +138,8 @@ class Saved8:
 
     def with_value(self, value):
         """The same codes for a value that differs by its place in the graph alone."""
-        return Saved8(value, self.codes, self.exps, self._act, self._base, self._order)
+        pre = self._pre if value is self.value else None
+        return Saved8(value, self.codes, self.exps, self._act, self._base, self._order, pre)
 
     def _meta(self):
         return self._act, self._base, self._order, self.value.dtype
@@ -165,8 +170,8 @@ def checkpoint8(x):
 
 # ------------------------------------------------------------------ contractions
 
-def _explicit(equation, x_rank, y_rank):
-    """The equation with an ellipsis of the first operand written out."""
+def _explicit(equation, x_rank):
+    """The equation with an ellipsis of the first operand written out, or None."""
     if "..." not in equation:
         return equation
     (ex, ey), ez = equation.split("->")[0].split(","), equation.split("->")[1]
@@ -178,6 +183,72 @@ def _explicit(equation, x_rank, y_rank):
     return f"{ex.replace('...', fill)},{ey}->{ez.replace('...', fill)}"
 
 
+def _inverse(order):
+    back = [0] * len(order)
+    for i, o in enumerate(order):
+        back[o] = i
+    return tuple(back)
+
+
+def _moved(t, order):
+    return t if order is None else t.permute(order)
+
+
+def _order(names, wanted):
+    """Permutation that brings axes ``names`` into the order ``wanted`` (None: they are in it)."""
+    order = tuple(names.index(c) for c in wanted)
+    return None if order == tuple(range(len(order))) else order
+
+
+@dataclass(frozen=True)
+class _Product:
+    """A two-operand contraction as [batch, rows, red] x [batch, red, cols]."""
+
+    equation: str
+    gemm: tuple       # batch, rows, cols, red extents
+    x_order: tuple    # x's axes to batch + rows + red, y's to batch + red + cols, the product's to the result's
+    y_order: tuple
+    z_order: tuple
+    x_shape: tuple    # lengths in those orders
+    y_shape: tuple
+    z_shape: tuple    # (of the product)
+
+    def operand_x(self, x):
+        B, M, _, K = self.gemm
+        return _moved(x, self.x_order).reshape(B, M, K)
+
+    def operand_y(self, y):
+        B, _, N, K = self.gemm
+        return _moved(y, self.y_order).reshape(B, K, N)
+
+    def result(self, z):
+        return _moved(z.view(self.z_shape), self.z_order)
+
+    def product_of(self, z):
+        """A tensor of the result's axes as [batch, rows, cols]."""
+        B, M, N, _ = self.gemm
+        return _moved(z, None if self.z_order is None else _inverse(self.z_order)).reshape(B, M, N)
+
+
+@lru_cache(maxsize=1024)
+def _product(equation, x_shape, y_shape):
+    explicit = _explicit(equation, len(x_shape))
+    plan = None if explicit is None else canonical_gemm(explicit, x_shape, y_shape)
+    if plan is None or plan["x_only"] or plan["y_only"]:
+        raise NotImplementedError("a Saved8 operand takes part in plain two-operand contractions only: no repeated, "
+                                  "broadcast or summed-out axes")
+    size = plan["size"]
+    batch, rows, cols, red = (plan[k] for k in ("batch", "rows", "cols", "red"))
+
+    def lengths(letters):
+        return tuple(size[c] for c in letters)
+
+    extents = tuple(math.prod(lengths(k)) for k in (batch, rows, cols, red))
+    return _Product(explicit, extents, _order(list(plan["ex"]), batch + rows + red),
+                    _order(list(plan["ey"]), batch + red + cols), _order(batch + rows + cols, list(plan["ez"])),
+                    lengths(batch + rows + red), lengths(batch + red + cols), lengths(batch + rows + cols))
+
+
 def _silu_forward(h, dtype):
     """(silu(h) in dtype, codes, exps) of an fp32 (fp64) [rows, d] pre-activation."""
     if h.dtype == torch.float32 and _on_kernels(h, dtype):
@@ -186,95 +257,100 @@ def _silu_forward(h, dtype):
     return (h * torch.sigmoid(h)).to(dtype), codes, exps
 
 
-def _inverse(order):
-    back = [0] * len(order)
-    for i, o in enumerate(order):
-        back[o] = i
-    return back
+def _silu_grad(grad, codes, exps, order):
+    """grad * silu'(h^), in grad's axes; ``order`` leads from the quantised tensor's axes to them."""
+    g = _moved(grad, None if order is None else _inverse(order))
+    d = _restored(codes, exps, grad.dtype, _SILU_GRAD, g.reshape(codes.shape).contiguous()).view(g.shape)
+    return _moved(d, order)
 
 
-def _extents(plan):
-    return [_product(plan["size"][c] for c in plan[k]) for k in ("batch", "rows", "cols", "red")]
+def _place_of(a):
+    """A tensor that stands for a's pre-activation in the graph: its shape, without values."""
+    return a.new_empty(()).expand(a.shape)
 
 
-def _product(sizes):
-    out = 1
-    for s in sizes:
-        out *= s
-    return out
+class _Contraction8(torch.autograd.Function):
+    """x y with x kept in 8 bits.
 
-
-def _act_layout(plan, x, y):
-    """How the pre-activation is kept: (on the native GEMM, shape of the quantised tensor, permutation from its
-    axes to the result's).  The native product is quantised as it comes, [batch, rows, cols]."""
-    size, ez = plan["size"], plan["ez"]
-    if all(_extents(plan)) and gemm.eligible(x, y):
-        letters = plan["batch"] + plan["rows"] + plan["cols"]
-        return True, tuple(size[c] for c in letters), [letters.index(c) for c in ez]
-    return False, tuple(size[c] for c in ez), None
-
-
-def _product_silu(plan, equation, layout, x, y):
-    """(silu of the contraction, codes, exps of its pre-activation)."""
-    native, base, order = layout
-    if native:
-        batch, rows, cols, red = (plan[k] for k in ("batch", "rows", "cols", "red"))
-        B, M, N, K = _extents(plan)
-        xv = x.permute([plan["ex"].index(c) for c in batch + rows + red]).reshape(B, M, K)
-        yv = y.permute([plan["ey"].index(c) for c in batch + red + cols]).reshape(B, K, N)
-        h = gemm.native_bmm(xv, yv, out_dtype=torch.float32)
-        a, codes, exps = _silu_forward(h.view(B * M, N), x.dtype)
-        return a.view(base).permute(order), codes, exps
-    wide = torch.promote_types(x.dtype, torch.float32)
-    h = contract(equation, x.to(wide), y.to(wide))
-    a, codes, exps = _silu_forward(_rows(h) if h.dim() else h.view(1, 1), x.dtype)
-    return a.view(base), codes, exps
-
-
-class _SavedContraction(torch.autograd.Function):
-    """x y with x kept in 8 bits; with a ``layout``, silu of it and its pre-activation in 8 bits."""
+    ``x`` carries the values.  Its gradient goes to ``x``, or, where x is a
+    silu, to ``pre``, its pre-activation's place in the graph (``x`` is detached
+    then).  With ``silu`` the result is silu(x y), its pre-activation in 8 bits
+    and that one's place."""
 
     @staticmethod
-    def forward(ctx, x, y, equation, plan, codes, exps, meta, layout):
+    def forward(ctx, x, pre, y, plan, native, codes, exps, meta, silu):
         ctx.set_materialize_grads(False)
-        ctx.equation, ctx.meta, ctx.layout = equation, meta, layout
-        if layout is None:
+        ctx.plan, ctx.native, ctx.meta, ctx.silu = plan, native, meta, silu
+        mod = _native.require() if native else None
+        if not silu:
             ctx.save_for_backward(y, codes, exps)
-            return contract(equation, x, y)
-        a, h_codes, h_exps = _product_silu(plan, equation, layout, x, y)
+            if native:
+                return plan.result(gemm.native_bmm(plan.operand_x(x), plan.operand_y(y)))
+            return contract(plan.equation, x, y)
+        if native:
+            xv, yv = gemm._prepare(plan.operand_x(x)), gemm._prepare(plan.operand_y(y))
+            a, h_codes, h_exps = mod.gemm_silu8(xv, yv, _native.error_word(x.device))
+            a = plan.result(a)
+        else:
+            wide = torch.promote_types(x.dtype, torch.float32)
+            h = contract(plan.equation, x.to(wide), y.to(wide))
+            a, h_codes, h_exps = _silu_forward(_rows(h) if h.dim() else h.view(1, 1), x.dtype)
+            a = a.view(h.shape)
         ctx.save_for_backward(y, codes, exps, h_codes, h_exps)
         ctx.mark_non_differentiable(h_codes, h_exps)
-        return a, h_codes, h_exps
+        return a, _place_of(a), h_codes, h_exps
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, grad, *_):
-        if grad is None:
-            return (None,) * 8
+    def backward(ctx, grad, grad_pre=None, *_):
         y, codes, exps = ctx.saved_tensors[:3]
-        if ctx.layout is not None:
-            grad = _silu_grad(grad, *ctx.saved_tensors[3:], ctx.layout)
-        (ex, ey), ez = ctx.equation.split("->")[0].split(","), ctx.equation.split("->")[1]
-        dx = dy = None
-        if ctx.needs_input_grad[0]:
-            dx = contract(f"{ez},{ey}->{ex}", grad, y)
-        if ctx.needs_input_grad[1]:
-            x = _restore_operand(codes, exps, ctx.meta)
-            own = next((c for c in ey if c not in ex or c not in ez), "")
-            # the product's rows are the letters that come first in y: its gradient comes out in y's order
-            if own and own in ez:
-                dy = contract(f"{ez},{ex}->{ey}", grad, x)
-            else:
-                dy = contract(f"{ex},{ez}->{ey}", x, grad)
-        return dx, dy, None, None, None, None, None, None
+        plan, native = ctx.plan, ctx.native
+        if grad is not None and ctx.silu:
+            grad = _silu_grad(grad, *ctx.saved_tensors[3:], plan.z_order if native else None)
+        if grad_pre is not None:
+            grad = grad_pre if grad is None else grad + grad_pre
+        if grad is None:
+            return (None,) * 9
+        want_x, want_pre, want_y = ctx.needs_input_grad[:3]
+        act, base, order, dtype = ctx.meta
+        dx = dpre = dy = restored = None
+        if native:
+            gz, yv = plan.product_of(grad), plan.operand_y(y)
+            yt = yv.transpose(1, 2)
+            if want_pre and _same_rows(plan, codes, base, order):
+                # (dz y^T) silu'(h^) and silu(h^) from one product
+                gz = gemm._prepare(gz)
+                dpre, restored = _native.require().gemm_silu8_grad(gz, gemm._prepare(yt), codes, exps,
+                                                                   _native.error_word(gz.device))
+                dpre = _moved(dpre.view(plan.x_shape), None if plan.x_order is None else _inverse(plan.x_order))
+            elif want_x or want_pre:
+                dx = gemm.native_bmm(gz, yt).view(plan.x_shape)
+                dx = _moved(dx, None if plan.x_order is None else _inverse(plan.x_order))
+            if want_y:
+                if restored is None:
+                    restored = plan.operand_x(_restore_operand(codes, exps, ctx.meta))
+                # a transposed y (an [out, in] weight) gets its gradient in its own memory order
+                if yv.stride(1) == 1 and yv.size(1) > 1:
+                    dy = gemm.native_bmm(gz.transpose(1, 2), restored).transpose(1, 2)
+                else:
+                    dy = gemm.native_bmm(restored.transpose(1, 2), gz)
+                dy = _moved(dy.reshape(plan.y_shape), None if plan.y_order is None else _inverse(plan.y_order))
+        else:
+            (ex, ey), ez = plan.equation.split("->")[0].split(","), plan.equation.split("->")[1]
+            if want_x or want_pre:
+                dx = contract(f"{ez},{ey}->{ex}", grad, y)
+            if want_y:
+                dy = contract(f"{ez},{ex}->{ey}", grad, _restore_operand(codes, exps, ctx.meta))
+        if want_pre and dpre is None:
+            dpre = _silu_grad(dx, codes, exps, order)
+        return dx if want_x else None, dpre, dy, None, None, None, None, None, None
 
 
-def _silu_grad(grad, codes, exps, layout):
-    """grad * silu'(h^), in grad's axes."""
-    _, _, order = layout
-    g = grad if order is None else grad.permute(_inverse(order))
-    d = _restored(codes, exps, grad.dtype, _SILU_GRAD, g.reshape(codes.shape).contiguous()).view(g.shape)
-    return d if order is None else d.permute(order)
+def _same_rows(plan, codes, base, order):
+    """Whether the pre-activation was quantised in the very rows this product reads."""
+    B, M, _, K = plan.gemm
+    identity = order is None or tuple(order) == tuple(range(len(order)))
+    return identity and plan.x_order is None and codes.shape == (B * M, K) and codes.numel() > 0
 
 
 def contract_saved(equation, saved, y, activation=None):
@@ -285,16 +361,17 @@ def contract_saved(equation, saved, y, activation=None):
     if y.dtype != x.dtype or y.device != x.device:
         raise ValueError(f"a Saved8 operand of {x.dtype} on {x.device} needs the other one alike, "
                          f"not {y.dtype} on {y.device}")
-    explicit = _explicit(equation, x.dim(), y.dim())
-    plan = None if explicit is None else canonical_gemm(explicit, tuple(x.shape), tuple(y.shape))
-    if plan is None or plan["x_only"] or plan["y_only"]:
-        raise NotImplementedError("a Saved8 operand takes part in plain two-operand contractions only: no repeated, "
-                                  "broadcast or summed-out axes")
-    layout = None if activation is None else _act_layout(plan, x, y)
-    out = _SavedContraction.apply(x, y, explicit, plan, saved.codes, saved.exps, saved._meta(), layout)
-    if layout is None:
+    plan = _product(equation, tuple(x.shape), tuple(y.shape))
+    native = all(plan.gemm) and gemm.eligible(x, y)
+    pre = saved._pre
+    out = _Contraction8.apply(x if pre is None else x.detach(), pre, y, plan, native, saved.codes, saved.exps,
+                              saved._meta(), activation is not None)
+    if activation is None:
         return out
-    return Saved8(*out, True, *layout[1:])
+    a, pre, codes, exps = out
+    if native:
+        return Saved8(a, codes, exps, True, plan.z_shape, plan.z_order, pre)
+    return Saved8(a, codes, exps, True, None, None, pre)
 
 
 class _SiluSaved(torch.autograd.Function):
@@ -310,7 +387,7 @@ class _SiluSaved(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad, *_):
-        return None if grad is None else _silu_grad(grad, *ctx.saved_tensors, (False, None, None))
+        return None if grad is None else _silu_grad(grad, *ctx.saved_tensors, None)
 
 
 def silu_saved(h):
