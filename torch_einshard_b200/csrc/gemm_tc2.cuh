@@ -42,14 +42,11 @@ struct SharedState2 {
   int epi[32];
 };
 
-// The kernel body; tmD: a second output map for epilogues that write two tensors
-// (EpiTile.tmw).  Those have a second staging buffer per epilogue warp behind the
-// first ones (kSmem2DualBytes).
-constexpr int kSmem2DualBytes = kSmem2Bytes + 4 * kStage2Out;
-
-template <class Epi>
+// The kernel body.  kEpiWarps 4 hands the policy 256 columns a warp; 8 hands it 128
+// (two warps a lane quadrant, for longer epilogues).
+template <class Epi, int kEpiWarps>
 __device__ __forceinline__ void gemm_tc2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmC,
-                                              const CUtensorMap& tmD, const GemmShape& shp, Epi& epi) {
+                                              const GemmShape& shp, Epi& epi) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -72,7 +69,7 @@ __device__ __forceinline__ void gemm_tc2_body(const CUtensorMap& tmA, const CUte
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&st->tfull[a], 1);
-      mbar_init(&st->tempty[a], 2 * (kEpiThreads / 32));
+      mbar_init(&st->tempty[a], 2 * kEpiWarps);
     }
     mbar_init(&st->drain, 1);
     st->abort_flag = 0;
@@ -189,6 +186,8 @@ __device__ __forceinline__ void gemm_tc2_body(const CUtensorMap& tmA, const CUte
   } else {
     // ------------------------------------------------------------ epilogue (both CTAs)
     const int q = warp & 3;
+    const int part = (warp - 2) >> 2;
+    constexpr int kCols = kBN / (kEpiWarps / 4);
     uint32_t tc = 0;
     for (int p = cluster; p < pairs; p += nclusters, ++tc) {
       const uint32_t acc = tc & 1u;
@@ -198,14 +197,14 @@ __device__ __forceinline__ void gemm_tc2_body(const CUtensorMap& tmA, const CUte
       EpiTile et;
       et.t = 2 * p + static_cast<int>(rank);
       et.c = tile_coord(shp, et.t);
-      et.tmem = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * kBN;
+      et.c.n0 += part * kCols;
+      et.tmem = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * kBN + part * kCols;
       et.row = q * 32 + lane;
       et.q = q;
       et.lane = lane;
       et.tmc = &tmC;
-      et.tmw = &tmD;
-      et.stage = out_stage + q * kStage2Out;
-      const bool ok = epi.tile(et, shp, abort_flag);
+      et.stage = out_stage + (kEpiWarps == 4 ? q : warp - 2) * kStage2Out;
+      const bool ok = et.c.n0 < shp.N ? epi.tile(et, shp, abort_flag) : true;
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster(tempty_leader0 + acc * 8);
@@ -231,16 +230,20 @@ template <class Epi>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmC, const GemmShape shp, Epi epi) {
-  gemm_tc2_body(tmA, tmB, tmC, tmC, shp, epi);
+  gemm_tc2_body<Epi, 4>(tmA, tmB, tmC, shp, epi);
 }
 
-// Two outputs.
+// For epilogues that are long and store from registers: eight epilogue warps, no
+// staging buffers.
+constexpr int kLongEpiWarps = 8;
+constexpr int kLongThreads = 64 + 32 * kLongEpiWarps;
+constexpr int kSmem2LongBytes = kStages2 * kStage2Bytes + 1024 + 1024;
+
 template <class Epi>
-__global__ void __launch_bounds__(kThreads, 1)
-    gemm_tc2_dual_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
-                         const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmD,
+__global__ void __launch_bounds__(kLongThreads, 1)
+    gemm_tc2_long_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                          const GemmShape shp, Epi epi) {
-  gemm_tc2_body(tmA, tmB, tmC, tmD, shp, epi);
+  gemm_tc2_body<Epi, kLongEpiWarps>(tmA, tmB, tmA, shp, epi);
 }
 
 }  // namespace es
