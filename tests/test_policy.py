@@ -436,6 +436,52 @@ def test_other_stream_and_capture():
                 assert torch.equal(a, b)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_backward_captured_apart_from_forward(dtype):
+    """An eager forward pass, its backward pass captured and replayed with other upstream gradients; and a captured
+    forward pass with an eager backward pass, whose result a later replay leaves alone."""
+    t = off_border(make("cuda", dtype, 2, 9, 130), 0.2, 0.2)
+    z = t.pop("logits").requires_grad_(True)
+    factor = torch.ones((), device="cuda")
+
+    def gradient(scale):
+        loss = es.einpolicy("b s v", z, axis="v", kl=0.1, **t).loss
+        return torch.autograd.grad(loss, z, torch.tensor(scale, device="cuda"))[0]
+
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        loss = es.einpolicy("b s v", z, axis="v", kl=0.1, **t).loss
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        (g,) = torch.autograd.grad(loss, z, factor)
+    for scale in (0.5, 1.0, 1.0, 2.0, 0.0, 1.0):
+        factor.fill_(scale)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(g, gradient(scale))
+    del loss
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        loss = es.einpolicy("b s v", z, axis="v", kl=0.1, **t).loss
+    graph.replay()
+    torch.cuda.synchronize()
+    (g,) = torch.autograd.grad(loss, z, retain_graph=True)
+    want = gradient(1.0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(g, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [(1, 16385), (4100, 5), (3, 7001)])
+@pytest.mark.parametrize("reduction", ["mean", "sequence", "sum"])
+def test_many_tokens(tokens, reduction):
+    check(off_border(make("cuda", torch.float32, *tokens, 40, advantage="sequence"), 0.2, 0.2), reduction=reduction)
+
+
 @pytest.fixture
 def one_rank_mesh(request):
     from torch.distributed.device_mesh import init_device_mesh

@@ -282,21 +282,19 @@ PolicyArgs policy_args(const at::Tensor& logits, const at::Tensor& ids, const Op
   return a;
 }
 
-PolicyState policy_state(const at::Tensor& logp, const at::Tensor& terms, const at::Tensor& norm,
-                         const at::Tensor& weight) {
+PolicyState policy_state(const at::Tensor& terms, const at::Tensor& norm, const at::Tensor& share) {
   PolicyState s;
-  s.logp = logp.data_ptr<float>();
   s.terms = reinterpret_cast<float4*>(terms.data_ptr<float>());
   s.norm = reinterpret_cast<float2*>(norm.data_ptr<float>());
-  s.weight = weight.data_ptr<float>();
+  s.share = share.data_ptr<float>();
   return s;
 }
 
-// (loss, KL, clipped share, logp, terms, norm, weight)
+// (loss, KL, clipped share, logp, terms, norm, token shares) and, with `gradient`, that of the logits and its factors
 std::vector<at::Tensor> policy_forward_op(const at::Tensor& logits, const at::Tensor& ids, const Opt& mask,
                                           const Opt& old, const Opt& ref, const at::Tensor& adv, int64_t length,
                                           double lo, double hi, double kl, double temperature, int64_t reduction,
-                                          double weight) {
+                                          double weight, bool gradient) {
   const c10::cuda::CUDAGuard guard(logits.device());
   const PolicyArgs a = policy_args(logits, ids, mask, old, ref, adv, length, lo, hi, kl, temperature, reduction, weight);
   const auto f32 = logits.options().dtype(at::kFloat);
@@ -304,35 +302,49 @@ std::vector<at::Tensor> policy_forward_op(const at::Tensor& logits, const at::Te
   TORCH_CHECK(a.tokens > 0, "einshard policy loss: no tokens");
   at::Tensor loss = at::empty({}, f32), kl_out = at::empty({}, f32), clipped = at::empty({}, f32);
   at::Tensor logp = at::empty({a.tokens}, f32), terms = at::empty({a.tokens, 4}, f32);
-  at::Tensor norm = at::empty({a.tokens, 2}, f32), weights = at::empty({sequences}, f32);
-  at::Tensor sums = at::empty({sequences, 4}, f32);
-  PolicyState s = policy_state(logp, terms, norm, weights);
+  at::Tensor norm = at::empty({a.tokens, 2}, f32), shares = at::empty({sequences}, f32);
+  at::Tensor sums = at::empty({policy_sum_blocks(a.tokens), 4}, f32);
+  PolicyState s = policy_state(terms, norm, shares);
+  s.logp = logp.data_ptr<float>();
   s.sums = reinterpret_cast<float4*>(sums.data_ptr<float>());
   s.loss = loss.data_ptr<float>();
   s.kl = kl_out.data_ptr<float>();
   s.clipped = clipped.data_ptr<float>();
+  std::vector<at::Tensor> out{loss, kl_out, clipped, logp, terms, norm, shares};
+  if (gradient) {
+    out.push_back(at::empty(logits.sizes(), logits.options()));
+    out.push_back(at::empty({a.tokens}, f32));
+    s.dlogits = out[7].data_ptr();
+    s.factors = out[8].data_ptr<float>();
+  }
   int launches = 0;
-  counted(policy_forward(a, s, at::cuda::getCurrentCUDAStream(), &launches), "policy loss", 0);
-  g_count->fetch_add(launches, std::memory_order_relaxed);
-  return {loss, kl_out, clipped, logp, terms, norm, weights};
+  const int rc = policy_forward(a, s, at::cuda::getCurrentCUDAStream(), &launches);
+  counted(rc, "policy loss", launches);
+  return out;
 }
 
+// The gradient of the logits; in `kept` (with its factors), which the forward pass wrote, or a new tensor.
 at::Tensor policy_backward_op(const at::Tensor& grad, const at::Tensor& logits, const at::Tensor& ids,
                               const Opt& mask, const Opt& old, const Opt& ref, const at::Tensor& adv, int64_t length,
-                              double lo, double hi, double kl, double temperature, int64_t reduction, double weight_factor,
-                              const at::Tensor& terms, const at::Tensor& norm, const at::Tensor& weight) {
+                              double lo, double hi, double kl, double temperature, int64_t reduction, double weight,
+                              const at::Tensor& terms, const at::Tensor& norm, const at::Tensor& shares,
+                              const Opt& kept, const Opt& factors) {
   const c10::cuda::CUDAGuard guard(logits.device());
-  const PolicyArgs a = policy_args(logits, ids, mask, old, ref, adv, length, lo, hi, kl, temperature, reduction, weight_factor);
+  const PolicyArgs a = policy_args(logits, ids, mask, old, ref, adv, length, lo, hi, kl, temperature, reduction, weight);
   TORCH_CHECK(grad.device() == logits.device() && grad.numel() == 1 && grad.scalar_type() == at::kFloat,
               "einshard policy loss: fp32 gradient of the loss");
+  TORCH_CHECK(a.tokens > 0, "einshard policy loss: no tokens");
   per_token(terms, logits, 4 * a.tokens, at::kFloat, "terms");
   per_token(norm, logits, 2 * a.tokens, at::kFloat, "norms");
-  per_token(weight, logits, a.tokens / length, at::kFloat, "weights");
-  TORCH_CHECK(a.tokens > 0, "einshard policy loss: no tokens");
-  at::Tensor out = at::empty(logits.sizes(), logits.options());
-  const PolicyState s = policy_state(terms, terms, norm, weight);
-  counted(policy_backward(a, s, grad.data_ptr<float>(), out.data_ptr(), at::cuda::getCurrentCUDAStream()),
-          "policy loss backward");
+  per_token(shares, logits, a.tokens / length, at::kFloat, "token shares");
+  TORCH_CHECK(kept.has_value() == factors.has_value(), "einshard policy loss: a kept gradient has factors");
+  per_token(kept, logits, a.tokens * a.vocab, logits.scalar_type(), "kept gradient");
+  per_token(factors, logits, a.tokens, at::kFloat, "factors");
+  at::Tensor out = kept.has_value() ? *kept : at::empty(logits.sizes(), logits.options());
+  PolicyState s = policy_state(terms, norm, shares);
+  s.dlogits = out.data_ptr();
+  s.factors = factors.has_value() ? factors->data_ptr<float>() : nullptr;
+  counted(policy_backward(a, s, grad.data_ptr<float>(), at::cuda::getCurrentCUDAStream()), "policy loss backward");
   return out;
 }
 

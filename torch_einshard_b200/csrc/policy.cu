@@ -9,24 +9,40 @@
 // sequence's tokens) or 1.  A masked token has no loss and a gradient of zeros,
 // whatever its logits, id and other inputs hold: its row is not read.
 //
-// Forward, a block reads a token's row once with a running maximum m and sum s
-// of 2^((z - m) log2(e) / T) a thread; z - m is formed before the scaling, so
-// rows of the type's lowest value or of very large logits keep their
-// differences.  Bound by the read: 2 bytes a 16-bit logit, against 16
-// exponentials a clock and SM.  Backward reads the row again and writes the
-// gradient (a row whose c is 0, masked or clipped, is written without being read).
+// A block reads a token's row with a running maximum m and sum s of
+// 2^((z - m) log2(e) / T) a thread; for very large m (rows of the type's lowest
+// value) the difference is formed before the scaling.  The
+// weights depend on the mask alone, so a training step's forward pass goes on to
+// write the row's gradient for g = 1 while the row is still in L2: memory moves
+// 2 + 2 bytes a 16-bit logit instead of the 2 + 2 + 2 of separate passes.  The
+// backward pass then only looks at g; where it is not 1 it forms the gradient
+// again from the logits, in 32 bits, so that nothing is rounded twice and a small
+// fp16 gradient is scaled before it could vanish.  What a row's gradient was formed
+// for is kept beside it (`factors`), so that running the backward pass again, as
+// the replay of a captured graph does, gives the gradient for the g of that run.
+// A row whose c is 0 (clipped) is written without a second read.
+//
+// Bounds: memory, then the exponentials (one a logit and pass, 16 a clock and SM).
 // Rows need no alignment: up to seven logits at either end are taken one by one.
 #include "policy.h"
 
 #include "gemm.h"
 #include "vec.cuh"
 
+#include <type_traits>
+
 namespace es {
 namespace {
 
-constexpr int kThreads = 512;
 constexpr int kUnroll = 4;
 constexpr float kLog2e = 1.4426950408889634f;
+
+// The larger one, NaN if either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -34,256 +50,545 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// Logits beyond this take differences before they are scaled (their products with c could overflow).
+constexpr float kHuge = 1e30f;
+
 // Running maximum and sum of 2^((z - m) c).
 struct Running {
   float m, s;
   __device__ __forceinline__ static float base(float m) { return m == -INFINITY ? 0.0f : m; }
-  __device__ __forceinline__ void raise(float top, float c) {
-    if (top > m) {
-      s *= exp2_fast((m - base(top)) * c);  // m = -inf: s is 0 and stays it
-      m = top;
-    }
-  }
-  __device__ __forceinline__ void add(float z, float c) {
-    raise(z, c);
-    s += exp2_fast((z - base(m)) * c);
-  }
+  __device__ __forceinline__ void add(float z, float c) { merge(z, 1.0f, c); }
   __device__ __forceinline__ void merge(float m2, float s2, float c) {
-    const float top = fmaxf(m, m2);
+    const float top = max_nan(m, m2);
     const float b = base(top);
     s = s * exp2_fast((m - b) * c) + s2 * exp2_fast((m2 - b) * c);
     m = top;
+  }
+  // Joined over the warp: the maximum as an integer of the same order (a NaN ends up in s), one scaling, the sum.
+  __device__ __forceinline__ void over_warp(float c) {
+    const int bits = __float_as_int(m);
+    const int top = __reduce_max_sync(0xffffffffu, bits ^ ((bits >> 31) & 0x7fffffff));
+    const float largest = __int_as_float(top ^ ((top >> 31) & 0x7fffffff));
+    s = warp_sum(s * exp2_fast((m - base(largest)) * c));
+    m = largest;
+  }
+};
+
+// The same over a thread's chunks.  2^(z c - q) takes one FMA before the
+// exponential, exact up to its one rounding for any q; q is m c rounded, and
+// close() makes up for that rounding.
+struct ChunkSum {
+  float m = -INFINITY, q = 0.0f, s = 0.0f;
+  __device__ __forceinline__ void raise(float top, float c) {
+    if (top > m) {
+      const float next = fabsf(top) < kHuge ? top * c : 0.0f;
+      if (m == -INFINITY) {
+        // nothing summed yet but zeros
+      } else if (fabsf(m) < kHuge && fabsf(top) < kHuge) {
+        s *= exp2_fast(q - next);
+      } else {
+        close(c);
+        s *= exp2_fast((m - top) * c);
+        if (fabsf(top) < kHuge) s *= exp2_fast(fmaf(top, c, -next));
+      }
+      m = top;
+      q = next;
+    }
+  }
+  // s relative to 2^(m c) exactly
+  __device__ __forceinline__ void close(float c) {
+    if (fabsf(m) < kHuge) s *= exp2_fast(-fmaf(m, c, -q));
+  }
+  __device__ __forceinline__ Running total(float c) {
+    close(c);
+    return {m, s};
   }
 };
 
 // Elements before the first 16-byte boundary of a row.
 template <typename T>
-__device__ __forceinline__ int head_of(const T* row, long long n) {
+__device__ __forceinline__ int head_of(const T* row, int n) {
   const int off = static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
   const int head = off == 0 ? 0 : static_cast<int>(16 / sizeof(T)) - off;
-  return head < n ? head : static_cast<int>(n);
+  return head < n ? head : n;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) policy_rows_kernel(const PolicyArgs a, const PolicyState o) {
-  __shared__ float2 red[kThreads / 32];
-  const float c = a.inv_temp * kLog2e;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  for (long long t = blockIdx.x; t < a.tokens; t += gridDim.x) {
-    if (a.mask != nullptr && !a.mask[t]) {  // uniform
-      if (threadIdx.x == 0) {
-        o.logp[t] = 0.0f;
-        o.terms[t] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        o.norm[t] = make_float2(0.0f, 0.0f);
-      }
-      continue;
+// Eight columns from j0 of a token's gradient k (1[j = id] - 2^((z_j - norm.x) c - norm.y)).
+struct GradientRow {
+  float k, c, off, factor, m;
+  int id;
+  bool huge;
+  __device__ __forceinline__ GradientRow(float k_, float2 norm, int id_, float c_) : k(k_), c(c_), m(norm.x), id(id_) {
+    huge = !(fabsf(norm.x) < kHuge);
+    // 2^(z c - q) and a factor for what the rounding of q = m c left, with the sum's
+    const float q = huge ? 0.0f : norm.x * c;
+    off = -q;
+    factor = -k * exp2_fast((huge ? 0.0f : -fmaf(norm.x, c, -q)) - norm.y);
+  }
+  __device__ __forceinline__ float minus_p(float z) const {
+    return factor * exp2_fast(huge ? (z - m) * c : fmaf(z, c, off));
+  }
+  // (scalar arithmetic: the exponentials' results would have to be moved into pairs)
+  template <typename T>
+  __device__ __forceinline__ void put(T* out, int j0, const Raw8<T>& raw) const {
+    float z[8];
+    unpack8(raw, z);
+    if (huge) {  // uniform
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = minus_p(z[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = factor * exp2_fast(fmaf(z[e], c, off));
     }
-    const T* row = static_cast<const T*>(a.logits) + t * a.ld;
-    const int head = head_of(row, a.vocab);
-    const T* body = row + head;
-    const long long chunks = (a.vocab - head) / 8;
-    Running r{-INFINITY, 0.0f};
-    for (long long i = threadIdx.x; i < chunks; i += kThreads * kUnroll) {
+    const uint32_t at = static_cast<uint32_t>(id - j0);
+    if (at < 8u) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e == static_cast<int>(at)) z[e] += k;
+    }
+    store8(out, z);
+  }
+  __device__ __forceinline__ float one(float z, int j) const { return minus_p(z) + (j == id ? k : 0.0f); }
+};
+
+// A token's gradient row; zeros for k = 0 without reading the logits.
+template <typename T>
+__device__ __forceinline__ void gradient_row(const T* row, T* out, int vocab, float k, float2 norm, int id, float c) {
+  const bool zero = k == 0.0f;  // NaN is not zero
+  const int head = head_of(out, vocab);
+  const bool vec = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+  const int chunks = (vocab - head) / 8, threads = static_cast<int>(blockDim.x), tid = static_cast<int>(threadIdx.x);
+  const GradientRow g(k, norm, id, c);
+  auto one = [&](int j) { out[j] = from_float<T>(zero ? 0.0f : g.one(to_float<T>(row[j]), j)); };
+  if (zero) {
+    const Pair nil[4] = {0ull, 0ull, 0ull, 0ull};
+    for (int i = tid; i < chunks; i += threads) store8(out + head + i * 8, nil);
+  } else if (vec) {
+    const int stride = threads * 8;
+    int i = tid, j = head + tid * 8;
+    const T* p = row + j;
+    T* q = out + j;
+    for (; i + (kUnroll - 1) * threads < chunks; i += kUnroll * threads) {
       Raw8<T> raw[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (i + u * kThreads < chunks) raw[u] = load8_stream(body + (i + u * kThreads) * 8);
+      for (int u = 0; u < kUnroll; ++u) raw[u] = load8_stream(p + u * stride);
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        if (i + u * kThreads >= chunks) break;
-        float z[8];
-        unpack8(raw[u], z);
-        float top = z[0];
-#pragma unroll
-        for (int k = 1; k < 8; ++k) top = fmaxf(top, z[k]);
-        r.raise(top, c);
-        const float b = Running::base(r.m);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) r.s += exp2_fast((z[k] - b) * c);
-      }
+      for (int u = 0; u < kUnroll; ++u) g.put(q + u * stride, j + u * stride, raw[u]);
+      p += kUnroll * stride, q += kUnroll * stride, j += kUnroll * stride;
     }
-    // the ends of the row
-    const int tail = static_cast<int>(a.vocab - head - chunks * 8);
-    if (static_cast<int>(threadIdx.x) < head) r.add(to_float<T>(row[threadIdx.x]), c);
-    if (static_cast<int>(threadIdx.x) < tail) r.add(to_float<T>(body[chunks * 8 + threadIdx.x]), c);
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1)
-      r.merge(__shfl_xor_sync(0xffffffffu, r.m, off), __shfl_xor_sync(0xffffffffu, r.s, off), c);
-    __syncthreads();  // the previous token's words are read
-    if (lane == 0) red[warp] = make_float2(r.m, r.s);
-    __syncthreads();
-    if (warp == 0) {
-      const float2 v = lane < kThreads / 32 ? red[lane] : make_float2(-INFINITY, 0.0f);
-      r.m = v.x;
-      r.s = v.y;
-#pragma unroll
-      for (int off = 16; off > 0; off >>= 1)
-        r.merge(__shfl_xor_sync(0xffffffffu, r.m, off), __shfl_xor_sync(0xffffffffu, r.s, off), c);
-      if (lane == 0) {
-        const int64_t id = a.ids[t];
-        // an id outside the vocabulary makes the loss NaN
-        const float z = id >= 0 && id < a.vocab ? to_float<T>(row[id]) : __uint_as_float(0x7fc00000u);
-        const float lp = (z - r.m) * a.inv_temp - logf(r.s);
-        const float adv = a.adv[a.adv_per_sequence ? t / a.length : t];
-        const float ratio = a.old != nullptr ? expf(lp - a.old[t]) : expf(lp - lp);
-        const float kept = fminf(fmaxf(ratio, 1.0f - a.lo), 1.0f + a.hi);
-        const float s1 = ratio * adv, s2 = kept * adv;
-        const bool clipped = s1 > s2;
-        float loss = 0.0f, slope = 0.0f, kl = 0.0f;
-        if (adv != 0.0f) {
-          loss = clipped ? -s2 : -s1;
-          slope = clipped ? 0.0f : -s1;
-        }
-        if (a.ref != nullptr) {
-          const float away = a.ref[t] - lp;
-          const float rise = expm1f(away);
-          kl = rise - away;
-          loss += a.kl * kl;
-          slope -= a.kl * rise;
-        }
-        o.logp[t] = lp;
-        o.terms[t] = make_float4(loss, kl, clipped ? 1.0f : 0.0f, slope);
-        o.norm[t] = make_float2(r.m, log2f(r.s));
-      }
-    }
+    for (; i < chunks; i += threads, p += stride, q += stride, j += stride) g.put(q, j, load8_stream(p));
+  } else {
+    for (int j = head + tid; j < head + chunks * 8; j += threads) one(j);
+  }
+  const int tail = vocab - head - chunks * 8;
+  if (tid < head) one(tid);
+  if (tid < tail) one(head + chunks * 8 + tid);
+}
+
+// The largest of eight elements.
+template <typename T>
+__device__ __forceinline__ float largest_of(const Raw8<T>& r) {
+  if constexpr (sizeof(T) == 4) {
+    float f[8];
+    unpack8(r, f);
+    return fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+  } else {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2* e = reinterpret_cast<const T2*>(r.w);
+    const T2 m = __hmax2(__hmax2(e[0], e[1]), __hmax2(e[2], e[3]));
+    const float2 f = word_to_floats<T>(*reinterpret_cast<const uint32_t*>(&m));
+    return fmaxf(f.x, f.y);
   }
 }
 
-// Sums of a sequence's terms: block a sequence.
-__global__ void __launch_bounds__(256) policy_sequence_kernel(const PolicyArgs a, const PolicyState o) {
-  __shared__ float4 red[8];
-  const long long q = blockIdx.x;
-  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (long long i = threadIdx.x; i < a.length; i += 256) {
-    const long long t = q * a.length + i;
-    if (a.mask != nullptr && !a.mask[t]) continue;
-    const float4 v = o.terms[t];
-    s.x += v.x, s.y += v.y, s.z += v.z, s.w += 1.0f;
-  }
-  s = make_float4(warp_sum(s.x), warp_sum(s.y), warp_sum(s.z), warp_sum(s.w));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
-  __syncthreads();
+// An id as a column, or -1.
+__device__ __forceinline__ int in_vocabulary(int64_t id, long long vocab) {
+  return id >= 0 && id < vocab ? static_cast<int>(id) : -1;
+}
+
+// A token's sequence.
+__device__ __forceinline__ long long sequence_of(const PolicyArgs& a, long long t) {
+  if (a.tokens < (1ll << 31)) return static_cast<uint32_t>(t) / static_cast<uint32_t>(a.length);
+  return t / a.length;
+}
+
+// A token's share in the reduction.
+__device__ __forceinline__ float share_of(const PolicyArgs& a, const PolicyState& o, long long t) {
+  if (a.reduction == kReduceSum) return 1.0f;
+  if (a.mask == nullptr) return 1.0f / static_cast<float>(a.tokens);  // both means: sequences of one length
+  return o.share[a.reduction == kReduceSequence ? sequence_of(a, t) : 0];
+}
+
+// A token's other inputs, on their way to the first thread while the row is read.
+struct Inputs {
+  float z, adv, old, ref, share;
+};
+
+template <typename T>
+__device__ __forceinline__ Inputs inputs_of(const PolicyArgs& a, const PolicyState& o, const T* row, long long t, int id) {
+  Inputs in{__uint_as_float(0x7fc00000u), 0.0f, 0.0f, 0.0f, 0.0f};
   if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; ++i) s.x += red[i].x, s.y += red[i].y, s.z += red[i].z, s.w += red[i].w;
-    o.sums[q] = s;
+    in.share = share_of(a, o, t);
+    in.adv = a.adv[a.adv_per_sequence ? sequence_of(a, t) : t];
+    if (a.old != nullptr) in.old = a.old[t];
+    if (a.ref != nullptr) in.ref = a.ref[t];
+    if (id >= 0) in.z = to_float<T>(row[id]);  // an id outside the vocabulary makes the loss NaN
+  }
+  return in;
+}
+
+// The token's terms from its row's maximum and sum: loss, KL, clipped, slope.
+__device__ __forceinline__ float4 terms_of(const PolicyArgs& a, const Inputs& in, float m, float s, float* logp) {
+  const float lp = (in.z - m) * a.inv_temp - logf(s);
+  const float ratio = expf(lp - (a.old != nullptr ? in.old : lp));
+  const float kept = fminf(fmaxf(ratio, 1.0f - a.lo), 1.0f + a.hi);
+  const float s1 = ratio * in.adv, s2 = kept * in.adv;
+  const bool clipped = s1 > s2;
+  float loss = 0.0f, slope = 0.0f, kl = 0.0f;
+  if (in.adv != 0.0f) {
+    loss = clipped ? -s2 : -s1;
+    slope = clipped ? 0.0f : -s1;
+  }
+  if (a.ref != nullptr) {
+    const float away = in.ref - lp;
+    const float rise = expm1f(away);
+    kl = rise - away;
+    loss += a.kl * kl;
+    slope -= a.kl * rise;
+  }
+  *logp = lp;
+  return make_float4(loss, kl, clipped ? 1.0f : 0.0f, slope);
+}
+
+__device__ __forceinline__ float coefficient(const PolicyArgs& a, float share, float slope) {
+  return slope == 0.0f ? 0.0f : a.weight * share * slope * a.inv_temp;
+}
+
+// What a token leaves behind for a row's blocks: shared words.
+struct RowWords {
+  float2 red[32];
+  float2 norm;
+  float k;
+};
+
+// The block's maxima and sums joined, the token's terms stored; the row's norm and the gradient's coefficient go to
+// w (behind a barrier of the caller's).
+__device__ __forceinline__ void finish_token(const PolicyArgs& a, const PolicyState& o, RowWords& w, Running r, float c,
+                                             const Inputs& in, long long t) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  r.over_warp(c);
+  __syncthreads();  // the previous token's words are read
+  if (lane == 0) w.red[warp] = make_float2(r.m, r.s);
+  __syncthreads();
+  if (warp != 0) return;
+  const float2 v = lane < static_cast<int>(blockDim.x >> 5) ? w.red[lane] : make_float2(-INFINITY, 0.0f);
+  r.m = v.x;
+  r.s = v.y;
+  r.over_warp(c);
+  if (lane != 0) return;
+  float lp;
+  const float4 terms = terms_of(a, in, r.m, r.s, &lp);
+  const float2 norm = make_float2(r.m, log2f(r.s));
+  o.logp[t] = lp;
+  o.terms[t] = terms;
+  o.norm[t] = norm;
+  if (o.factors != nullptr) o.factors[t] = 1.0f;
+  w.norm = norm;
+  w.k = coefficient(a, in.share, terms.w);
+}
+
+__device__ __forceinline__ void masked_token(const PolicyState& o, long long t) {
+  if (threadIdx.x != 0) return;
+  o.logp[t] = 0.0f;
+  o.terms[t] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  o.norm[t] = make_float2(0.0f, 0.0f);
+  if (o.factors != nullptr) o.factors[t] = 1.0f;
+}
+
+// Exponentials of kCount chunks of eight under one maximum.
+template <typename T, int kCount>
+__device__ __forceinline__ void add_chunks(ChunkSum& r, const Raw8<T> (&raw)[kCount], float c) {
+  float largest = largest_of(raw[0]);
+#pragma unroll
+  for (int u = 1; u < kCount; ++u) largest = fmaxf(largest, largest_of(raw[u]));
+  r.raise(largest, c);
+  float s[2] = {0.0f, 0.0f};
+  if (r.m == -INFINITY || fabsf(r.m) < kHuge) {
+#pragma unroll
+    for (int u = 0; u < kCount; ++u) {
+      float z[8];
+      unpack8(raw[u], z);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s[k & 1] += exp2_fast(fmaf(z[k], c, -r.q));
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < kCount; ++u) {
+      float z[8];
+      unpack8(raw[u], z);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s[k & 1] += exp2_fast((z[k] - r.m) * c);
+    }
+  }
+  r.s += s[0] + s[1];
+}
+
+// Any alignment.  kGrad: the gradient as well, for an upstream gradient of 1, from a second read of the row.
+template <typename T, bool kGrad>
+__global__ void __maxnreg__(kGrad && sizeof(T) == 2 ? 40 : 64)
+    policy_rows_kernel(const PolicyArgs a, const PolicyState o, const long long run) {
+  __shared__ RowWords w;
+  const float c = a.inv_temp * kLog2e;
+  const int threads = static_cast<int>(blockDim.x), tid = static_cast<int>(threadIdx.x);
+  const int vocab = static_cast<int>(a.vocab);
+  const long long last = min(a.tokens, (blockIdx.x + 1) * run);
+  for (long long t = blockIdx.x * run; t < last; ++t) {
+    const T* row = static_cast<const T*>(a.logits) + t * a.ld;
+    T* out = kGrad ? static_cast<T*>(o.dlogits) + t * a.vocab : nullptr;
+    if (a.mask != nullptr && !a.mask[t]) {  // uniform
+      masked_token(o, t);
+      if (kGrad) gradient_row(row, out, vocab, 0.0f, make_float2(0.0f, 0.0f), -1, c);
+      continue;
+    }
+    const int id = in_vocabulary(a.ids[t], a.vocab);
+    const Inputs in = inputs_of(a, o, row, t, id);
+    const int head = head_of(row, vocab);
+    const T* body = row + head;
+    const int chunks = (vocab - head) / 8;
+    ChunkSum sum;
+    auto load = [&](const T* p) { return kGrad ? load8_l2(p) : load8_stream(p); };
+    const int stride = threads * 8;
+    const T* p = body + tid * 8;
+    int i = tid;
+    for (; i + (kUnroll - 1) * threads < chunks; i += kUnroll * threads, p += kUnroll * stride) {
+      Raw8<T> raw[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) raw[u] = load(p + u * stride);
+      add_chunks(sum, raw, c);
+    }
+    for (; i < chunks; i += threads, p += stride) {
+      const Raw8<T> raw[1] = {load(p)};
+      add_chunks(sum, raw, c);
+    }
+    Running r = sum.total(c);
+    // the ends of the row
+    const int tail = vocab - head - chunks * 8;
+    if (tid < head) r.add(to_float<T>(row[tid]), c);
+    if (tid < tail) r.add(to_float<T>(body[chunks * 8 + tid]), c);
+    finish_token(a, o, w, r, c, in, t);
+    if (kGrad) {
+      __syncthreads();
+      gradient_row(row, out, vocab, w.k, w.norm, id, c);
+    }
   }
 }
 
-// The reduction over sequences and the weights of their tokens: one block.
-__global__ void __launch_bounds__(256) policy_reduce_kernel(const PolicyArgs a, const PolicyState o) {
-  __shared__ float4 red[8];
-  __shared__ float total;
+// Shares of a masked batch's tokens, one a sequence ("sequence") or one for all
+// ("mean"): one block counts the mask.  Counts are whole numbers, so their order
+// does not matter.
+__global__ void __launch_bounds__(1024) policy_shares_kernel(const PolicyArgs a, const PolicyState o) {
+  __shared__ int red[32];
+  __shared__ int counts[1024];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const long long sequences = a.tokens / a.length;
   const bool each = a.reduction == kReduceSequence;
+  int mine = 0;  // counted tokens, or sequences that have any
+  if (!each || sequences <= 1024) {
+    counts[threadIdx.x] = 0;
+    __syncthreads();
+    for (long long base = warp * 32ll; base < a.tokens; base += 1024 * 4) {
+      bool on[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const long long t = base + u * 1024 + lane;
+        on[u] = t < a.tokens && a.mask[t];
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const long long t0 = base + u * 1024;
+        if (!each) {
+          mine += on[u] ? 1 : 0;
+        } else if (t0 < a.tokens) {
+          const uint32_t votes = __ballot_sync(0xffffffffu, on[u]);
+          const int q = static_cast<int>(sequence_of(a, t0)), left = static_cast<int>(min((q + 1) * a.length - t0, 32ll));
+          if (left == 32) {
+            if (lane == 0) atomicAdd(&counts[q], __popc(votes));
+          } else if (on[u]) {
+            atomicAdd(&counts[static_cast<int>(sequence_of(a, t0 + lane))], 1);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    if (each && static_cast<int>(threadIdx.x) < sequences) {
+      const int n = counts[threadIdx.x];
+      mine = n > 0 ? 1 : 0;
+      o.share[threadIdx.x] = 1.0f / static_cast<float>(n > 0 ? n : 1);
+    }
+  } else {
+    for (long long q = warp; q < sequences; q += 32) {
+      int n = 0;
+      for (long long i = lane; i < a.length; i += 32) n += a.mask[q * a.length + i] ? 1 : 0;
+      n = __reduce_add_sync(0xffffffffu, n);
+      if (lane == 0) {
+        mine += n > 0 ? 1 : 0;
+        o.share[q] = 1.0f / static_cast<float>(n > 0 ? n : 1);
+      }
+    }
+  }
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  if (lane == 0) red[warp] = mine;
+  __syncthreads();
+  const int total = __reduce_add_sync(0xffffffffu, red[lane]);
+  const float share = 1.0f / static_cast<float>(total > 0 ? total : 1);
+  if (!each) {
+    if (threadIdx.x == 0) o.share[0] = share;
+  } else {
+    for (long long q = threadIdx.x; q < sequences; q += 1024) o.share[q] *= share;
+  }
+}
+
+// Sum over the block of 1024 threads, in its first thread.
+__device__ __forceinline__ float4 block_total(float4 s, float4* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  s = make_float4(warp_sum(s.x), warp_sum(s.y), warp_sum(s.z), 0.0f);
+  if (lane == 0) red[warp] = s;
+  __syncthreads();
+  s = red[lane];
+  return make_float4(warp_sum(s.x), warp_sum(s.y), warp_sum(s.z), 0.0f);
+}
+
+// Loss, KL and clipped share: every block a run of tokens, the only (kLast) one the scalars.
+template <bool kLast>
+__global__ void __launch_bounds__(1024) policy_sum_kernel(const PolicyArgs a, const PolicyState o, long long run) {
+  __shared__ float4 red[32];
   float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (long long q = threadIdx.x; q < sequences; q += 256) {
-    const float4 v = o.sums[q];
-    if (v.w == 0.0f) continue;
-    const float f = each ? 1.0f / v.w : 1.0f;
-    s.x += v.x * f, s.y += v.y * f, s.z += v.z * f, s.w += each ? 1.0f : v.w;
+  const long long last = min(a.tokens, (blockIdx.x + 1) * run);
+  // eight tokens a thread in flight
+  for (long long t0 = blockIdx.x * run + threadIdx.x; t0 < last; t0 += 8 * 1024) {
+    float4 v[8];
+    float f[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const long long t = t0 + u * 1024;
+      v[u] = t < last ? o.terms[t] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // zeros where masked, too
+      f[u] = t < last ? share_of(a, o, t) : 0.0f;
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) s.x += f[u] * v[u].x, s.y += f[u] * v[u].y, s.z += f[u] * v[u].z;
   }
-  s = make_float4(warp_sum(s.x), warp_sum(s.y), warp_sum(s.z), warp_sum(s.w));
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; ++i) s.x += red[i].x, s.y += red[i].y, s.z += red[i].z, s.w += red[i].w;
-    const float f = a.reduction == kReduceSum ? 1.0f : 1.0f / fmaxf(s.w, 1.0f);
-    *o.loss = a.weight * s.x * f;
-    *o.kl = s.y * f;
-    *o.clipped = s.z * f;
-    total = a.weight * f;
+  s = block_total(s, red);
+  if (threadIdx.x != 0) return;
+  if (kLast) {
+    *o.loss = a.weight * s.x;
+    *o.kl = s.y;
+    *o.clipped = s.z;
+  } else {
+    o.sums[blockIdx.x] = s;
   }
-  __syncthreads();
-  for (long long q = threadIdx.x; q < sequences; q += 256)
-    o.weight[q] = each ? total / fmaxf(o.sums[q].w, 1.0f) : total;
+}
+
+__global__ void __launch_bounds__(1024) policy_total_kernel(const PolicyArgs a, const PolicyState o, int blocks) {
+  __shared__ float4 red[32];
+  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int i = threadIdx.x; i < blocks; i += 1024) {
+    const float4 v = o.sums[i];
+    s.x += v.x, s.y += v.y, s.z += v.z;
+  }
+  s = block_total(s, red);
+  if (threadIdx.x != 0) return;
+  *o.loss = a.weight * s.x;
+  *o.kl = s.y;
+  *o.clipped = s.z;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    policy_backward_kernel(const PolicyArgs a, const PolicyState o, const float* grad, T* __restrict__ dlogits) {
+__global__ void __launch_bounds__(1024)
+    policy_backward_kernel(const PolicyArgs a, const PolicyState o, const float* grad) {
   const float c = a.inv_temp * kLog2e;
   const float g = *grad;
+  if (o.factors != nullptr) {
+    // rows of this block whose gradient is not for g (a NaN is for nothing)
+    int stale = 0;
+    for (long long t = blockIdx.x + static_cast<long long>(threadIdx.x) * gridDim.x; t < a.tokens;
+         t += static_cast<long long>(blockDim.x) * gridDim.x)
+      stale |= o.factors[t] == g ? 0 : 1;
+    if (!__syncthreads_or(stale)) return;
+  }
   for (long long t = blockIdx.x; t < a.tokens; t += gridDim.x) {
+    if (o.factors != nullptr && o.factors[t] == g) continue;  // uniform
     const T* row = static_cast<const T*>(a.logits) + t * a.ld;
-    T* out = dlogits + t * a.vocab;
     const bool live = a.mask == nullptr || a.mask[t];
     const float slope = live ? o.terms[t].w : 0.0f;
-    const float k = slope == 0.0f ? 0.0f : g * o.weight[t / a.length] * slope * a.inv_temp;
-    const bool zero = k == 0.0f;  // NaN is not zero
-    const float2 norm = o.norm[t];
-    const long long id = zero ? -1 : a.ids[t];
-    const int head = head_of(out, a.vocab);
-    const bool vec = !zero && ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-    const long long chunks = (a.vocab - head) / 8;
-    auto one = [&](long long j) {
-      float v = 0.0f;
-      if (!zero) {
-        const float p = exp2_fast((to_float<T>(row[j]) - norm.x) * c - norm.y);
-        v = k * ((j == id ? 1.0f : 0.0f) - p);
-      }
-      out[j] = from_float<T>(v);
-    };
-    if (zero) {
-      const float nil[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-      for (long long i = threadIdx.x; i < chunks; i += kThreads) store8(out + head + i * 8, nil);
-    } else if (vec) {
-      for (long long i = threadIdx.x; i < chunks; i += kThreads * kUnroll) {
-        Raw8<T> raw[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u)
-          if (i + u * kThreads < chunks) raw[u] = load8_stream(row + head + (i + u * kThreads) * 8);
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          if (i + u * kThreads >= chunks) break;
-          const long long j0 = head + (i + u * kThreads) * 8;
-          float z[8];
-          unpack8(raw[u], z);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) z[e] = -k * exp2_fast((z[e] - norm.x) * c - norm.y);
-          if (id >= j0 && id < j0 + 8) {
-            const int at = static_cast<int>(id - j0);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (e == at) z[e] += k;
-          }
-          store8(out + j0, z);
-        }
-      }
-    } else {
-      for (long long j = head + threadIdx.x; j < head + chunks * 8; j += kThreads) one(j);
+    const float k = slope == 0.0f ? 0.0f : g * coefficient(a, share_of(a, o, t), slope);
+    gradient_row(row, static_cast<T*>(o.dlogits) + t * a.vocab, static_cast<int>(a.vocab), k, o.norm[t],
+                 k == 0.0f ? -1 : in_vocabulary(a.ids[t], a.vocab), c);
+    if (o.factors != nullptr) {
+      __syncthreads();  // every thread has read the factor
+      if (threadIdx.x == 0) o.factors[t] = g;
     }
-    const int tail = static_cast<int>(a.vocab - head - chunks * 8);
-    if (static_cast<int>(threadIdx.x) < head) one(threadIdx.x);
-    if (static_cast<int>(threadIdx.x) < tail) one(head + chunks * 8 + threadIdx.x);
   }
 }
 
-int grid_for(const PolicyArgs& a) {
-  const long long cap = a.sms * (2048ll / kThreads);
-  return static_cast<int>(a.tokens < cap ? a.tokens : cap);
+// Threads of a row's block: about sixteen chunks each.  With 40 registers a
+// thread an SM holds some 1500 of them, so that between its two reads a row of a
+// large vocabulary shares L2 (126 MB) with one or two of every other SM (fp32
+// rows and those read once take 64).
+int threads_for(const PolicyArgs& a) {
+  int threads = 64;
+  while (threads < 1024 && threads * 128ll < a.vocab) threads *= 2;
+  return threads;
 }
+
+// A block adds the terms of this many tokens (16 bytes each at some 100 GB/s an SM against a launch more).
+constexpr long long kRun = 16384;
 
 template <typename T>
 int forward_type(const PolicyArgs& a, const PolicyState& s, cudaStream_t stream, int* launches) {
-  policy_rows_kernel<T><<<grid_for(a), kThreads, 0, stream>>>(a, s);
-  policy_sequence_kernel<<<static_cast<unsigned>(a.tokens / a.length), 256, 0, stream>>>(a, s);
-  policy_reduce_kernel<<<1, 256, 0, stream>>>(a, s);
-  *launches = 3;
+  const bool grad = s.dlogits != nullptr;
+  *launches = 2;
+  if (a.mask != nullptr && a.reduction != kReduceSum) {
+    policy_shares_kernel<<<1, 1024, 0, stream>>>(a, s);
+    ++*launches;
+  }
+  const int threads = threads_for(a);
+  const long long resident = a.sms * (1536ll / threads);
+  const long long run = a.tokens / (resident * 16) < 1 ? 1 : a.tokens / (resident * 16);
+  const unsigned grid = static_cast<unsigned>((a.tokens + run - 1) / run);
+  if (grad)
+    policy_rows_kernel<T, true><<<grid, threads, 0, stream>>>(a, s, run);
+  else
+    policy_rows_kernel<T, false><<<grid, threads, 0, stream>>>(a, s, run);
+  if (a.tokens <= kRun) {
+    policy_sum_kernel<true><<<1, 1024, 0, stream>>>(a, s, kRun);
+  } else {
+    const long long blocks = policy_sum_blocks(a.tokens);
+    policy_sum_kernel<false><<<static_cast<unsigned>(blocks), 1024, 0, stream>>>(a, s, (a.tokens + blocks - 1) / blocks);
+    policy_total_kernel<<<1, 1024, 0, stream>>>(a, s, static_cast<int>(blocks));
+    ++*launches;
+  }
   return static_cast<int>(cudaGetLastError());
 }
 
 template <typename T>
-int backward_type(const PolicyArgs& a, const PolicyState& s, const float* grad, void* dlogits, cudaStream_t stream) {
-  policy_backward_kernel<T><<<grid_for(a), kThreads, 0, stream>>>(a, s, grad, static_cast<T*>(dlogits));
+int backward_type(const PolicyArgs& a, const PolicyState& s, const float* grad, cudaStream_t stream) {
+  const int threads = threads_for(a);
+  const long long cap = a.sms * (1024ll / threads);
+  policy_backward_kernel<T><<<static_cast<unsigned>(a.tokens < cap ? a.tokens : cap), threads, 0, stream>>>(a, s, grad);
   return static_cast<int>(cudaGetLastError());
 }
 
 }  // namespace
 
+long long policy_sum_blocks(long long tokens) {
+  const long long blocks = (tokens + 4095) / 4096;
+  return blocks < 148 ? blocks : 148;
+}
+
 int policy_forward(const PolicyArgs& a, const PolicyState& s, cudaStream_t stream, int* launches) {
   *launches = 0;
   if (a.tokens <= 0) return 0;
-  if (a.vocab <= 0 || a.length <= 0 || a.tokens % a.length != 0) return static_cast<int>(cudaErrorInvalidValue);
+  if (a.vocab <= 0 || a.vocab > 0x7fffff00ll || a.length <= 0 || a.tokens % a.length != 0) return static_cast<int>(cudaErrorInvalidValue);
   switch (a.dtype) {
     case kDtypeBF16:
       return forward_type<__nv_bfloat16>(a, s, stream, launches);
@@ -296,16 +601,15 @@ int policy_forward(const PolicyArgs& a, const PolicyState& s, cudaStream_t strea
   }
 }
 
-int policy_backward(const PolicyArgs& a, const PolicyState& s, const float* grad, void* dlogits,
-                    cudaStream_t stream) {
+int policy_backward(const PolicyArgs& a, const PolicyState& s, const float* grad, cudaStream_t stream) {
   if (a.tokens <= 0) return 0;
   switch (a.dtype) {
     case kDtypeBF16:
-      return backward_type<__nv_bfloat16>(a, s, grad, dlogits, stream);
+      return backward_type<__nv_bfloat16>(a, s, grad, stream);
     case kDtypeF16:
-      return backward_type<__half>(a, s, grad, dlogits, stream);
+      return backward_type<__half>(a, s, grad, stream);
     case kDtypeF32:
-      return backward_type<float>(a, s, grad, dlogits, stream);
+      return backward_type<float>(a, s, grad, stream);
     default:
       return static_cast<int>(cudaErrorInvalidValue);
   }

@@ -29,15 +29,20 @@ struct PolicyState {
   float* logp = nullptr;    // [tokens] output: log-probability of the token, 0 where masked
   float4* terms = nullptr;  // [tokens] loss, KL, clipped, derivative of the loss by logp (without weights)
   float2* norm = nullptr;   // [tokens] largest logit and log2 of the sum of exponentials
-  float* weight = nullptr;  // [sequences] weight of a token's loss
-  float4* sums = nullptr;   // [sequences] scratch
+  float* share = nullptr;   // [sequences] a token's share in the reduction, where the mask decides it
+  float4* sums = nullptr;   // [policy_sum_blocks] scratch
   float* loss = nullptr;    // scalars
   float* kl = nullptr;
   float* clipped = nullptr;
+  // the gradient for an upstream gradient of `factors`: written by the forward pass (factors 1) where not null
+  void* dlogits = nullptr;  // [tokens, vocab] contiguous
+  float* factors = nullptr; // [tokens]
 };
 
+// Blocks that add the tokens' terms of a large batch.
+long long policy_sum_blocks(long long tokens);
 int policy_forward(const PolicyArgs& a, const PolicyState& s, cudaStream_t stream, int* launches);
-// dlogits [tokens, vocab] contiguous, for the gradient *grad of the loss
-int policy_backward(const PolicyArgs& a, const PolicyState& s, const float* grad, void* dlogits, cudaStream_t stream);
+// s.dlogits for the gradient *grad of the loss.  With s.factors, rows that hold it already are left.
+int policy_backward(const PolicyArgs& a, const PolicyState& s, const float* grad, cudaStream_t stream);
 
 }  // namespace es

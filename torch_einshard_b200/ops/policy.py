@@ -7,9 +7,10 @@ log-probability ``old`` under the policy that sampled it and advantage ``A``,
     r    = exp(lp - old)
     loss = -min(r A, clip(r, 1 - low, 1 + high) A) + kl * (exp(ref - lp) - (ref - lp) - 1)
 
-reduced over the tokens that ``mask`` keeps.  The gradient by the logits is
-formed from the logits again, so neither probabilities nor a 32-bit copy of the
-logits is ever written (``csrc/policy.cu``).  A token that the mask leaves out
+reduced over the tokens that ``mask`` keeps.  Neither probabilities nor a 32-bit
+copy of the logits is ever written: with gradients, the forward pass also writes
+that of the logits (``csrc/policy.cu``), which backward hands out, so a training
+step reads the logits once.  A token that the mask leaves out
 has no loss and a gradient of exactly zero, whatever its logits, id and other
 inputs hold.  A kept id outside the vocabulary makes the loss NaN.
 
@@ -58,10 +59,17 @@ def _on_kernels(x):
 
 
 class _NativePolicy(torch.autograd.Function):
+    """The forward pass writes the gradient for an upstream gradient of 1 while it has the logits at hand; the first
+    backward pass hands it out (formed again in place where the upstream gradient is another), later ones form their
+    own.  A backward pass captured apart from its forward pass, or the other way round, has its own too: a replay of
+    the one would write under the other's result."""
+
     @staticmethod
     def forward(ctx, logits, ids, mask, old, ref, adv, conf):
-        loss, kl, clipped, logp, *state = _native.require().policy_forward(logits, ids, mask, old, ref, adv, *conf)
-        ctx.conf = conf
+        loss, kl, clipped, logp, *state, dlogits, factors = _native.require().policy_forward(
+            logits, ids, mask, old, ref, adv, *conf, True)
+        ctx.conf, ctx.kept = conf, (dlogits, factors)
+        ctx.captured = torch.cuda.is_current_stream_capturing()
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(logits, ids, mask, old, ref, adv, *state)
         ctx.mark_non_differentiable(logp, kl, clipped)
@@ -72,8 +80,11 @@ class _NativePolicy(torch.autograd.Function):
     def backward(ctx, grad, *_):
         if grad is None:
             return (None,) * 7
-        *inputs, terms, norm, weight = ctx.saved_tensors
-        dlogits = _native.require().policy_backward(grad.contiguous(), *inputs, *ctx.conf, terms, norm, weight)
+        *inputs, terms, norm, shares = ctx.saved_tensors
+        kept, ctx.kept = ctx.kept, None
+        if kept is None or torch.cuda.is_current_stream_capturing() != ctx.captured:
+            kept = (None, None)
+        dlogits = _native.require().policy_backward(grad.contiguous(), *inputs, *ctx.conf, terms, norm, shares, *kept)
         return (dlogits,) + (None,) * 6
 
 
@@ -166,8 +177,8 @@ def einpolicy(shard, logits, ids, *, axis, advantages, old_logp=None, ref_logp=N
     ``(low, high)``.  ``reduction``: "mean" over kept tokens, "sequence" (mean
     over the tokens of a sequence, then over sequences that keep any) or "sum";
     no kept token at all gives 0.  ``weight`` multiplies the loss (a share of
-    accumulated steps): here it is free, where a factor outside costs backward
-    another pass over the logits."""
+    accumulated steps): here it is free, where a factor outside makes backward
+    form the gradient again."""
     if families is not None:
         shard, _ = cached_expand_axis_families(shard, families=families)
     if logits.dtype not in _FLOATS:
@@ -217,5 +228,5 @@ def einpolicy(shard, logits, ids, *, axis, advantages, old_logp=None, ref_logp=N
     elif torch.is_grad_enabled() and rows.requires_grad:
         loss, logp, kl_value, clipped = _NativePolicy.apply(*args)
     else:
-        loss, kl_value, clipped, logp, *_ = _native.require().policy_forward(*args[:-1], *conf)
+        loss, kl_value, clipped, logp, *_ = _native.require().policy_forward(*args[:-1], *conf, False)
     return PolicyLoss(loss, logp.view(shape), kl_value, clipped)
