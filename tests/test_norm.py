@@ -372,6 +372,33 @@ def test_refusals(device):
 
 
 @pytest.mark.gpu
+def test_no_second_derivative():
+    t, conf, dh, dn = make("cuda", torch.float32, (2, 5, 40))
+    h, n = run(t, conf)
+    (dx,) = torch.autograd.grad((h, n), t["x"], (dh, dn), create_graph=True)
+    assert torch.equal(dx.detach(), torch.autograd.grad(run(t, conf), t["x"], (dh, dn))[0])
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(dx.sum(), t["x"], allow_unused=True)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_results_may_be_changed_in_place(device):
+    t, conf, dh, dn = make(device, torch.float32, (2, 5, 40))
+    want = torch.autograd.grad(run(t, conf), t["x"], (dh, 2 * dn))
+    h, n = run(t, conf)
+    n *= 2
+    assert torch.allclose(torch.autograd.grad((h, n), t["x"], (dh, dn))[0], want[0], atol=1e-6)
+    # and an input changed between the passes is noticed
+    x = t["x"].detach().clone().requires_grad_(True)
+    moved = x * 1
+    h, n = run({**t, "x": moved}, conf)
+    moved.add_(1)
+    if device == "cuda":
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            torch.autograd.grad((h, n), x, (dh, dn))
+
+
+@pytest.mark.gpu
 def test_other_stream_and_capture():
     t, conf, dh, dn = make("cuda", torch.bfloat16, (2, 64, 256), gate="batch")
     want = run(t, conf)

@@ -353,6 +353,16 @@ def test_backward_twice_and_beside_another_loss(device):
         assert not es.einpolicy("b s v", z, axis="v", **t).loss.requires_grad
 
 
+@pytest.mark.gpu
+def test_no_second_derivative():
+    t = off_border(make("cuda", torch.float32, 2, 5, 40), 0.2, 0.2)
+    z = t.pop("logits").requires_grad_(True)
+    (g,) = torch.autograd.grad(es.einpolicy("b s v", z, axis="v", **t).loss, z, create_graph=True)
+    assert torch.equal(g.detach(), torch.autograd.grad(es.einpolicy("b s v", z, axis="v", **t).loss, z)[0])
+    with pytest.raises(RuntimeError, match="twice"):
+        torch.autograd.grad(g.sum(), z, allow_unused=True)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_refusals(device):
     t = make(device, torch.float32, 2, 3, 8)

@@ -4,7 +4,10 @@
 #include "bindings_train.h"
 
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
+#include <ATen/core/LegacyTypeDispatch.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 
 #include "gemm.h"
 #include "norm.h"
@@ -238,6 +241,90 @@ std::vector<Opt> norm_backward_op(const Opt& dh, const Opt& dn, const at::Tensor
   return out;
 }
 
+// A gradient that has no derivative of its own: under create_graph, using it further raises.
+struct Final : public torch::autograd::Function<Final> {
+  static at::Tensor forward(torch::autograd::AutogradContext*, const at::Tensor& t, const at::Tensor&) {
+    return t.view_as(t);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext*, torch::autograd::variable_list) {
+    TORCH_CHECK(false, "einshard: trying to differentiate twice a function that was marked with once_differentiable");
+  }
+};
+
+// `grads` as results of what they were formed from, where a graph of the backward pass is wanted.
+void finalise(std::vector<at::Tensor>& grads, const torch::autograd::variable_list& from) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor& input : from) {
+    if (!input.defined() || !input.requires_grad()) continue;
+    for (at::Tensor& g : grads)
+      if (g.defined()) g = Final::apply(g, input);
+    return;
+  }
+}
+
+Opt some(const at::Tensor& t) { return t.defined() ? Opt(t) : Opt(); }
+at::Tensor none(const Opt& t) { return t.has_value() ? *t : at::Tensor(); }
+
+// [rows, d] of a tensor whose last axis is the row, with a unit stride.
+at::Tensor rows_of(const at::Tensor& t) {
+  if (!t.defined()) return t;
+  const int64_t d = t.size(-1);
+  at::Tensor r = t.dim() == 2 ? t : t.reshape({t.numel() / d, d});
+  return r.stride(1) == 1 || d == 1 ? r : r.contiguous();
+}
+
+struct NormFunction : public torch::autograd::Function<NormFunction> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x,
+                                                const Opt& y, const Opt& w, const Opt& b, const Opt& pw, const Opt& pb,
+                                                const Opt& gate, int64_t inner, int64_t count, bool post, bool center, double scale,
+                                                double eps) {
+    const at::Tensor xr = rows_of(x), yr = rows_of(none(y));
+    auto out = norm_forward_op(xr, some(yr), w, b, pw, pb, gate, inner, count, post, center, scale, eps, true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({x, none(y), none(w), none(b), none(pw), none(pb), none(gate), *out[2]});
+    ctx->saved_data["conf"] = c10::ivalue::Tuple::create({inner, count, post, center, scale, eps});
+    at::AutoDispatchBelowADInplaceOrView plain;  // results of their own, not views
+    if (!y.has_value()) return {out[1]->view(x.sizes())};
+    return {out[0]->view(x.sizes()), out[1]->view(x.sizes())};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const auto conf = ctx->saved_data["conf"].toTuple()->elements();
+    at::Tensor dh = grads.size() == 2 ? grads[0] : at::Tensor(), dn = grads.back();
+    torch::autograd::variable_list out(13);
+    if (!dh.defined() && !dn.defined()) return out;
+    std::vector<bool> want(7);
+    size_t edge = 0;  // absent inputs have none
+    for (size_t i = 0; i < 7; ++i) want[i] = s[i].defined() && ctx->needs_input_grad(edge++);
+    std::vector<at::Tensor> found(7);
+    {
+      at::AutoDispatchBelowAutograd below;
+      const at::Tensor xr = rows_of(s[0]), yr = rows_of(s[1]);
+      auto plain = [&](const at::Tensor& g) { return g.defined() ? Opt(g.reshape(xr.sizes()).contiguous()) : Opt(); };
+      auto got = norm_backward_op(plain(dh), plain(dn), xr, some(yr), some(s[2]), some(s[3]), some(s[4]),
+                                  some(s[5]), some(s[6]), conf[0].toInt(), conf[1].toInt(), conf[2].toBool(),
+                                  conf[3].toBool(), conf[4].toDouble(), conf[5].toDouble(), s[7], want);
+      for (size_t i = 0; i < 7; ++i) {
+        found[i] = none(got[i]);
+        if (i < 2 && found[i].defined()) found[i] = found[i].view(s[0].sizes());
+      }
+    }
+    finalise(found, grads);
+    finalise(found, s);
+    for (size_t i = 0; i < 7; ++i) out[i] = found[i];
+    return out;
+  }
+};
+
+// norm_forward on tensors whose last axis is normalised, with gradients: (h, n) or (n)
+std::vector<at::Tensor> norm_op(const at::Tensor& x, const Opt& y, const Opt& w, const Opt& b, const Opt& pw,
+                                const Opt& pb, const Opt& gate, int64_t inner, int64_t count, bool post, bool center,
+                                double scale, double eps) {
+  return NormFunction::apply(x, y, w, b, pw, pb, gate, inner, count, post, center, scale, eps);
+}
+
 // ------------------------------------------------------------------ policy loss
 
 void per_token(const Opt& t, const at::Tensor& logits, int64_t count, at::ScalarType type, const char* name) {
@@ -348,6 +435,69 @@ at::Tensor policy_backward_op(const at::Tensor& grad, const at::Tensor& logits, 
   return out;
 }
 
+// The forward pass writes the gradient for an upstream gradient of 1 while it has the logits at hand; the first
+// backward pass hands it out (formed again in place where the upstream gradient is another), later ones form their
+// own.  A backward pass captured apart from its forward pass, or the other way round, has its own too: a replay of the
+// one would write under the other's result.
+struct PolicyFunction : public torch::autograd::Function<PolicyFunction> {
+  static bool capturing() {
+    return at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None;
+  }
+
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits,
+                                                const at::Tensor& ids, const Opt& mask, const Opt& old, const Opt& ref,
+                                                const at::Tensor& adv, int64_t length, double lo, double hi, double kl, double temperature, int64_t reduction,
+                                                double weight) {
+    const at::Tensor rows = rows_of(logits);
+    auto r = policy_forward_op(rows, ids, mask, old, ref, adv, length, lo, hi, kl, temperature, reduction, weight, true);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({logits, ids, none(mask), none(old), none(ref), adv, r[4], r[5], r[6]});
+    ctx->saved_data["conf"] = c10::ivalue::Tuple::create({length, lo, hi, kl, temperature, reduction, weight});
+    ctx->saved_data["kept"] = r[7];
+    ctx->saved_data["factors"] = r[8];
+    ctx->saved_data["captured"] = capturing();
+    ctx->mark_non_differentiable({r[1], r[2], r[3]});
+    return {r[0], r[1], r[2], r[3]};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    torch::autograd::variable_list out(13);
+    if (!grads[0].defined()) return out;
+    const auto s = ctx->get_saved_variables();
+    const auto conf = ctx->saved_data["conf"].toTuple()->elements();
+    Opt kept, factors;
+    if (ctx->saved_data.count("kept")) {
+      if (ctx->saved_data["captured"].toBool() == capturing()) {
+        kept = ctx->saved_data["kept"].toTensor();
+        factors = ctx->saved_data["factors"].toTensor();
+      }
+      ctx->saved_data.erase("kept");
+      ctx->saved_data.erase("factors");
+    }
+    std::vector<at::Tensor> found(1);
+    {
+      at::AutoDispatchBelowAutograd below;
+      found[0] = policy_backward_op(grads[0].contiguous(), rows_of(s[0]), s[1], some(s[2]), some(s[3]), some(s[4]), s[5],
+                                    conf[0].toInt(), conf[1].toDouble(), conf[2].toDouble(), conf[3].toDouble(),
+                                    conf[4].toDouble(), conf[5].toInt(), conf[6].toDouble(), s[6], s[7], s[8], kept,
+                                    factors)
+                     .view(s[0].sizes());
+    }
+    finalise(found, grads);
+    finalise(found, s);
+    out[0] = found[0];
+    return out;
+  }
+};
+
+// policy_forward on logits whose last axis is the vocabulary, with gradients: (loss, KL, clipped share, logp)
+std::vector<at::Tensor> policy_op(const at::Tensor& logits, const at::Tensor& ids, const Opt& mask, const Opt& old,
+                                  const Opt& ref, const at::Tensor& adv, int64_t length, double lo, double hi,
+                                  double kl, double temperature, int64_t reduction, double weight) {
+  return PolicyFunction::apply(logits, ids, mask, old, ref, adv, length, lo, hi, kl, temperature, reduction, weight);
+}
+
 }  // namespace
 
 void bind_training_ops(pybind11::module_& m, std::atomic<long long>& launches) {
@@ -355,9 +505,9 @@ void bind_training_ops(pybind11::module_& m, std::atomic<long long>& launches) {
   m.def("quant8", &quant8_op, "(codes, exponents) of a [rows, d] tensor kept in 8 bits");
   m.def("quant8_silu", &quant8_silu_op, "(silu(h), codes, exponents) of an fp32 pre-activation");
   m.def("norm_forward", &norm_forward_op, "(h, n, statistics) of the norms around a block's residual");
-  m.def("norm_backward", &norm_backward_op, "gradients of norm_forward");
+  m.def("norm", &norm_op, "norm_forward with gradients", pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("policy", &policy_op, "policy_forward with gradients", pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("policy_forward", &policy_forward_op, "clipped policy loss of token logits, with what its gradient needs");
-  m.def("policy_backward", &policy_backward_op, "gradient of policy_forward by the logits");
   m.def("restore8", &restore8_op, "what 8-bit codes stand for, its silu, or grad * silu'");
 }
 

@@ -676,17 +676,17 @@ __global__ void __launch_bounds__(kThreads)
   };
   long long g0 = 0;  // the gate's row
   auto kept = [&](int k, Pair (&f)[kP]) {
-    if (kShared) {
+    if constexpr (kShared) {
       param<T, kA>(k == 0 ? a.w : a.gate, k == 0 ? 0 : g0, 1.0f, f, s);
       if (k == 1 && kPost) times<T, kA>(a.pw, 0, f, s);
       if (k == 2) times<T, kA>(a.pb, 0, f, s);
-      return;
-    }
+    } else {
 #pragma unroll
-    for (int q = 0; q < kP / 2; ++q) {
-      const ulonglong2 v = vectors[(k * (kP / 2) + q) * blockDim.x + threadIdx.x];
-      f[2 * q] = v.x;
-      f[2 * q + 1] = v.y;
+      for (int q = 0; q < kP / 2; ++q) {
+        const ulonglong2 v = vectors[(k * (kP / 2) + q) * blockDim.x + threadIdx.x];
+        f[2 * q] = v.x;
+        f[2 * q + 1] = v.y;
+      }
     }
   };
   if (!kShared) {
@@ -697,8 +697,10 @@ __global__ void __launch_bounds__(kThreads)
   long long gate_at = -1;
   if (blocks > 1) cluster_sync();  // every block runs before one writes another's words
   int stage = 0;
+  float4 next_st = first < last ? reinterpret_cast<const float4*>(o.stats)[first] : make_float4(0.0f, 1.0f, 0.0f, 1.0f);
   for (long long row = first; row < last; ++row) {
-    const float4 st = reinterpret_cast<const float4*>(o.stats)[row];
+    const float4 st = next_st;
+    if (row + 1 < last) next_st = reinterpret_cast<const float4*>(o.stats)[row + 1];
     const long long g = gate_row(a, row);
     g0 = g * a.d;
     Pair hh[kP], yh[kP], t[kP], u[kP];
@@ -1151,16 +1153,20 @@ Launch forward_launch(const NormArgs& a, bool vec) {
 
 template <class Kernel, class... Args>
 int launch_rows(Kernel kernel, long long units, const NormArgs& a, const Launch& l, cudaStream_t stream,
-                Args... args) {
-  cudaError_t e = cudaSuccess;
-  const int bytes = l.bytes;
-  if (bytes > 48 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return static_cast<int>(e);
+                unsigned long long* prepared, Args... args) {
+  // the kernel's shared memory limit, once a device (`prepared`: a bit each)
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!(*prepared >> dev & 1ull)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedBytes);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    *prepared |= 1ull << dev;
+  }
   const int blocks = blocks_for(a);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(units * blocks));
   cfg.blockDim = dim3(static_cast<unsigned>(l.threads));
-  cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
+  cfg.dynamicSmemBytes = static_cast<size_t>(l.bytes);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1176,7 +1182,8 @@ template <typename T, int kA, bool kPost>
 int forward_rows(const NormArgs& a, const NormForward& f, cudaStream_t stream) {
   const Launch l = forward_launch(a, kA != kAny);
   const long long cap = a.sms * l.resident / blocks_for(a);
-  return launch_rows(norm_forward_kernel<T, kA, kPost>, a.rows < cap ? a.rows : cap, a, l, stream, f);
+  static unsigned long long prepared = 0;
+  return launch_rows(norm_forward_kernel<T, kA, kPost>, a.rows < cap ? a.rows : cap, a, l, stream, &prepared, f);
 }
 
 template <typename T>
@@ -1196,16 +1203,20 @@ int forward_type(const NormArgs& a, const NormForward& f, cudaStream_t stream) {
   }
 }
 
+template <typename T, int kA, bool kPost, bool kFull, bool kWide>
+int backward_rows(const NormArgs& a, const NormPlan& plan, const NormBackward& b, cudaStream_t stream) {
+  const Launch l = backward_launch(a, plan, kA != kAny);
+  static unsigned long long prepared = 0;
+  return launch_rows(norm_backward_kernel<T, kA, kPost, kFull, kWide>, plan.units(), a, l, stream, &prepared, plan, b);
+}
+
 template <typename T, int kA, bool kPost>
 int backward_sums(const NormArgs& a, const NormPlan& plan, const NormBackward& b, cudaStream_t stream) {
-  const Launch l = backward_launch(a, plan, kA != kAny);
-  const long long units = plan.units();
   if (wide_rows(a))
-    return plan.full
-               ? launch_rows(norm_backward_kernel<T, kA, kPost, true, true>, units, a, l, stream, plan, b)
-               : launch_rows(norm_backward_kernel<T, kA, kPost, false, true>, units, a, l, stream, plan, b);
-  return plan.full ? launch_rows(norm_backward_kernel<T, kA, kPost, true, false>, units, a, l, stream, plan, b)
-                   : launch_rows(norm_backward_kernel<T, kA, kPost, false, false>, units, a, l, stream, plan, b);
+    return plan.full ? backward_rows<T, kA, kPost, true, true>(a, plan, b, stream)
+                     : backward_rows<T, kA, kPost, false, true>(a, plan, b, stream);
+  return plan.full ? backward_rows<T, kA, kPost, true, false>(a, plan, b, stream)
+                   : backward_rows<T, kA, kPost, false, false>(a, plan, b, stream);
 }
 
 template <typename T>

@@ -24,7 +24,6 @@ from dataclasses import dataclass
 from functools import lru_cache
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ..notation.families import cached_expand_axis_families
 from ..notation.parser import parse_sharding
@@ -155,37 +154,16 @@ def _gate_rows(gate, plan):
     return gate.reshape(plan.count, plan.d)
 
 
-def _rows(t, plan):
-    if plan.place != t.dim() - 1:
-        t = t.movedim(plan.place, -1)
-    t = t.reshape(math.prod(plan.lead), plan.d)
-    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
-
-
-class _NativeNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, y, w, b, pw, pb, gate, conf):
-        h, n, stats = _native.require().norm_forward(x, y, w, b, pw, pb, gate, *conf, any(ctx.needs_input_grad))
-        ctx.conf = conf
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, y, w, b, pw, pb, gate, stats)
-        return (h, n) if y is not None else n
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, *grads):
-        *tensors, stats = ctx.saved_tensors
-        dh, dn = grads if len(grads) == 2 else (None, grads[0])
-        if dh is None and dn is None:
-            return (None,) * 8
-        dh, dn = (None if g is None else g.contiguous() for g in (dh, dn))
-        out = _native.require().norm_backward(dh, dn, *tensors, *ctx.conf, stats, list(ctx.needs_input_grad[:7]))
-        return (*out, None)
+def _last(t, plan):
+    """t with the normalised axis last."""
+    return t if t is None or plan.place == len(plan.lead) else t.movedim(plan.place, -1)
 
 
 def _torch_norm(x, y, w, b, pw, pb, gate, conf):
     inner, count, post, center, scale, eps = conf
-    dtype = x.dtype
+    dtype, shape = x.dtype, x.shape
+    x = x.reshape(-1 if x.numel() else 0, shape[-1])
+    y = None if y is None else y.reshape(x.shape)
     wide = torch.promote_types(dtype, torch.float32)
 
     def normed(t, weight, bias):
@@ -204,8 +182,8 @@ def _torch_norm(x, y, w, b, pw, pb, gate, conf):
             rows = torch.arange(x.shape[0], device=x.device) // inner % count
             p = p * gate.to(wide)[rows]
         h = scale * h + p
-    n = normed(h, w, b).to(dtype)
-    return n if y is None else (h.to(dtype), n)
+    n = normed(h, w, b).to(dtype).view(shape)
+    return (n,) if y is None else (h.to(dtype).view(shape), n)
 
 
 def _on_kernels(x):
@@ -259,19 +237,12 @@ def einnorm(shard, x, y=None, *, axis, weight=None, bias=None, kind="layer", eps
             gate, inner, count = gate.sum().expand(1, plan.d), 1, 1  # no row to weigh: a gradient of zero
 
     conf = (inner, count, bool(post), kind == "layer", float(scale), float(eps))
-    args = [_rows(x, plan), None if y is None else _rows(y, plan)]
+    args = [_last(x, plan), _last(y, plan)]
     args += [None if t is None else t.contiguous() for t in (weight, bias, post_weight, post_bias, gate)]
     if not _on_kernels(x):
         out = _torch_norm(*args, conf)
-    elif torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
-        out = _NativeNorm.apply(*args, conf)
     else:
-        h, n, _ = _native.require().norm_forward(*args, *conf, False)
-        out = n if y is None else (h, n)
-
-    def back(t):
-        if plan.place == len(plan.lead):
-            return t.view(x.shape)
-        return t.view(*plan.lead, plan.d).movedim(-1, plan.place)
-
-    return (x, back(out)) if y is None else (back(out[0]), back(out[1]))
+        out = _native.require().norm(*args, *conf)
+    if plan.place != len(plan.lead):
+        out = [t.movedim(-1, plan.place) for t in out]
+    return (x, out[0]) if y is None else (out[0], out[1])

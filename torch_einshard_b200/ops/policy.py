@@ -23,7 +23,6 @@ from functools import lru_cache
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ..notation.families import cached_expand_axis_families
 from ..notation.parser import parse_sharding
@@ -58,39 +57,11 @@ def _on_kernels(x):
     return False
 
 
-class _NativePolicy(torch.autograd.Function):
-    """The forward pass writes the gradient for an upstream gradient of 1 while it has the logits at hand; the first
-    backward pass hands it out (formed again in place where the upstream gradient is another), later ones form their
-    own.  A backward pass captured apart from its forward pass, or the other way round, has its own too: a replay of
-    the one would write under the other's result."""
-
-    @staticmethod
-    def forward(ctx, logits, ids, mask, old, ref, adv, conf):
-        loss, kl, clipped, logp, *state, dlogits, factors = _native.require().policy_forward(
-            logits, ids, mask, old, ref, adv, *conf, True)
-        ctx.conf, ctx.kept = conf, (dlogits, factors)
-        ctx.captured = torch.cuda.is_current_stream_capturing()
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(logits, ids, mask, old, ref, adv, *state)
-        ctx.mark_non_differentiable(logp, kl, clipped)
-        return loss, logp, kl, clipped
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad, *_):
-        if grad is None:
-            return (None,) * 7
-        *inputs, terms, norm, shares = ctx.saved_tensors
-        kept, ctx.kept = ctx.kept, None
-        if kept is None or torch.cuda.is_current_stream_capturing() != ctx.captured:
-            kept = (None, None)
-        dlogits = _native.require().policy_backward(grad.contiguous(), *inputs, *ctx.conf, terms, norm, shares, *kept)
-        return (dlogits,) + (None,) * 6
-
-
 def _torch_policy(logits, ids, mask, old, ref, adv, conf):
     length, low, high, kl_weight, temperature, reduction, weight = conf
-    tokens, vocab = logits.shape
+    vocab = logits.shape[-1]
+    logits = logits.reshape(-1, vocab)
+    tokens = logits.shape[0]
     wide = torch.promote_types(logits.dtype, torch.float32)
     keep = torch.ones(tokens, dtype=torch.bool, device=logits.device) if mask is None else mask
     z = torch.where(keep[:, None], logits.to(wide), 0)
@@ -123,7 +94,7 @@ def _torch_policy(logits, ids, mask, old, ref, adv, conf):
         return (t / count.clamp(min=1)).sum() / (count > 0).sum().clamp(min=1)
 
     loss = weight * reduced(-gain + kl_weight * kl)
-    return loss, kept(lp).detach(), reduced(kl).detach(), reduced(clipped).detach()
+    return loss, reduced(kl).detach(), reduced(clipped).detach(), kept(lp).detach()
 
 
 @lru_cache(maxsize=1024)
@@ -216,17 +187,17 @@ def einpolicy(shard, logits, ids, *, axis, advantages, old_logp=None, ref_logp=N
         zero = logits.detach().new_zeros((), dtype=torch.promote_types(logits.dtype, torch.float32))
         return PolicyLoss(logits.sum(dtype=zero.dtype), zero.expand(shape), zero, zero)
     rows = logits if place == len(shape) else logits.movedim(place, -1)
-    rows = rows.reshape(tokens, vocab)
-    if rows.stride(1) != 1 and vocab > 1:
-        rows = rows.contiguous()
     mask = None if mask is None else _flat(mask)
     conf = (max(shape[-1], 1) if shape else 1, float(low), float(high), float(kl), float(temperature),
             _REDUCTIONS[reduction], float(weight))
     args = (rows, _flat(ids.long()), mask, old, ref, adv, conf)
     if not _on_kernels(logits):
-        loss, logp, kl_value, clipped = _torch_policy(*args)
+        loss, kl_value, clipped, logp = _torch_policy(*args)
     elif torch.is_grad_enabled() and rows.requires_grad:
-        loss, logp, kl_value, clipped = _NativePolicy.apply(*args)
+        loss, kl_value, clipped, logp = _native.require().policy(*args[:-1], *conf)
     else:
-        loss, kl_value, clipped, logp, *_ = _native.require().policy_forward(*args[:-1], *conf, False)
+        rows = rows.reshape(tokens, vocab)
+        if rows.stride(1) != 1 and vocab > 1:
+            rows = rows.contiguous()
+        loss, kl_value, clipped, logp, *_ = _native.require().policy_forward(rows, *args[1:-1], *conf, False)
     return PolicyLoss(loss, logp.view(shape), kl_value, clipped)
