@@ -93,6 +93,32 @@ def test_error_is_half_a_step(device):
     assert s.nbytes == 64 * 257 + 64 * 9
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [3, 7, 9, 15, 31, 33, 39, 65, 511, 513, 2047, 2048, 2049, 4001, 8127, 8191, 8195])
+def test_rows_without_alignment(dtype, width):
+    """Every start of a row inside a 16-byte word, in the values, the codes and the result."""
+    gen = torch.Generator().manual_seed(width)
+    base = (torch.randn(21 * width + 16, generator=gen) * 3).to(dtype).cuda()
+    for off in (0, 1, 2, 3, 5, 7):
+        check_restore(base[off:off + 19 * width].view(19, width))
+    x = base[1:1 + 9 * width].view(9, width).clone()
+    x[3, width // 2] = float("nan")
+    x[5, 0] = float("inf")
+    x[8, width - 1] = -float("inf")
+    check_restore(x)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,width", [(5003, 9), (3001, 33), (1999, 65), (701, 301), (67, 8191), (3, 40001)])
+def test_blocks_across_tiles(dtype, rows, width):
+    """Rows of odd widths over many blocks of the grid, and the gradient of a SiLU kept with them."""
+    gen = torch.Generator().manual_seed(rows)
+    x = (torch.randn(rows, width, generator=gen) * torch.exp(torch.randn(rows, 1, generator=gen))).to(dtype)
+    check_restore(x.cuda())
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_views_and_alignments(device):
     base = torch.randn(6, 130, 70, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).to(device)

@@ -33,14 +33,26 @@ __device__ __forceinline__ float scale8_of(int byte) {
   return byte == kQuantNan ? __uint_as_float(0x7fc00000u) : __uint_as_float(static_cast<uint32_t>(byte) << 23);
 }
 
-// Four codes in a word.  1.5 2^23 + x 2^-e rounds to the nearest whole number
+// The low bytes of four words.
+__device__ __forceinline__ uint32_t bytes_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
+// A code, in the low byte.  1.5 2^23 + x 2^-e rounds to the nearest whole number
 // (ties to even) in one FMA, whose low byte is the code in two's complement.
+constexpr float kCodeMagic = 12582912.0f;
+
+// Four codes of one block in a word.
 __device__ __forceinline__ uint32_t codes8_of(float a, float b, float c, float d, const Step8& s) {
-  constexpr float kMagic = 12582912.0f;
-  const uint32_t ca = __float_as_uint(fmaf(a, s.inv, kMagic)), cb = __float_as_uint(fmaf(b, s.inv, kMagic));
-  const uint32_t cc = __float_as_uint(fmaf(c, s.inv, kMagic)), cd = __float_as_uint(fmaf(d, s.inv, kMagic));
-  const uint32_t w = __byte_perm(__byte_perm(ca, cb, 0x0040), __byte_perm(cc, cd, 0x0040), 0x5410);
+  const uint32_t w =
+      bytes_of(__float_as_uint(fmaf(a, s.inv, kCodeMagic)), __float_as_uint(fmaf(b, s.inv, kCodeMagic)),
+               __float_as_uint(fmaf(c, s.inv, kCodeMagic)), __float_as_uint(fmaf(d, s.inv, kCodeMagic)));
   return s.byte == kQuantNan ? 0u : w;
+}
+
+// One code, in the low byte; 0 for an infinity or a NaN, whose block has inv 0 (the maximum drops the NaN).
+__device__ __forceinline__ uint32_t code8_of(float x, float inv) {
+  return __float_as_uint(fmaxf(fmaf(x, inv, kCodeMagic), 0.0f));
 }
 
 // Code i of a word of four: the byte, its sign bit flipped, below 2^23 as a float is code + 128 + 2^23.
@@ -52,6 +64,12 @@ __device__ __forceinline__ float code8_at(uint32_t word, int i) {
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
 
