@@ -410,3 +410,115 @@ def test_models_keep_their_outputs_and_gradients(one_rank_mesh):
         assert (p - q).norm() <= 0.05 * p.norm() + 1e-6
     with pytest.raises(ValueError):
         TPMLP(64, 256, mesh, dtype=dtype, device=device, checkpoint="int4")
+
+
+# ------------------------------------------------------------------ one operand, several contractions
+
+def shared_case(dtype, device, shape, outs, gen):
+    """x [b, s, c], weights and gradients of ``outs`` projections of different widths, and dx in 64 bits."""
+    b, s, c = shape
+    widths = [max(8, c // (i + 1)) for i in range(outs)]
+    x = torch.randn(shape, generator=gen).to(dtype).to(device).requires_grad_(True)
+    w = [(torch.randn(n, c, generator=gen) / c ** 0.5).to(dtype).to(device).requires_grad_(True) for n in widths]
+    dy = [torch.randn(b, s, n, generator=gen).to(dtype).to(device) for n in widths]
+    with torch.no_grad():
+        want = sum(d.double() @ v.double() for d, v in zip(dy, w))
+        size = sum(d.double().abs() @ v.double().abs() for d, v in zip(dy, w))
+    return x, w, dy, want, size
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,outs", [((2, 5, 24), 2), ((1, 300, 136), 3), ((3, 64, 129), 4), ((2, 33, 256), 6),
+                                        ((1, 1, 64), 3), ((1, 1024, 512), 3)])
+def test_shared_operand_is_rounded_once(device, dtype, shape, outs):
+    """dx = sum_i dz_i w_i: half a step of the result, and for the 32-bit sums 2^-22 of the sum of absolute values.
+
+    An fp32 product is a library's: K products and additions one after the other, each off by at most 2^-24 of a
+    partial sum, which the sum of absolute values bounds, so (K + 1) 2^-24 of it."""
+    x, w, dy, want, size = shared_case(dtype, device, shape, outs, torch.Generator().manual_seed(outs))
+    kept = es.checkpoint8(x)
+    ys = [es.einshard("b s c, n c -> b s n", kept, v) for v in w]
+    dx = torch.autograd.grad(ys, x, dy, retain_graph=True)[0]
+    terms = sum(v.shape[0] for v in w)
+    sums = (terms + 1) * 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -22
+    allowed = half_step(dtype) * want.abs() + size * sums + torch.finfo(dtype).tiny
+    assert ((dx.double() - want).abs() <= allowed).all()
+    # again, a part of them, and the weights alone: nothing is left over from one pass to the next
+    assert torch.equal(dx, torch.autograd.grad(ys, x, dy, retain_graph=True)[0])
+    dw = torch.autograd.grad(ys, w, dy, retain_graph=True)
+    one = torch.autograd.grad(ys[1], x, dy[1], retain_graph=True)[0]
+    want1 = dy[1].double() @ w[1].double()
+    size1 = dy[1].double().abs() @ w[1].double().abs()
+    assert ((one.double() - want1).abs() <= half_step(dtype) * want1.abs() + size1 * sums + torch.finfo(dtype).tiny).all()
+    both = torch.autograd.grad(ys, [x, *w], dy)
+    assert torch.equal(both[0], dx) and all(torch.equal(a, b) for a, b in zip(both[1:], dw))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_shared_operand_in_different_equations(device):
+    """Gradients meet in the operand's axes, whatever the contractions' layouts."""
+    gen = torch.Generator().manual_seed(9)
+    x = torch.randn(2, 16, 4, 32, generator=gen).to(torch.bfloat16).to(device).requires_grad_(True)
+    w = torch.randn(4, 32, 24, generator=gen).to(torch.bfloat16).to(device)
+    v = torch.randn(32, 8, generator=gen).to(torch.bfloat16).to(device)
+    kept = es.checkpoint8(x)
+    a = es.einshard("b s h d, h d n -> b s n", kept, w)
+    b = es.einshard("b s h d, d n -> b h s n", kept, v)
+    c = es.einshard("b s h d, h d n -> n b s", kept, w)
+    ga, gb, gc = (torch.randn(t.shape, generator=gen).to(torch.bfloat16).to(device) for t in (a, b, c))
+    dx = torch.autograd.grad([a, b, c], x, [ga, gb, gc])[0]
+    d = [t.double() for t in (ga, gb, gc, w, v)]
+    want = [torch.einsum("bsn,hdn->bshd", d[0], d[3]), torch.einsum("bhsn,dn->bshd", d[1], d[4]),
+            torch.einsum("nbs,hdn->bshd", d[2], d[3])]
+    size = sum(torch.einsum(e, p.abs(), q.abs()) for e, p, q in (
+        ("bsn,hdn->bshd", d[0], d[3]), ("bhsn,dn->bshd", d[1], d[4]), ("nbs,hdn->bshd", d[2], d[3])))
+    # at most two groups are rounded by themselves before they are added
+    allowed = half_step(x.dtype) * (2 * (want[0] + want[2]).abs() + 2 * want[1].abs() + sum(want).abs()) + size * 2.0 ** -22
+    assert ((dx.double() - sum(want)).abs() <= allowed).all()
+
+
+@pytest.mark.gpu
+def test_shared_operand_on_two_streams():
+    """The same bits as on one stream."""
+    x, w, dy, _, _ = shared_case(torch.bfloat16, "cuda", (4, 512, 512), 3, torch.Generator().manual_seed(4))
+
+    def contractions(stream):
+        kept = es.checkpoint8(x)
+        ys = [es.einshard("b s c, n c -> b s n", kept, w[0])]
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            ys.append(es.einshard("b s c, n c -> b s n", kept, w[1], activation="silu").value)
+            ys.append(es.einshard("b s c, n c -> b s n", kept, w[2]))
+        torch.cuda.current_stream().wait_stream(stream)
+        return ys
+
+    ys, alone = contractions(torch.cuda.Stream()), contractions(torch.cuda.current_stream())
+    want = torch.autograd.grad(alone, x, dy)[0]
+    for _ in range(4):
+        assert torch.equal(torch.autograd.grad(ys, x, dy, retain_graph=True)[0], want)
+
+
+@pytest.mark.gpu
+def test_shared_operand_captured():
+    x, w, dy, want, size = shared_case(torch.bfloat16, "cuda", (2, 128, 256), 3, torch.Generator().manual_seed(5))
+
+    def step():
+        kept = es.checkpoint8(x)
+        ys = [es.einshard("b s c, n c -> b s n", kept, v) for v in w]
+        return torch.autograd.grad(ys, [x, *w], dy)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    with torch.no_grad():
+        x.mul_(0.5)
+        dy[0].mul_(2)
+    graph.replay()
+    for a, b in zip(out, step()):
+        assert torch.equal(a, b)

@@ -158,6 +158,26 @@ void gemm_out(const at::Tensor& a, const at::Tensor& b, at::Tensor out, int64_t 
   run_gemm(a, b, out, act, err);
 }
 
+// sum_i a[i] @ b[i], added in one accumulator; nothing where the parts' layouts differ.
+c10::optional<at::Tensor> gemm_parts(const std::vector<at::Tensor>& a, const std::vector<at::Tensor>& b,
+                                     const at::Tensor& err) {
+  TORCH_CHECK(!a.empty() && a.size() == b.size(), "einshard native gemm: as many left as right operands");
+  const c10::cuda::CUDAGuard guard(a[0].device());
+  at::Tensor out = at::empty({a[0].size(0), a[0].size(1), b[0].size(2)}, a[0].options());
+  std::vector<es::GemmArgs> parts;
+  for (size_t i = 0; i < a.size(); ++i) {
+    TORCH_CHECK(a[i].device() == out.device() && b[i].device() == out.device() &&
+                    a[i].scalar_type() == out.scalar_type(),
+                "einshard native gemm: parts of one device and type");
+    parts.push_back(gemm_args(a[i], b[i], out, 0, err));
+  }
+  const int rc = es::gemm_launch_parts(parts, at::cuda::getCurrentCUDAStream());
+  if (rc == static_cast<int>(cudaErrorNotSupported)) return c10::nullopt;
+  TORCH_CHECK(rc == 0, "einshard native gemm: launch failed (", rc, ")");
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return out;
+}
+
 int act_dtype(const at::Tensor& t) {
   TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, "einshard silu: bf16 or fp16");
   return t.scalar_type() == at::kBFloat16 ? 0 : 1;
@@ -1080,6 +1100,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         return es::conv_pair_otile(static_cast<int>(C), static_cast<int>(O), static_cast<int>(KH), static_cast<int>(KW));
       }, "output-channel tile of the CTA-pair conv for this shape (0: the kernel does not take it)");
   m.def("roll_copy", &roll_copy, "cyclic roll along several dims in one kernel");
+  m.def("gemm_parts", &gemm_parts, "sum of up to four products in one accumulator, or None");
   m.def("gemm_silu", &gemm_silu, "(silu(a @ b), a @ b), fused on the wide kernel when it runs the GEMM");
   m.def("gemm_silu8", &gemm_silu8, "(silu(a @ b), codes, exponents): the product kept in 8 bits");
   m.def("gemm_silu8_grad", &gemm_silu8_grad, "((a @ b) silu'(h), silu(h)) for h kept in 8 bits");

@@ -359,8 +359,8 @@ PolicyArgs policy_args(const at::Tensor& logits, const at::Tensor& ids, const Op
   a.ref = ref.has_value() ? ref->data_ptr<float>() : nullptr;
   a.adv = adv.data_ptr<float>();
   a.adv_per_sequence = per_sequence;
-  a.lo = static_cast<float>(lo);
-  a.hi = static_cast<float>(hi);
+  a.least = 1.0 - lo;
+  a.most = 1.0 + hi;
   a.kl = static_cast<float>(kl);
   a.inv_temp = static_cast<float>(1.0 / temperature);
   a.reduction = static_cast<int>(reduction);
@@ -390,10 +390,10 @@ std::vector<at::Tensor> policy_forward_op(const at::Tensor& logits, const at::Te
   at::Tensor loss = at::empty({}, f32), kl_out = at::empty({}, f32), clipped = at::empty({}, f32);
   at::Tensor logp = at::empty({a.tokens}, f32), terms = at::empty({a.tokens, 4}, f32);
   at::Tensor norm = at::empty({a.tokens, 2}, f32), shares = at::empty({sequences}, f32);
-  at::Tensor sums = at::empty({policy_sum_blocks(a.tokens), 4}, f32);
+  at::Tensor sums = at::empty({policy_sum_blocks(a.tokens), 3}, f32.dtype(at::kDouble));
   PolicyState s = policy_state(terms, norm, shares);
   s.logp = logp.data_ptr<float>();
-  s.sums = reinterpret_cast<float4*>(sums.data_ptr<float>());
+  s.sums = reinterpret_cast<PolicySums*>(sums.data_ptr<double>());
   s.loss = loss.data_ptr<float>();
   s.kl = kl_out.data_ptr<float>();
   s.clipped = clipped.data_ptr<float>();

@@ -85,11 +85,9 @@ GemmShape make_shape_pair(const GemmArgs& g) {
   return s;
 }
 
-// Launch a 2-SM kernel instantiation on clusters of two CTAs.
-template <class Epi>
-int launch_pair(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mc, const GemmShape& s,
-                const Epi& epi, int num_sms, cudaStream_t stream) {
-  auto kernel = gemm_tc2_kernel<Epi>;
+// Launch a 2-SM kernel instantiation on clusters of two CTAs; maps: one operand pair's, or a PartMaps.
+template <class Kernel, class... Maps>
+int launch_clusters(Kernel kernel, const GemmShape& s, int num_sms, cudaStream_t stream, const Maps&... args) {
   static unsigned long long attr_set = 0;
   int dev = 0;
   cudaGetDevice(&dev);
@@ -113,7 +111,13 @@ int launch_pair(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap&
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, ma, mb, mc, s, epi));
+  return static_cast<int>(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
+template <class Epi>
+int launch_pair(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mc, const GemmShape& s,
+                const Epi& epi, int num_sms, cudaStream_t stream) {
+  return launch_clusters(gemm_tc2_kernel<Epi>, s, num_sms, stream, ma, mb, mc, s, epi);
 }
 
 // C = A B computed as C^T = B^T A^T: operand roles and majorness swap, the
@@ -288,6 +292,47 @@ static int launch_store(const GemmArgs& g0, cudaStream_t stream) {
   epi.tma = make_output_map(g, trans, &mc) ? 1 : 0;
   kernel<<<grid, kThreads, kSmemBytes, stream>>>(ma, mb, mc, s, epi, GemmLoads{});
   return static_cast<int>(cudaGetLastError());
+}
+
+template <typename OutT>
+static int launch_parts(const std::vector<GemmArgs>& parts, cudaStream_t stream) {
+  GemmArgs g = parts[0];
+  PartMaps maps;
+  memset(&maps, 0, sizeof(maps));
+  int blocks = 0;
+  for (int i = 0; i < kMaxParts; ++i) {
+    maps.first[i] = 0x7fffffff;
+    if (i >= static_cast<int>(parts.size())) continue;
+    make_operand_maps(parts[i], &maps.a[i], &maps.b[i], true);
+    maps.first[i] = blocks;
+    blocks += (parts[i].K + kBK - 1) / kBK;
+  }
+  GemmShape s = make_shape_pair(g);
+  s.num_kb = blocks;
+  StoreEpilogue<OutT> epi;
+  epi.C = reinterpret_cast<OutT*>(g.C);
+  epi.ldc = g.ldc;
+  epi.batch_stride = g.c_batch_stride;
+  epi.act = kActNone;
+  epi.trans = 0;
+  epi.vec_ok = ((reinterpret_cast<uintptr_t>(g.C) & 15) == 0) && ((g.ldc * 2) % 16 == 0) &&
+               (g.batch == 1 || (g.c_batch_stride * 2) % 16 == 0);
+  CUtensorMap mc;
+  epi.tma = make_output_map(g, false, &mc) ? 1 : 0;
+  return launch_clusters(gemm_tc2_parts_kernel<StoreEpilogue<OutT>>, s, g.num_sms, stream, maps, mc, s, epi);
+}
+
+int gemm_launch_parts(const std::vector<GemmArgs>& parts, cudaStream_t stream) {
+  if (parts.size() < 2 || parts.size() > kMaxParts) return static_cast<int>(cudaErrorNotSupported);
+  const GemmArgs& g = parts[0];
+  for (const GemmArgs& p : parts) {
+    if (check_gemm_args(p) || p.M != g.M || p.N != g.N || p.batch != g.batch || p.C != g.C || p.dtype != g.dtype)
+      return -1;
+    if (p.a_mn != g.a_mn || p.b_mn != g.b_mn) return static_cast<int>(cudaErrorNotSupported);
+  }
+  if (g.out_dtype == kDtypeBF16) return launch_parts<__nv_bfloat16>(parts, stream);
+  if (g.out_dtype == kDtypeF16) return launch_parts<__half>(parts, stream);
+  return static_cast<int>(cudaErrorNotSupported);
 }
 
 // ------------------------------------------------------------------ stream-K tail

@@ -50,6 +50,11 @@ const char* check_gemm_args(const GemmArgs& g);
 void make_operand_maps(const GemmArgs& g, CUtensorMap* ma, CUtensorMap* mb, bool pair = false);
 bool use_pair_kernel(const GemmArgs& g);
 int gemm_launch(const GemmArgs& g, cudaStream_t stream);
+// C = sum of A_i @ B_i over 2 to 4 operand pairs that differ in K (and their
+// pointers and strides) alone: one accumulator, one rounding, no partial
+// products in memory.  cudaErrorNotSupported (nothing launched) for operands of
+// different majorness.
+int gemm_launch_parts(const std::vector<GemmArgs>& parts, cudaStream_t stream);
 // C = silu(A @ B) and pre = A @ B (same shape as C, row pitch ld_pre) in one
 // launch of the wide kernel; cudaErrorNotSupported when the shapes or layouts
 // do not allow it (nothing is launched).

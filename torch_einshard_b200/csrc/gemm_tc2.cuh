@@ -42,11 +42,40 @@ struct SharedState2 {
   int epi[32];
 };
 
+// Where K block kb of the product is read: one pair of operands, or several
+// whose products are added (each part's K in whole blocks, zeros behind it).
+struct OnePart {
+  const CUtensorMap& a;
+  const CUtensorMap& b;
+  __device__ __forceinline__ void at(int kb, const CUtensorMap*& ma, const CUtensorMap*& mb, int& k0) const {
+    ma = &a;
+    mb = &b;
+    k0 = kb * kBK;
+  }
+};
+
+constexpr int kMaxParts = 4;
+struct PartMaps {
+  CUtensorMap a[kMaxParts], b[kMaxParts];
+  int first[kMaxParts];  // K block where part i starts; past the last one for parts that are not there
+};
+
+struct SomeParts {
+  const PartMaps& parts;
+  __device__ __forceinline__ void at(int kb, const CUtensorMap*& ma, const CUtensorMap*& mb, int& k0) const {
+    int i = 0;
+    while (i + 1 < kMaxParts && kb >= parts.first[i + 1]) ++i;
+    ma = &parts.a[i];
+    mb = &parts.b[i];
+    k0 = (kb - parts.first[i]) * kBK;
+  }
+};
+
 // The kernel body.  kEpiWarps 4 hands the policy 256 columns a warp; 8 hands it 128
 // (two warps a lane quadrant, for longer epilogues).
-template <class Epi, int kEpiWarps>
-__device__ __forceinline__ void gemm_tc2_body(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmC,
-                                              const GemmShape& shp, Epi& epi) {
+template <class Epi, int kEpiWarps, class Source>
+__device__ __forceinline__ void gemm_tc2_body(const Source& source, const CUtensorMap& tmC, const GemmShape& shp,
+                                              Epi& epi) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -78,8 +107,11 @@ __device__ __forceinline__ void gemm_tc2_body(const CUtensorMap& tmA, const CUte
     fence_mbar_init();
   }
   if (warp == 0 && lane == 0) {
-    tma_prefetch_desc(&tmA);
-    tma_prefetch_desc(&tmB);
+    const CUtensorMap *ma, *mb;
+    int k0;
+    source.at(0, ma, mb, k0);
+    tma_prefetch_desc(ma);
+    tma_prefetch_desc(mb);
   }
   if (warp == 1) {
     tmem_alloc_pair(&st->tmem_base, kTmemCols);
@@ -110,18 +142,20 @@ __device__ __forceinline__ void gemm_tc2_body(const CUtensorMap& tmA, const CUte
           uint8_t* b = sB + s * kB2Bytes;
           const uint32_t fbar = full_leader0 + s * 8;
           if (leader) mbar_arrive_expect_tx(&st->full[s], 2 * kStage2Bytes);
-          const int k0 = kb * kBK;
+          const CUtensorMap *ma, *mb;
+          int k0;
+          source.at(kb, ma, mb, k0);
           if (!shp.a_mn) {
-            tma_load_3d_pair(a, &tmA, fbar, k0, c.m0, c.b);
+            tma_load_3d_pair(a, ma, fbar, k0, c.m0, c.b);
           } else {
-            tma_load_3d_pair(a, &tmA, fbar, c.m0, k0, c.b);
-            tma_load_3d_pair(a + 8192, &tmA, fbar, c.m0 + 64, k0, c.b);
+            tma_load_3d_pair(a, ma, fbar, c.m0, k0, c.b);
+            tma_load_3d_pair(a + 8192, ma, fbar, c.m0 + 64, k0, c.b);
           }
           if (!shp.b_mn) {
-            tma_load_3d_pair(b, &tmB, fbar, k0, n_half, c.b);
+            tma_load_3d_pair(b, mb, fbar, k0, n_half, c.b);
           } else {
-            tma_load_3d_pair(b, &tmB, fbar, n_half, k0, c.b);
-            tma_load_3d_pair(b + 8192, &tmB, fbar, n_half + 64, k0, c.b);
+            tma_load_3d_pair(b, mb, fbar, n_half, k0, c.b);
+            tma_load_3d_pair(b + 8192, mb, fbar, n_half + 64, k0, c.b);
           }
         }
         __syncwarp();
@@ -230,7 +264,15 @@ template <class Epi>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_tc2_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ CUtensorMap tmC, const GemmShape shp, Epi epi) {
-  gemm_tc2_body<Epi, 4>(tmA, tmB, tmC, shp, epi);
+  gemm_tc2_body<Epi, 4>(OnePart{tmA, tmB}, tmC, shp, epi);
+}
+
+// Products of several operand pairs added in one accumulator.
+template <class Epi>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_tc2_parts_kernel(const __grid_constant__ PartMaps parts, const __grid_constant__ CUtensorMap tmC,
+                          const GemmShape shp, Epi epi) {
+  gemm_tc2_body<Epi, 4>(SomeParts{parts}, tmC, shp, epi);
 }
 
 // For epilogues that are long and store from registers: eight epilogue warps, no
@@ -243,7 +285,7 @@ template <class Epi>
 __global__ void __launch_bounds__(kLongThreads, 1)
     gemm_tc2_long_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                          const GemmShape shp, Epi epi) {
-  gemm_tc2_body<Epi, kLongEpiWarps>(tmA, tmB, tmA, shp, epi);
+  gemm_tc2_body<Epi, kLongEpiWarps>(OnePart{tmA, tmB}, tmA, shp, epi);
 }
 
 }  // namespace es

@@ -241,12 +241,13 @@ __device__ __forceinline__ Inputs inputs_of(const PolicyArgs& a, const PolicySta
 __device__ __forceinline__ float4 terms_of(const PolicyArgs& a, const Inputs& in, float m, float s, float* logp) {
   const float lp = (in.z - m) * a.inv_temp - logf(s);
   const float ratio = expf(lp - (a.old != nullptr ? in.old : lp));
-  const float kept = fminf(fmaxf(ratio, 1.0f - a.lo), 1.0f + a.hi);
+  const float kept = fminf(fmaxf(ratio, static_cast<float>(a.least)), static_cast<float>(a.most));
   const float s1 = ratio * in.adv, s2 = kept * in.adv;
   const bool clipped = s1 > s2;
   float loss = 0.0f, slope = 0.0f, kl = 0.0f;
   if (in.adv != 0.0f) {
-    loss = clipped ? -s2 : -s1;
+    // a clipped token's ratio is the border itself: its rounding to 32 bits would be every clipped token's error
+    loss = clipped ? static_cast<float>(-(ratio < 1.0f ? a.least : a.most) * in.adv) : -s1;
     slope = clipped ? 0.0f : -s1;
   }
   if (a.ref != nullptr) {
@@ -448,21 +449,29 @@ __global__ void __launch_bounds__(1024) policy_shares_kernel(const PolicyArgs a,
   }
 }
 
-// Sum over the block of 1024 threads, in its first thread.
-__device__ __forceinline__ float4 block_total(float4 s, float4* red) {
+// Sum over the block of 1024 threads, in its first thread.  In 64 bits: terms of
+// both signs cancel in the loss, and at 12288 tokens 32-bit sums were as far off as
+// all the log-probabilities together.
+__device__ __forceinline__ PolicySums block_total(PolicySums s, PolicySums* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  s = make_float4(warp_sum(s.x), warp_sum(s.y), warp_sum(s.z), 0.0f);
+  s = {warp_sum(s.loss), warp_sum(s.kl), warp_sum(s.clipped)};
   if (lane == 0) red[warp] = s;
   __syncthreads();
   s = red[lane];
-  return make_float4(warp_sum(s.x), warp_sum(s.y), warp_sum(s.z), 0.0f);
+  return {warp_sum(s.loss), warp_sum(s.kl), warp_sum(s.clipped)};
+}
+
+__device__ __forceinline__ void store_total(const PolicyArgs& a, const PolicyState& o, const PolicySums& s) {
+  *o.loss = static_cast<float>(a.weight * s.loss);
+  *o.kl = static_cast<float>(s.kl);
+  *o.clipped = static_cast<float>(s.clipped);
 }
 
 // Loss, KL and clipped share: every block a run of tokens, the only (kLast) one the scalars.
 template <bool kLast>
 __global__ void __launch_bounds__(1024) policy_sum_kernel(const PolicyArgs a, const PolicyState o, long long run) {
-  __shared__ float4 red[32];
-  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  __shared__ PolicySums red[32];
+  PolicySums s = {0.0, 0.0, 0.0};
   const long long last = min(a.tokens, (blockIdx.x + 1) * run);
   // eight tokens a thread in flight
   for (long long t0 = blockIdx.x * run + threadIdx.x; t0 < last; t0 += 8 * 1024) {
@@ -475,31 +484,28 @@ __global__ void __launch_bounds__(1024) policy_sum_kernel(const PolicyArgs a, co
       f[u] = t < last ? share_of(a, o, t) : 0.0f;
     }
 #pragma unroll
-    for (int u = 0; u < 8; ++u) s.x += f[u] * v[u].x, s.y += f[u] * v[u].y, s.z += f[u] * v[u].z;
+    for (int u = 0; u < 8; ++u) {
+      const double share = f[u];
+      s.loss += share * v[u].x, s.kl += share * v[u].y, s.clipped += share * v[u].z;
+    }
   }
   s = block_total(s, red);
   if (threadIdx.x != 0) return;
-  if (kLast) {
-    *o.loss = a.weight * s.x;
-    *o.kl = s.y;
-    *o.clipped = s.z;
-  } else {
+  if (kLast)
+    store_total(a, o, s);
+  else
     o.sums[blockIdx.x] = s;
-  }
 }
 
 __global__ void __launch_bounds__(1024) policy_total_kernel(const PolicyArgs a, const PolicyState o, int blocks) {
-  __shared__ float4 red[32];
-  float4 s = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  __shared__ PolicySums red[32];
+  PolicySums s = {0.0, 0.0, 0.0};
   for (int i = threadIdx.x; i < blocks; i += 1024) {
-    const float4 v = o.sums[i];
-    s.x += v.x, s.y += v.y, s.z += v.z;
+    const PolicySums v = o.sums[i];
+    s.loss += v.loss, s.kl += v.kl, s.clipped += v.clipped;
   }
   s = block_total(s, red);
-  if (threadIdx.x != 0) return;
-  *o.loss = a.weight * s.x;
-  *o.kl = s.y;
-  *o.clipped = s.z;
+  if (threadIdx.x == 0) store_total(a, o, s);
 }
 
 template <typename T>

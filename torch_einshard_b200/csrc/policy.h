@@ -19,10 +19,15 @@ struct PolicyArgs {
   const float* ref = nullptr;      // [tokens]; null: no KL term
   const float* adv = nullptr;      // [tokens], or one a sequence
   int adv_per_sequence = 0;
-  float lo = 0.2f, hi = 0.2f, kl = 0.0f, inv_temp = 1.0f;
+  double least = 0.8, most = 1.2;  // the clip range
+  float kl = 0.0f, inv_temp = 1.0f;
   float weight = 1.0f;             // factor of the loss
   int reduction = kReduceMean;
   int sms = 148;
+};
+
+struct PolicySums {
+  double loss, kl, clipped;
 };
 
 struct PolicyState {
@@ -30,7 +35,7 @@ struct PolicyState {
   float4* terms = nullptr;  // [tokens] loss, KL, clipped, derivative of the loss by logp (without weights)
   float2* norm = nullptr;   // [tokens] largest logit and log2 of the sum of exponentials
   float* share = nullptr;   // [sequences] a token's share in the reduction, where the mask decides it
-  float4* sums = nullptr;   // [policy_sum_blocks] scratch
+  PolicySums* sums = nullptr;  // [policy_sum_blocks] scratch
   float* loss = nullptr;    // scalars
   float* kl = nullptr;
   float* clipped = nullptr;

@@ -106,7 +106,7 @@ class Saved8:
     kept.  ``restore()`` gives the values that backward sees.
     """
 
-    __slots__ = ("value", "codes", "exps", "_act", "_base", "_order", "_pre")
+    __slots__ = ("value", "codes", "exps", "_act", "_base", "_order", "_pre", "_readers")
 
     def __init__(self, value, codes, exps, act=False, base=None, order=None, pre=None):
         self.value, self.codes, self.exps = value, codes, exps
@@ -114,6 +114,7 @@ class Saved8:
         self._base = tuple(value.shape) if base is None else base  # shape of the tensor that was quantised
         self._order = order  # permutation from there to the value's axes
         self._pre = pre  # the pre-activation's place in the graph (a tensor without values of its own)
+        self._readers = None  # the place and box of :class:`_Readers`
 
     @property
     def shape(self):
@@ -138,8 +139,9 @@ class Saved8:
 
     def with_value(self, value):
         """The same codes for a value that differs by its place in the graph alone."""
-        pre = self._pre if value is self.value else None
-        return Saved8(value, self.codes, self.exps, self._act, self._base, self._order, pre)
+        if value is self.value:
+            return self
+        return Saved8(value, self.codes, self.exps, self._act, self._base, self._order)
 
     def _meta(self):
         return self._act, self._base, self._order, self.value.dtype
@@ -269,18 +271,83 @@ def _place_of(a):
     return a.new_empty(()).expand(a.shape)
 
 
+class _Box:
+    """What one backward pass's products leave for the gradient of the operand that they share, by the pass's number:
+    passes over one graph (again, or from two threads) do not meet."""
+
+    __slots__ = ("passes",)
+
+    def __init__(self):
+        self.passes = {}
+
+    def add(self, *part):
+        self.passes.setdefault(torch._C._current_graph_task_id(), []).append(part)
+
+    def take(self):
+        return self.passes.pop(torch._C._current_graph_task_id(), [])
+
+
+class _Readers(torch.autograd.Function):
+    """The place in the graph where the gradients of an operand's contractions meet.
+
+    sum_i dz_i y_i^T is formed at once, in 32 bits, and rounded once; autograd
+    would add the contractions' rounded gradients one by one.  A contraction's
+    backward leaves its factors in the box and hands on no gradient."""
+
+    @staticmethod
+    def forward(ctx, x, box):
+        ctx.set_materialize_grads(False)
+        ctx.box = box
+        return _place_of(x)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, _):
+        parts = ctx.box.take()
+        here = torch.cuda.current_stream(parts[0][2].device) if parts and parts[0][2].is_cuda else None
+        for _, _, dz, y, stream in parts:
+            if stream != here:  # its backward ran on its own stream
+                here.wait_stream(stream)
+                dz.record_stream(here)
+                y.record_stream(here)
+        groups = {}
+        for plan, native, dz, y, _ in parts:
+            groups.setdefault((native, plan.x_order, plan.x_shape, plan.gemm[0], plan.gemm[3]), []).append((plan, dz, y))
+        total = None
+        for (native, *_), group in groups.items():
+            dx = _operand_grad(native, group)
+            total = dx if total is None else total + dx
+        return total, None
+
+
+def _operand_grad(native, group):
+    """sum of dz y^T over contractions of one operand alike but for their other axes."""
+    plan = group[0][0]
+    if native:
+        dx = gemm.native_bmm_sum([(p.product_of(dz), p.operand_y(y).transpose(1, 2)) for p, dz, y in group])
+        return _moved(dx.view(plan.x_shape), None if plan.x_order is None else _inverse(plan.x_order))
+    total, dtype = None, group[0][1].dtype
+    wide = torch.promote_types(dtype, torch.float32) if len(group) > 1 else dtype
+    for p, dz, y in group:
+        (ex, ey), ez = p.equation.split("->")[0].split(","), p.equation.split("->")[1]
+        dx = contract(f"{ez},{ey}->{ex}", dz.to(wide), y.to(wide))
+        total = dx if total is None else total + dx
+    return total.to(dtype)
+
+
 class _Contraction8(torch.autograd.Function):
     """x y with x kept in 8 bits.
 
-    ``x`` carries the values.  Its gradient goes to ``x``, or, where x is a
-    silu, to ``pre``, its pre-activation's place in the graph (``x`` is detached
-    then).  With ``silu`` the result is silu(x y), its pre-activation in 8 bits
-    and that one's place."""
+    ``x`` carries the values.  Its gradient goes to ``place`` (``x`` is detached
+    then): its pre-activation's place in the graph where x is a silu, and with a
+    ``box`` the place where its contractions' gradients meet.  Without a place it
+    goes to ``x``.  With ``silu`` the result is silu(x y), its pre-activation in
+    8 bits and that one's place."""
 
     @staticmethod
-    def forward(ctx, x, pre, y, plan, native, codes, exps, meta, silu):
+    def forward(ctx, x, place, box, y, plan, native, codes, exps, meta, silu):
         ctx.set_materialize_grads(False)
-        ctx.plan, ctx.native, ctx.meta, ctx.silu = plan, native, meta, silu
+        ctx.plan, ctx.native, ctx.meta, ctx.silu, ctx.box = plan, native, meta, silu, box
         mod = _native.require() if native else None
         if not silu:
             ctx.save_for_backward(y, codes, exps)
@@ -310,8 +377,12 @@ class _Contraction8(torch.autograd.Function):
         if grad_pre is not None:
             grad = grad_pre if grad is None else grad + grad_pre
         if grad is None:
-            return (None,) * 9
-        want_x, want_pre, want_y = ctx.needs_input_grad[:3]
+            return (None,) * 10
+        want_x, want_pre, _, want_y = ctx.needs_input_grad[:4]
+        if ctx.box is not None:
+            if torch._C._will_engine_execute_node(ctx.next_functions[1][0]):  # the operand's gradient is asked for
+                ctx.box.add(plan, native, grad, y, torch.cuda.current_stream(grad.device) if grad.is_cuda else None)
+            want_x = want_pre = False
         act, base, order, dtype = ctx.meta
         dx = dpre = dy = restored = None
         if native:
@@ -324,8 +395,7 @@ class _Contraction8(torch.autograd.Function):
                                                                    _native.error_word(gz.device))
                 dpre = _moved(dpre.view(plan.x_shape), None if plan.x_order is None else _inverse(plan.x_order))
             elif want_x or want_pre:
-                dx = gemm.native_bmm(gz, yt).view(plan.x_shape)
-                dx = _moved(dx, None if plan.x_order is None else _inverse(plan.x_order))
+                dx = _operand_grad(native, [(plan, grad, y)])
             if want_y:
                 if restored is None:
                     restored = plan.operand_x(_restore_operand(codes, exps, ctx.meta))
@@ -338,12 +408,12 @@ class _Contraction8(torch.autograd.Function):
         else:
             (ex, ey), ez = plan.equation.split("->")[0].split(","), plan.equation.split("->")[1]
             if want_x or want_pre:
-                dx = contract(f"{ez},{ey}->{ex}", grad, y)
+                dx = _operand_grad(native, [(plan, grad, y)])
             if want_y:
                 dy = contract(f"{ez},{ex}->{ey}", grad, _restore_operand(codes, exps, ctx.meta))
         if want_pre and dpre is None:
             dpre = _silu_grad(dx, codes, exps, order)
-        return dx if want_x else None, dpre, dy, None, None, None, None, None, None
+        return dx if want_x else None, dpre, None, dy, None, None, None, None, None, None
 
 
 def _same_rows(plan, codes, base, order):
@@ -363,9 +433,14 @@ def contract_saved(equation, saved, y, activation=None):
                          f"not {y.dtype} on {y.device}")
     plan = _product(equation, tuple(x.shape), tuple(y.shape))
     native = all(plan.gemm) and gemm.eligible(x, y)
-    pre = saved._pre
-    out = _Contraction8.apply(x if pre is None else x.detach(), pre, y, plan, native, saved.codes, saved.exps,
-                              saved._meta(), activation is not None)
+    place, box = saved._pre, None
+    if place is None and x.requires_grad and torch.is_grad_enabled():
+        if saved._readers is None:
+            box = _Box()
+            saved._readers = _Readers.apply(x, box), box
+        place, box = saved._readers
+    out = _Contraction8.apply(x if place is None else x.detach(), place, box, y, plan, native, saved.codes,
+                              saved.exps, saved._meta(), activation is not None)
     if activation is None:
         return out
     a, pre, codes, exps = out
