@@ -158,6 +158,10 @@ void gemm_out(const at::Tensor& a, const at::Tensor& b, at::Tensor out, int64_t 
   run_gemm(a, b, out, act, err);
 }
 
+at::Tensor native_bmm(const at::Tensor& a, const at::Tensor& b, const at::Tensor& err) {
+  return gemm(a, b, dtype_code(a.scalar_type()), 0, err);
+}
+
 // sum_i a[i] @ b[i], added in one accumulator; nothing where the parts' layouts differ.
 c10::optional<at::Tensor> gemm_parts(const std::vector<at::Tensor>& a, const std::vector<at::Tensor>& b,
                                      const at::Tensor& err) {
@@ -206,56 +210,46 @@ std::vector<at::Tensor> gemm_silu(const at::Tensor& a, const at::Tensor& b, cons
 
 int64_t quant_blocks(int64_t n) { return (n + es::kQuantBlock - 1) / es::kQuantBlock; }
 
+// Columns between two rows of what the 8-bit SiLU products write: whole sectors.
+int64_t sector_pitch(int64_t n) { return (n + 15) / 16 * 16; }
+
 // (silu(a @ b), codes [batch M, N], exponents): the product kept in 8 bits from its 32-bit accumulator, in the
-// epilogue of the pair kernel, or from an fp32 product where that does not take the shape.
+// epilogue of the pair kernel.  Rows of the first two are a multiple of 16 apart.
 std::vector<at::Tensor> gemm_silu8(const at::Tensor& a, const at::Tensor& b, const at::Tensor& err) {
   const c10::cuda::CUDAGuard guard(a.device());
   TORCH_CHECK(a.dim() == 3 && b.dim() == 3, "einshard gemm+silu8: 3-D operands required");
-  const int64_t rows = a.size(0) * a.size(1), n = b.size(2);
-  at::Tensor out = at::empty({a.size(0), a.size(1), n}, a.options());
-  at::Tensor codes = at::empty({rows, n}, a.options().dtype(at::kChar));
+  const int64_t rows = a.size(0) * a.size(1), n = b.size(2), pitch = sector_pitch(n);
+  at::Tensor out = at::empty({a.size(0), a.size(1), pitch}, a.options()).narrow(2, 0, n);
+  at::Tensor codes = at::empty({rows, pitch}, a.options().dtype(at::kChar)).narrow(1, 0, n);
   at::Tensor exps = at::empty({rows, quant_blocks(n)}, a.options().dtype(at::kByte));
   const es::GemmArgs g = gemm_args(a, b, out, 0, err);
-  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  int rc = es::gemm_launch_silu8(g, codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), stream);
-  if (rc == static_cast<int>(cudaErrorNotSupported)) {
-    at::Tensor h = at::empty(out.sizes(), out.options().dtype(at::kFloat));
-    run_gemm(a, b, h, 0, err);
-    rc = es::quant8_silu(h.data_ptr<float>(), out.data_ptr(), dtype_code(out.scalar_type()), codes.data_ptr<int8_t>(),
-                         exps.data_ptr<uint8_t>(), rows, n, num_sms(a.get_device()), stream);
-  }
+  const int rc = es::gemm_launch_silu8(g, codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(),
+                                       at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(rc == 0, "einshard gemm+silu8: launch failed (", rc, ")");
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return {out, codes, exps};
 }
 
-// ((a @ b) silu'(h^), silu(h^)) for a pre-activation h^ of the product's shape kept in 8 bits.
-std::vector<at::Tensor> gemm_silu8_grad(const at::Tensor& a, const at::Tensor& b, const at::Tensor& codes,
+// ((a @ b) silu'(h^), silu(h^)) for a pre-activation h^ of the product's shape kept in 8 bits, with rows like gemm_silu8's.
+std::vector<at::Tensor> gemm_silu8_grad(const at::Tensor& a, const at::Tensor& b, const at::Tensor& kept,
                                         const at::Tensor& exps, const at::Tensor& err) {
   const c10::cuda::CUDAGuard guard(a.device());
   TORCH_CHECK(a.dim() == 3 && b.dim() == 3, "einshard gemm+silu8: 3-D operands required");
-  const int64_t rows = a.size(0) * a.size(1), n = b.size(2);
-  TORCH_CHECK(codes.device() == a.device() && codes.is_contiguous() && codes.scalar_type() == at::kChar &&
-                  codes.dim() == 2 && codes.size(0) == rows && codes.size(1) == n &&
-                  exps.device() == a.device() && exps.is_contiguous() && exps.scalar_type() == at::kByte &&
-                  exps.numel() == rows * quant_blocks(n),
+  const int64_t rows = a.size(0) * a.size(1), n = b.size(2), pitch = sector_pitch(n);
+  TORCH_CHECK(kept.device() == a.device() && kept.scalar_type() == at::kChar && kept.dim() == 2 &&
+                  kept.size(0) == rows && kept.size(1) == n && exps.device() == a.device() && exps.is_contiguous() &&
+                  exps.scalar_type() == at::kByte && exps.numel() == rows * quant_blocks(n),
               "einshard gemm+silu8: codes and exponents of the product's shape");
-  at::Tensor out = at::empty({a.size(0), a.size(1), n}, a.options());
-  at::Tensor act = at::empty_like(out);
-  const es::GemmArgs g = gemm_args(a, b, out, 0, err);
-  cudaStream_t stream = at::cuda::getCurrentCUDAStream();
-  int rc = es::gemm_launch_silu8_grad(g, codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), act.data_ptr(), stream);
-  if (rc == static_cast<int>(cudaErrorNotSupported)) {
-    at::Tensor da = at::empty_like(out);
-    run_gemm(a, b, da, 0, err);
-    const int dt = dtype_code(out.scalar_type()), sms = num_sms(a.get_device());
-    rc = es::restore8(codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), da.data_ptr(), out.data_ptr(), dt,
-                      es::kRestoreSiluGrad, rows, n, sms, stream);
-    if (rc == 0)
-      rc = es::restore8(codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), nullptr, act.data_ptr(), dt,
-                        es::kRestoreSilu, rows, n, sms, stream);
-    g_launches.fetch_add(1, std::memory_order_relaxed);
+  at::Tensor codes = kept;
+  if (kept.stride(0) != pitch || kept.stride(1) != 1) {
+    codes = at::empty({rows, pitch}, kept.options()).narrow(1, 0, n);
+    codes.copy_(kept);
   }
+  at::Tensor out = at::empty({a.size(0), a.size(1), pitch}, a.options()).narrow(2, 0, n);
+  at::Tensor act = at::empty({a.size(0), a.size(1), pitch}, a.options()).narrow(2, 0, n);
+  const es::GemmArgs g = gemm_args(a, b, out, 0, err);
+  const int rc = es::gemm_launch_silu8_grad(g, codes.data_ptr<int8_t>(), exps.data_ptr<uint8_t>(), act.data_ptr(),
+                                            at::cuda::getCurrentCUDAStream());
   TORCH_CHECK(rc == 0, "einshard gemm+silu8: launch failed (", rc, ")");
   g_launches.fetch_add(1, std::memory_order_relaxed);
   return {out, act};
@@ -1100,10 +1094,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         return es::conv_pair_otile(static_cast<int>(C), static_cast<int>(O), static_cast<int>(KH), static_cast<int>(KW));
       }, "output-channel tile of the CTA-pair conv for this shape (0: the kernel does not take it)");
   m.def("roll_copy", &roll_copy, "cyclic roll along several dims in one kernel");
-  m.def("gemm_parts", &gemm_parts, "sum of up to four products in one accumulator, or None");
   m.def("gemm_silu", &gemm_silu, "(silu(a @ b), a @ b), fused on the wide kernel when it runs the GEMM");
-  m.def("gemm_silu8", &gemm_silu8, "(silu(a @ b), codes, exponents): the product kept in 8 bits");
-  m.def("gemm_silu8_grad", &gemm_silu8_grad, "((a @ b) silu'(h), silu(h)) for h kept in 8 bits");
   m.def("silu_forward", &silu_forward, "elementwise silu");
   m.def("silu_backward", &silu_backward, "grad * silu'(h)");
   m.def("wait_probe", &wait_probe, "bounded wait on a flag (tests the timeout path)");
@@ -1207,5 +1198,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("set_tma_l2_promotion", [](int64_t v) { es::tma_l2_promotion() = static_cast<int>(v); },
         "L2 promotion of TMA loads: 0 none, 1 64B, 2 128B, 3 256B (tuning)");
   es::bind_training_ops(m, g_launches);
+  es::bind_saved8_ops(m, {&native_bmm, &gemm_parts, &gemm_silu8, &gemm_silu8_grad});
   m.def("launch_count", []() { return g_launches.load(); }, "native kernel launches so far");
 }

@@ -75,7 +75,8 @@ std::vector<at::Tensor> quant8_silu_op(const at::Tensor& h, int64_t out_dtype) {
   return {out, codes, exps};
 }
 
-// What the codes stand for, its silu, or grad times its silu' (mode 0, 1, 2)
+}  // namespace
+
 at::Tensor restore8_op(const at::Tensor& codes, const at::Tensor& exps, const c10::optional<at::Tensor>& grad,
                        int64_t dtype, int64_t mode) {
   TORCH_CHECK(codes.is_cuda() && codes.dim() == 2 && codes.is_contiguous() && codes.scalar_type() == at::kChar,
@@ -100,6 +101,8 @@ at::Tensor restore8_op(const at::Tensor& codes, const at::Tensor& exps, const c1
           "restore8");
   return out;
 }
+
+namespace {
 
 // ------------------------------------------------------------------ norms
 
@@ -251,8 +254,9 @@ struct Final : public torch::autograd::Function<Final> {
   }
 };
 
-// `grads` as results of what they were formed from, where a graph of the backward pass is wanted.
-void finalise(std::vector<at::Tensor>& grads, const torch::autograd::variable_list& from) {
+}  // namespace
+
+void finalise(std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& from) {
   if (!at::GradMode::is_enabled()) return;
   for (const at::Tensor& input : from) {
     if (!input.defined() || !input.requires_grad()) continue;
@@ -261,6 +265,8 @@ void finalise(std::vector<at::Tensor>& grads, const torch::autograd::variable_li
     return;
   }
 }
+
+namespace {
 
 Opt some(const at::Tensor& t) { return t.defined() ? Opt(t) : Opt(); }
 at::Tensor none(const Opt& t) { return t.has_value() ? *t : at::Tensor(); }

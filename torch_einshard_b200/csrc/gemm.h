@@ -60,11 +60,12 @@ int gemm_launch_parts(const std::vector<GemmArgs>& parts, cudaStream_t stream);
 // do not allow it (nothing is launched).
 int gemm_launch_silu_dual(const GemmArgs& g, void* pre, long long ld_pre, long long pre_batch_stride,
                           cudaStream_t stream);
-// C = silu(A @ B) with the product kept in 8 bits (quant8.h: codes [batch M, N],
-// exps [batch M, ceil(N / 32)]), in one launch of the 256 x 256 pair kernel.
-// cudaErrorNotSupported (nothing launched) for shapes or layouts it does not take.
+// C = silu(A @ B) with the product kept in 8 bits (quant8.h: codes of C's shape
+// and pitch, exps [batch M, ceil(N / 32)]), in one launch of the 256 x 256 pair
+// kernel.  Rows are ldc, a multiple of 16, apart; what lies between N and ldc
+// is written, too.
 int gemm_launch_silu8(const GemmArgs& g, int8_t* codes, uint8_t* exps, cudaStream_t stream);
-// C = (A @ B) silu'(h^) and act = silu(h^) (like C) for a pre-activation h^ kept in 8 bits.
+// C = (A @ B) silu'(h^) and act = silu(h^) (like C) for a pre-activation h^ kept in 8 bits (codes like C).
 int gemm_launch_silu8_grad(const GemmArgs& g, const int8_t* codes, const uint8_t* exps, void* act,
                            cudaStream_t stream);
 struct GemmShape;

@@ -49,16 +49,18 @@ __device__ __forceinline__ void load32(uint32_t* w, const void* p) {
                : "l"(p));
 }
 
-// What both epilogues know of the 8-bit tensor: rows of N codes and `blocks` exponents.
+// What both epilogues know of the 8-bit tensor and the 16-bit ones: rows of N
+// columns, `pitch` (a multiple of 16) apart, and of `blocks` exponents.  The
+// columns between N and the pitch are written (a sector at a time), not used.
 struct Codes {
   int8_t* codes;
   uint8_t* exps;
-  int blocks;
+  int blocks, pitch;
 };
 
 template <typename T>
 struct Silu8Epilogue {
-  T* out;  // [batch M, N]
+  T* out;  // [batch M, pitch]
   Codes kept;
 
   __device__ __forceinline__ void setup(int*, const GemmShape&) {}
@@ -91,11 +93,11 @@ struct Silu8Epilogue {
         sigmoid_pair(x1, x2, s1, s2);
         w[i] = floats_to_word<T>(x1 * s1, x2 * s2);
       }
-      int8_t* code_row = kept.codes + at * s.N + col;
-      T* out_row = out + at * s.N + col;
+      int8_t* code_row = kept.codes + at * kept.pitch + col;
+      T* out_row = out + at * kept.pitch + col;
       kept.exps[at * kept.blocks + col / 32] = static_cast<uint8_t>(step.byte);
       store32(out_row, w);
-      if (col + 32 <= s.N) {
+      if (col + 32 <= kept.pitch) {
         store32(out_row + 16, w + 8);
         if ((reinterpret_cast<uintptr_t>(code_row) & 31) == 0) {
           store32(code_row, q);
@@ -104,7 +106,7 @@ struct Silu8Epilogue {
           reinterpret_cast<uint4*>(code_row)[1] = make_uint4(q[4], q[5], q[6], q[7]);
         }
       } else {
-        reinterpret_cast<uint4*>(code_row)[0] = make_uint4(q[0], q[1], q[2], q[3]);  // N a multiple of 16
+        reinterpret_cast<uint4*>(code_row)[0] = make_uint4(q[0], q[1], q[2], q[3]);
       }
     }
     return true;
@@ -113,7 +115,7 @@ struct Silu8Epilogue {
 
 template <typename T>
 struct Silu8GradEpilogue {
-  T* out;  // [batch M, N]
+  T* out;  // [batch M, pitch]
   T* act;
   Codes kept;
 
@@ -129,18 +131,18 @@ struct Silu8GradEpilogue {
 #pragma unroll
     for (int j = 0; j < kCols / 32; ++j) {
       const int col = et.c.n0 + 32 * j;
-      const int8_t* p = kept.codes + at * s.N + col;
+      const int8_t* p = kept.codes + at * kept.pitch + col;
 #pragma unroll
       for (int i = 0; i < 8; ++i) code[8 * j + i] = 0;
       byte[j] = 127;
       if (row >= s.M || col >= s.N) continue;
       byte[j] = kept.exps[at * kept.blocks + col / 32];
-      if (col + 32 <= s.N && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
+      if (col + 32 <= kept.pitch && (reinterpret_cast<uintptr_t>(p) & 31) == 0) {
         load32(&code[8 * j], p);
       } else {
         const uint4 lo = reinterpret_cast<const uint4*>(p)[0];
         code[8 * j] = lo.x, code[8 * j + 1] = lo.y, code[8 * j + 2] = lo.z, code[8 * j + 3] = lo.w;
-        if (col + 32 <= s.N) {
+        if (col + 32 <= kept.pitch) {
           const uint4 hi = reinterpret_cast<const uint4*>(p)[1];
           code[8 * j + 4] = hi.x, code[8 * j + 5] = hi.y, code[8 * j + 6] = hi.z, code[8 * j + 7] = hi.w;
         }
@@ -165,11 +167,11 @@ struct Silu8GradEpilogue {
         dh[i] = floats_to_word<T>(__uint_as_float(r[2 * i]) * silu_slope(x1, s1),
                                   __uint_as_float(r[2 * i + 1]) * silu_slope(x2, s2));
       }
-      T* out_row = out + at * s.N + col;
-      T* act_row = act + at * s.N + col;
+      T* out_row = out + at * kept.pitch + col;
+      T* act_row = act + at * kept.pitch + col;
       store32(out_row, dh);
       store32(act_row, aw);
-      if (col + 32 <= s.N) {  // N a multiple of 16
+      if (col + 32 <= kept.pitch) {
         store32(out_row + 16, dh + 8);
         store32(act_row + 16, aw + 8);
       }
@@ -208,36 +210,39 @@ bool aligned32(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 
 
 // Whether the pair kernel takes the product: dense outputs whose rows are whole 32-byte sectors of 16-bit values.
 bool fits(const GemmArgs& g, const int8_t* codes) {
-  return check_gemm_args(g) == nullptr && g.N % 16 == 0 && g.out_dtype == g.dtype && g.ldc == g.N &&
-         (g.batch == 1 || g.c_batch_stride == static_cast<long long>(g.M) * g.N) && aligned32(g.C) &&
+  return check_gemm_args(g) == nullptr && g.ldc >= g.N && g.ldc % 16 == 0 && g.ldc < (1ll << 31) &&
+         g.out_dtype == g.dtype && (g.batch == 1 || g.c_batch_stride == g.M * g.ldc) && aligned32(g.C) &&
          (reinterpret_cast<uintptr_t>(codes) & 15) == 0;
+}
+
+Codes codes_of(const GemmArgs& g, const int8_t* codes, const uint8_t* exps) {
+  return {const_cast<int8_t*>(codes), const_cast<uint8_t*>(exps), (g.N + kQuantBlock - 1) / kQuantBlock,
+          static_cast<int>(g.ldc)};
 }
 
 template <typename T>
 int launch_silu8(const GemmArgs& g, int8_t* codes, uint8_t* exps, cudaStream_t stream) {
-  const Silu8Epilogue<T> epi{static_cast<T*>(g.C), {codes, exps, (g.N + kQuantBlock - 1) / kQuantBlock}};
+  const Silu8Epilogue<T> epi{static_cast<T*>(g.C), codes_of(g, codes, exps)};
   return launch_long(g, epi, stream);
 }
 
 template <typename T>
 int launch_silu8_grad(const GemmArgs& g, const int8_t* codes, const uint8_t* exps, void* act, cudaStream_t stream) {
-  const Silu8GradEpilogue<T> epi{static_cast<T*>(g.C), static_cast<T*>(act),
-                                 {const_cast<int8_t*>(codes), const_cast<uint8_t*>(exps),
-                                  (g.N + kQuantBlock - 1) / kQuantBlock}};
+  const Silu8GradEpilogue<T> epi{static_cast<T*>(g.C), static_cast<T*>(act), codes_of(g, codes, exps)};
   return launch_long(g, epi, stream);
 }
 
 }  // namespace
 
 int gemm_launch_silu8(const GemmArgs& g, int8_t* codes, uint8_t* exps, cudaStream_t stream) {
-  if (!fits(g, codes)) return static_cast<int>(cudaErrorNotSupported);
+  if (!fits(g, codes)) return static_cast<int>(cudaErrorInvalidValue);
   return g.dtype == kDtypeBF16 ? launch_silu8<__nv_bfloat16>(g, codes, exps, stream)
                                : launch_silu8<__half>(g, codes, exps, stream);
 }
 
 int gemm_launch_silu8_grad(const GemmArgs& g, const int8_t* codes, const uint8_t* exps, void* act,
                            cudaStream_t stream) {
-  if (!fits(g, codes) || !aligned32(act)) return static_cast<int>(cudaErrorNotSupported);
+  if (!fits(g, codes) || !aligned32(act)) return static_cast<int>(cudaErrorInvalidValue);
   return g.dtype == kDtypeBF16 ? launch_silu8_grad<__nv_bfloat16>(g, codes, exps, act, stream)
                                : launch_silu8_grad<__half>(g, codes, exps, act, stream);
 }

@@ -72,16 +72,6 @@ def native_bmm(a: torch.Tensor, b: torch.Tensor, out_dtype=None, act=None) -> to
     return mod.gemm(a, b, _OUT_CODE[out_dtype], _ACTS[act], _native.error_word(a.device))
 
 
-def native_bmm_sum(pairs) -> torch.Tensor:
-    """The products of several operand pairs, added in 32 bits and rounded once."""
-    if len(pairs) == 1:
-        return native_bmm(*pairs[0])
-    a, b = [_prepare(a) for a, _ in pairs], [_prepare(b) for _, b in pairs]
-    out = _native.require().gemm_parts(a, b, _native.error_word(a[0].device))
-    # more than four, or of different layouts: as one product over all their K
-    return native_bmm(torch.cat(a, 2), torch.cat(b, 1)) if out is None else out
-
-
 class _NativeMatmul(torch.autograd.Function):
     @staticmethod
     def forward(ctx, a, b):

@@ -32,7 +32,7 @@ keeps activations whole or recomputes them.
 import math
 import string
 from dataclasses import dataclass
-from functools import lru_cache
+from functools import cached_property, lru_cache
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -80,7 +80,7 @@ def _quantise(x):
 def _restored(codes, exps, dtype, mode, grad=None):
     """[rows, d] values of the codes through ``mode`` (value, silu, grad * silu')."""
     if _on_kernels(codes, dtype):
-        return _native.require().restore8(codes, exps, grad, _CODE[dtype], mode)
+        return _native.require().restore8(codes.contiguous(), exps, grad, _CODE[dtype], mode)
     wide = torch.float64 if dtype == torch.float64 else torch.float32
     e = exps.to(torch.int32).repeat_interleave(_BLOCK, dim=1)[:, :codes.shape[1]]
     x = torch.ldexp(codes.to(wide), e - 127)
@@ -106,7 +106,7 @@ class Saved8:
     kept.  ``restore()`` gives the values that backward sees.
     """
 
-    __slots__ = ("value", "codes", "exps", "_act", "_base", "_order", "_pre", "_readers")
+    __slots__ = ("value", "codes", "exps", "_act", "_base", "_order", "_pre", "_readers", "_box")
 
     def __init__(self, value, codes, exps, act=False, base=None, order=None, pre=None):
         self.value, self.codes, self.exps = value, codes, exps
@@ -114,7 +114,8 @@ class Saved8:
         self._base = tuple(value.shape) if base is None else base  # shape of the tensor that was quantised
         self._order = order  # permutation from there to the value's axes
         self._pre = pre  # the pre-activation's place in the graph (a tensor without values of its own)
-        self._readers = None  # the place and box of :class:`_Readers`
+        self._readers = None  # the place where the gradients of its native contractions meet
+        self._box = None  # and of the others, with what they leave there
 
     @property
     def shape(self):
@@ -131,7 +132,8 @@ class Saved8:
     @property
     def nbytes(self):
         """Bytes that backward keeps."""
-        return self.codes.numel() + self.exps.numel()
+        rows, d = self.codes.shape
+        return rows * (self.codes.stride(0) if d else 0) + self.exps.numel()  # up to 15 codes lie between two rows
 
     def restore(self):
         """The operand as backward reads it, in the value's type (no gradient)."""
@@ -215,21 +217,11 @@ class _Product:
     y_shape: tuple
     z_shape: tuple    # (of the product)
 
-    def operand_x(self, x):
-        B, M, _, K = self.gemm
-        return _moved(x, self.x_order).reshape(B, M, K)
-
-    def operand_y(self, y):
-        B, _, N, K = self.gemm
-        return _moved(y, self.y_order).reshape(B, K, N)
-
-    def result(self, z):
-        return _moved(z.view(self.z_shape), self.z_order)
-
-    def product_of(self, z):
-        """A tensor of the result's axes as [batch, rows, cols]."""
-        B, M, N, _ = self.gemm
-        return _moved(z, None if self.z_order is None else _inverse(self.z_order)).reshape(B, M, N)
+    @cached_property
+    def on_kernels(self):
+        """The plan of csrc/bindings_saved8.cpp."""
+        orders = [() if o is None else o for o in (self.x_order, self.y_order, self.z_order)]
+        return _native.require().ContractPlan(self.gemm, *orders, self.x_shape, self.y_shape, self.z_shape)
 
 
 @lru_cache(maxsize=1024)
@@ -271,28 +263,13 @@ def _place_of(a):
     return a.new_empty(()).expand(a.shape)
 
 
-class _Box:
-    """What one backward pass's products leave for the gradient of the operand that they share, by the pass's number:
-    passes over one graph (again, or from two threads) do not meet."""
-
-    __slots__ = ("passes",)
-
-    def __init__(self):
-        self.passes = {}
-
-    def add(self, *part):
-        self.passes.setdefault(torch._C._current_graph_task_id(), []).append(part)
-
-    def take(self):
-        return self.passes.pop(torch._C._current_graph_task_id(), [])
-
-
 class _Readers(torch.autograd.Function):
     """The place in the graph where the gradients of an operand's contractions meet.
 
     sum_i dz_i y_i^T is formed at once, in 32 bits, and rounded once; autograd
     would add the contractions' rounded gradients one by one.  A contraction's
-    backward leaves its factors in the box and hands on no gradient."""
+    backward leaves its factors in the box, under the number of the backward
+    pass, and hands on no gradient."""
 
     @staticmethod
     def forward(ctx, x, box):
@@ -303,40 +280,22 @@ class _Readers(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, _):
-        parts = ctx.box.take()
-        here = torch.cuda.current_stream(parts[0][2].device) if parts and parts[0][2].is_cuda else None
-        for _, _, dz, y, stream in parts:
-            if stream != here:  # its backward ran on its own stream
-                here.wait_stream(stream)
-                dz.record_stream(here)
-                y.record_stream(here)
-        groups = {}
-        for plan, native, dz, y, _ in parts:
-            groups.setdefault((native, plan.x_order, plan.x_shape, plan.gemm[0], plan.gemm[3]), []).append((plan, dz, y))
+        parts = ctx.box.pop(torch._C._current_graph_task_id(), [])
         total = None
-        for (native, *_), group in groups.items():
-            dx = _operand_grad(native, group)
+        for equation, dz, y in parts:
+            wide = torch.promote_types(dz.dtype, torch.float32) if len(parts) > 1 else dz.dtype
+            dx = _operand_grad(equation, dz.to(wide), y.to(wide))
             total = dx if total is None else total + dx
-        return total, None
+        return None if total is None else total.to(parts[0][1].dtype), None
 
 
-def _operand_grad(native, group):
-    """sum of dz y^T over contractions of one operand alike but for their other axes."""
-    plan = group[0][0]
-    if native:
-        dx = gemm.native_bmm_sum([(p.product_of(dz), p.operand_y(y).transpose(1, 2)) for p, dz, y in group])
-        return _moved(dx.view(plan.x_shape), None if plan.x_order is None else _inverse(plan.x_order))
-    total, dtype = None, group[0][1].dtype
-    wide = torch.promote_types(dtype, torch.float32) if len(group) > 1 else dtype
-    for p, dz, y in group:
-        (ex, ey), ez = p.equation.split("->")[0].split(","), p.equation.split("->")[1]
-        dx = contract(f"{ez},{ey}->{ex}", dz.to(wide), y.to(wide))
-        total = dx if total is None else total + dx
-    return total.to(dtype)
+def _operand_grad(equation, dz, y):
+    (ex, ey), ez = equation.split("->")[0].split(","), equation.split("->")[1]
+    return contract(f"{ez},{ey}->{ex}", dz, y)
 
 
 class _Contraction8(torch.autograd.Function):
-    """x y with x kept in 8 bits.
+    """x y with x kept in 8 bits, on torch's own products (the native ones' nodes are in csrc/bindings_saved8.cpp).
 
     ``x`` carries the values.  Its gradient goes to ``place`` (``x`` is detached
     then): its pre-activation's place in the graph where x is a silu, and with a
@@ -345,24 +304,16 @@ class _Contraction8(torch.autograd.Function):
     8 bits and that one's place."""
 
     @staticmethod
-    def forward(ctx, x, place, box, y, plan, native, codes, exps, meta, silu):
+    def forward(ctx, x, place, box, y, equation, codes, exps, meta, silu):
         ctx.set_materialize_grads(False)
-        ctx.plan, ctx.native, ctx.meta, ctx.silu, ctx.box = plan, native, meta, silu, box
-        mod = _native.require() if native else None
+        ctx.equation, ctx.meta, ctx.silu, ctx.box = equation, meta, silu, box
         if not silu:
             ctx.save_for_backward(y, codes, exps)
-            if native:
-                return plan.result(gemm.native_bmm(plan.operand_x(x), plan.operand_y(y)))
-            return contract(plan.equation, x, y)
-        if native:
-            xv, yv = gemm._prepare(plan.operand_x(x)), gemm._prepare(plan.operand_y(y))
-            a, h_codes, h_exps = mod.gemm_silu8(xv, yv, _native.error_word(x.device))
-            a = plan.result(a)
-        else:
-            wide = torch.promote_types(x.dtype, torch.float32)
-            h = contract(plan.equation, x.to(wide), y.to(wide))
-            a, h_codes, h_exps = _silu_forward(_rows(h) if h.dim() else h.view(1, 1), x.dtype)
-            a = a.view(h.shape)
+            return contract(equation, x, y)
+        wide = torch.promote_types(x.dtype, torch.float32)
+        h = contract(equation, x.to(wide), y.to(wide))
+        a, h_codes, h_exps = _silu_forward(_rows(h) if h.dim() else h.view(1, 1), x.dtype)
+        a = a.view(h.shape)
         ctx.save_for_backward(y, codes, exps, h_codes, h_exps)
         ctx.mark_non_differentiable(h_codes, h_exps)
         return a, _place_of(a), h_codes, h_exps
@@ -371,56 +322,25 @@ class _Contraction8(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad, grad_pre=None, *_):
         y, codes, exps = ctx.saved_tensors[:3]
-        plan, native = ctx.plan, ctx.native
         if grad is not None and ctx.silu:
-            grad = _silu_grad(grad, *ctx.saved_tensors[3:], plan.z_order if native else None)
+            grad = _silu_grad(grad, *ctx.saved_tensors[3:], None)
         if grad_pre is not None:
             grad = grad_pre if grad is None else grad + grad_pre
         if grad is None:
-            return (None,) * 10
-        want_x, want_pre, _, want_y = ctx.needs_input_grad[:4]
+            return (None,) * 9
+        want_x, want_place, _, want_y = ctx.needs_input_grad[:4]
+        dx = dplace = dy = None
         if ctx.box is not None:
             if torch._C._will_engine_execute_node(ctx.next_functions[1][0]):  # the operand's gradient is asked for
-                ctx.box.add(plan, native, grad, y, torch.cuda.current_stream(grad.device) if grad.is_cuda else None)
-            want_x = want_pre = False
-        act, base, order, dtype = ctx.meta
-        dx = dpre = dy = restored = None
-        if native:
-            gz, yv = plan.product_of(grad), plan.operand_y(y)
-            yt = yv.transpose(1, 2)
-            if want_pre and _same_rows(plan, codes, base, order):
-                # (dz y^T) silu'(h^) and silu(h^) from one product
-                gz = gemm._prepare(gz)
-                dpre, restored = _native.require().gemm_silu8_grad(gz, gemm._prepare(yt), codes, exps,
-                                                                   _native.error_word(gz.device))
-                dpre = _moved(dpre.view(plan.x_shape), None if plan.x_order is None else _inverse(plan.x_order))
-            elif want_x or want_pre:
-                dx = _operand_grad(native, [(plan, grad, y)])
-            if want_y:
-                if restored is None:
-                    restored = plan.operand_x(_restore_operand(codes, exps, ctx.meta))
-                # a transposed y (an [out, in] weight) gets its gradient in its own memory order
-                if yv.stride(1) == 1 and yv.size(1) > 1:
-                    dy = gemm.native_bmm(gz.transpose(1, 2), restored).transpose(1, 2)
-                else:
-                    dy = gemm.native_bmm(restored.transpose(1, 2), gz)
-                dy = _moved(dy.reshape(plan.y_shape), None if plan.y_order is None else _inverse(plan.y_order))
-        else:
-            (ex, ey), ez = plan.equation.split("->")[0].split(","), plan.equation.split("->")[1]
-            if want_x or want_pre:
-                dx = _operand_grad(native, [(plan, grad, y)])
-            if want_y:
-                dy = contract(f"{ez},{ex}->{ey}", grad, _restore_operand(codes, exps, ctx.meta))
-        if want_pre and dpre is None:
-            dpre = _silu_grad(dx, codes, exps, order)
-        return dx if want_x else None, dpre, None, dy, None, None, None, None, None, None
-
-
-def _same_rows(plan, codes, base, order):
-    """Whether the pre-activation was quantised in the very rows this product reads."""
-    B, M, _, K = plan.gemm
-    identity = order is None or tuple(order) == tuple(range(len(order)))
-    return identity and plan.x_order is None and codes.shape == (B * M, K) and codes.numel() > 0
+                ctx.box.setdefault(torch._C._current_graph_task_id(), []).append((ctx.equation, grad, y))
+        elif want_x or want_place:
+            dx = _operand_grad(ctx.equation, grad, y)
+            if want_place:
+                dx, dplace = None, _silu_grad(dx, codes, exps, ctx.meta[2])
+        if want_y:
+            (ex, ey), ez = ctx.equation.split("->")[0].split(","), ctx.equation.split("->")[1]
+            dy = contract(f"{ez},{ex}->{ey}", grad, _restore_operand(codes, exps, ctx.meta))
+        return dx, dplace, None, dy, None, None, None, None, None
 
 
 def contract_saved(equation, saved, y, activation=None):
@@ -432,20 +352,32 @@ def contract_saved(equation, saved, y, activation=None):
         raise ValueError(f"a Saved8 operand of {x.dtype} on {x.device} needs the other one alike, "
                          f"not {y.dtype} on {y.device}")
     plan = _product(equation, tuple(x.shape), tuple(y.shape))
-    native = all(plan.gemm) and gemm.eligible(x, y)
+    silu = activation is not None
+    if all(plan.gemm) and gemm.eligible(x, y):
+        mod, err = _native.require(), _native.error_word(x.device)
+        place = saved._pre
+        if place is None and x.requires_grad and torch.is_grad_enabled():
+            place = saved._readers
+            if place is None:
+                place = saved._readers = mod.readers8(x, err)
+        order = () if saved._order is None else saved._order
+        out = mod.contract8(x, place, y, plan.on_kernels, saved.codes, saved.exps, saved._act, saved._base, order,
+                            silu, err)
+        if not silu:
+            return out[0]
+        a, pre, codes, exps = out
+        return Saved8(a, codes, exps, True, plan.z_shape, plan.z_order, pre)
     place, box = saved._pre, None
     if place is None and x.requires_grad and torch.is_grad_enabled():
-        if saved._readers is None:
-            box = _Box()
-            saved._readers = _Readers.apply(x, box), box
-        place, box = saved._readers
-    out = _Contraction8.apply(x if place is None else x.detach(), place, box, y, plan, native, saved.codes,
-                              saved.exps, saved._meta(), activation is not None)
-    if activation is None:
+        if saved._box is None:
+            box = {}
+            saved._box = _Readers.apply(x, box), box
+        place, box = saved._box
+    out = _Contraction8.apply(x if place is None else x.detach(), place, box, y, plan.equation, saved.codes,
+                              saved.exps, saved._meta(), silu)
+    if not silu:
         return out
     a, pre, codes, exps = out
-    if native:
-        return Saved8(a, codes, exps, True, plan.z_shape, plan.z_order, pre)
     return Saved8(a, codes, exps, True, None, None, pre)
 
 
