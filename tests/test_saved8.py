@@ -10,6 +10,7 @@ accumulation (2^-23 a term at most, which the same product bounds).
 import pytest
 import torch
 import torch.distributed as dist
+from dist_harness import run_ranks
 
 import torch_einshard_b200 as es
 from torch_einshard_b200.models.tp_mlp import TPMLP
@@ -522,3 +523,74 @@ def test_shared_operand_captured():
     graph.replay()
     for a, b in zip(out, step()):
         assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------ two ranks
+
+def _sharded_models(ctx):
+    """Values are those of whole operands; gradients those of operands within half a step (1/128 of a block's largest)."""
+    mesh = ctx.mesh((2,), ("tp",))
+    gen = torch.Generator().manual_seed(0)
+    models = [TPMLP(64, 256, mesh, dtype=torch.float32, device="cpu", std=0.1, checkpoint=c) for c in (None, "int8")]
+    x = [torch.randn(2, 24, 64, generator=gen).requires_grad_(True)]
+    x.append(x[0].detach().clone().requires_grad_(True))
+    ys = [m(v) for m, v in zip(models, x)]
+    assert (ys[0] - ys[1]).abs().max() <= 2.0 ** -20 * ys[0].abs().max()
+    for y in ys:
+        y.square().sum().backward()
+    assert (x[0].grad - x[1].grad).norm() <= 0.03 * x[0].grad.norm()
+    for p, q in zip(models[0].parameters(), models[1].parameters()):
+        assert (p.grad - q.grad).norm() <= 0.03 * p.grad.norm()
+
+    cfg = TransformerConfig(layers=2, d=64, heads=4, mlp=128, vocab=97, seq=16, dtype=torch.float32, norm="sandwich")
+    tokens = torch.randint(0, 97, (2, 16), generator=gen)
+    losses, grads = [], []
+    for mode in (False, "int8"):
+        model = TPTransformer(cfg, mesh, device="cpu", checkpoint=mode)
+        loss = model(tokens, tokens.roll(-1, 1))
+        loss.backward()
+        losses.append(loss.item())
+        grads.append([p.grad for p in model.parameters()])
+    assert abs(losses[0] - losses[1]) <= 1e-5 * abs(losses[0])
+    for p, q in zip(*grads):
+        assert (p - q).norm() <= 0.05 * p.norm() + 1e-6
+
+
+def _sharded_equations(ctx):
+    """Column parallel contractions of one operand are local, like those of a plain one: dx is the rank's share."""
+    mesh = ctx.mesh((2,), ("tp",))
+    gen = torch.Generator().manual_seed(1)
+    x = torch.randn(2, 6, 32, generator=gen).requires_grad_(True)
+    w = [torch.randn(n, 32, generator=gen) for n in (16, 24)]
+    local = [v.chunk(2, 0)[ctx.rank].clone().requires_grad_(True) for v in w]
+    kept = es.checkpoint8(x)
+    ys = [es.einshard("b s c, n/tp c -> b s n/tp", kept, v, mesh=mesh) for v in local]
+    dy = [torch.randn(2, 6, v.shape[0], generator=gen) for v in w]
+    mine = [d.chunk(2, -1)[ctx.rank].contiguous() for d in dy]
+    dx, *dw = torch.autograd.grad(ys, [x, *local], mine)
+    with torch.no_grad():
+        want = sum(d.double() @ v.double() for d, v in zip(mine, local))
+        size = sum(d.double().abs() @ v.double().abs() for d, v in zip(mine, local))
+    assert ((dx.double() - want).abs() <= size * 21 * 2.0 ** -24).all()  # 20 products and their sum
+    restored = kept.restore().double()
+    for g, d in zip(dw, mine):
+        full = torch.einsum("bsn,bsc->nc", d.double(), restored)
+        bound = torch.einsum("bsn,bsc->nc", d.double().abs(), restored.abs())
+        assert ((g.double() - full).abs() <= bound * 13 * 2.0 ** -24).all()
+
+    # a plan with communication: the same values and operand gradient as for the plain operand
+    for formula in ("b s c, n/tp c -> b s n", "b s c, n c -> b s n/tp"):
+        got = []
+        for operand in (x, es.checkpoint8(x)):
+            v = (local[0] if "n/tp c" in formula else w[0]).detach().clone().requires_grad_(True)
+            y = es.einshard(formula, operand, v, mesh=mesh)
+            d = dy[0] if formula.endswith("s n") else mine[0]
+            got.append((y.detach(), *torch.autograd.grad(y, [x, v], d)))
+        assert torch.equal(got[0][0], got[1][0])
+        assert (got[0][1] - got[1][1]).norm() <= 2.0 ** -20 * got[0][1].norm()
+        assert (got[0][2] - got[1][2]).norm() <= 0.03 * got[0][2].norm()
+
+
+@pytest.mark.parametrize("body", [_sharded_models, _sharded_equations])
+def test_two_ranks(body):
+    run_ranks(body, world_size=2)
