@@ -528,3 +528,48 @@ def test_transformer_policy_step(one_rank_mesh):
         assert all(torch.isfinite(g).all() for g in grads[-1])
     for a, b in zip(*grads):
         assert (a - b).norm() <= 0.06 * a.norm() + 1e-6
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("base", [-1e10, 1e10, -1e9, -3.0e7, 5.0e6, -5.0e6, 2.9e6, -2.9e6, 2907269.0, -2907270.0, 1e4])
+def test_rows_far_from_zero(device, dtype, base):
+    """A row is known by its differences: mask values and offsets of any size leave them alone.
+
+    The differences of these logits are exact in 32 bits; each is scaled with one rounding, and the exponentials are
+    2^-21 off."""
+    gen = torch.Generator().manual_seed(3)
+    z = torch.full((1, 6, 301), base, dtype=torch.float64)
+    z[0, 1] += torch.randn(301, generator=gen).double()
+    z[0, 2] += 4 * torch.randn(301, generator=gen).double()
+    z[0, 3, :150] = 0.0
+    z[0, 4] = torch.randn(301, generator=gen).double()
+    z[0, 4, 7] = base
+    z[0, 5, 9:] = -1e30
+    z = z.to(dtype)
+    t = make(device, dtype, 1, 6, 301)
+    t["logits"] = z.to(device)
+    t["ids"] = torch.tensor([[3, 5, 7, 11, 13, 2]], device=device)
+    want = torch.log_softmax(z.double(), -1).gather(-1, t["ids"].cpu()[..., None])[..., 0]
+    kept = want.abs() < 200  # further down 32 bits hold no ratio: old_logp's own rounding is more than 1e-5
+    t["mask"] = kept.to(device)
+    want = torch.where(kept, want, 0)
+    t["old_logp"] = (want + 0.1).float().to(device)
+    t["ref_logp"] = (want - 0.1).float().to(device)
+    logits = t["logits"].requires_grad_(True)
+    r = es.einpolicy("b s v", logits, t["ids"], axis="v", advantages=t["advantages"], old_logp=t["old_logp"],
+                     mask=t["mask"], ref_logp=t["ref_logp"], kl=0.1)
+    far = torch.where(kept, z.double().amax(-1) - z.double().gather(-1, t["ids"].cpu()[..., None])[..., 0], 0)
+    assert ((r.logp.double().cpu() - want).abs() <= 2.0 ** -19 + 2.0 ** -22 * (far + want.abs())).all()
+    (grad,) = torch.autograd.grad(r.loss, logits)
+    ratio = torch.exp(want - t["old_logp"].double().cpu())
+    adv = t["advantages"].double().cpu()
+    slope = torch.where(ratio * adv <= ratio.clamp(0.8, 1.2) * adv, -ratio * adv, 0)
+    slope = (slope + 0.1 * (1 - torch.exp(t["ref_logp"].double().cpu() - want))) / kept.sum() * kept
+    hit = torch.zeros(1, 6, 301, dtype=torch.float64).scatter_(-1, t["ids"].cpu()[..., None], 1.0)
+    p = torch.softmax(z.double(), -1)
+    exact = slope[..., None] * (hit - p)
+    # ratio (at most 1.2) and p follow the log-probability's error
+    err = 2.0 ** -18 + 2.0 ** -21 * (far + want.abs())[..., None]
+    bound = half_step(dtype) * exact.abs() + err * (hit + p) * (1.2 * adv.abs() + 0.2)[..., None] + 1e-30
+    assert ((grad.double().cpu() - exact).abs() <= bound).all()

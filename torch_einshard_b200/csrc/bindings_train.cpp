@@ -367,23 +367,22 @@ PolicyArgs policy_args(const at::Tensor& logits, const at::Tensor& ids, const Op
   a.adv_per_sequence = per_sequence;
   a.least = 1.0 - lo;
   a.most = 1.0 + hi;
-  a.kl = static_cast<float>(kl);
-  a.inv_temp = static_cast<float>(1.0 / temperature);
+  a.kl = kl;
+  a.inv_temp = 1.0 / temperature;
   a.reduction = static_cast<int>(reduction);
   a.weight = static_cast<float>(weight);
   a.sms = sms_of(logits);
   return a;
 }
 
-PolicyState policy_state(const at::Tensor& terms, const at::Tensor& norm, const at::Tensor& share) {
+PolicyState policy_state(const at::Tensor& terms, const at::Tensor& share) {
   PolicyState s;
   s.terms = reinterpret_cast<float4*>(terms.data_ptr<float>());
-  s.norm = reinterpret_cast<float2*>(norm.data_ptr<float>());
   s.share = share.data_ptr<float>();
   return s;
 }
 
-// (loss, KL, clipped share, logp, terms, norm, token shares) and, with `gradient`, that of the logits and its factors
+// (loss, KL, clipped share, logp, terms, token shares) and, with `gradient`, that of the logits and its factors
 std::vector<at::Tensor> policy_forward_op(const at::Tensor& logits, const at::Tensor& ids, const Opt& mask,
                                           const Opt& old, const Opt& ref, const at::Tensor& adv, int64_t length,
                                           double lo, double hi, double kl, double temperature, int64_t reduction,
@@ -395,20 +394,20 @@ std::vector<at::Tensor> policy_forward_op(const at::Tensor& logits, const at::Te
   TORCH_CHECK(a.tokens > 0, "einshard policy loss: no tokens");
   at::Tensor loss = at::empty({}, f32), kl_out = at::empty({}, f32), clipped = at::empty({}, f32);
   at::Tensor logp = at::empty({a.tokens}, f32), terms = at::empty({a.tokens, 4}, f32);
-  at::Tensor norm = at::empty({a.tokens, 2}, f32), shares = at::empty({sequences}, f32);
+  at::Tensor shares = at::empty({sequences}, f32);
   at::Tensor sums = at::empty({policy_sum_blocks(a.tokens), 3}, f32.dtype(at::kDouble));
-  PolicyState s = policy_state(terms, norm, shares);
+  PolicyState s = policy_state(terms, shares);
   s.logp = logp.data_ptr<float>();
   s.sums = reinterpret_cast<PolicySums*>(sums.data_ptr<double>());
   s.loss = loss.data_ptr<float>();
   s.kl = kl_out.data_ptr<float>();
   s.clipped = clipped.data_ptr<float>();
-  std::vector<at::Tensor> out{loss, kl_out, clipped, logp, terms, norm, shares};
+  std::vector<at::Tensor> out{loss, kl_out, clipped, logp, terms, shares};
   if (gradient) {
     out.push_back(at::empty(logits.sizes(), logits.options()));
     out.push_back(at::empty({a.tokens}, f32));
-    s.dlogits = out[7].data_ptr();
-    s.factors = out[8].data_ptr<float>();
+    s.dlogits = out[6].data_ptr();
+    s.factors = out[7].data_ptr<float>();
   }
   int launches = 0;
   const int rc = policy_forward(a, s, at::cuda::getCurrentCUDAStream(), &launches);
@@ -420,7 +419,7 @@ std::vector<at::Tensor> policy_forward_op(const at::Tensor& logits, const at::Te
 at::Tensor policy_backward_op(const at::Tensor& grad, const at::Tensor& logits, const at::Tensor& ids,
                               const Opt& mask, const Opt& old, const Opt& ref, const at::Tensor& adv, int64_t length,
                               double lo, double hi, double kl, double temperature, int64_t reduction, double weight,
-                              const at::Tensor& terms, const at::Tensor& norm, const at::Tensor& shares,
+                              const at::Tensor& terms, const at::Tensor& shares,
                               const Opt& kept, const Opt& factors) {
   const c10::cuda::CUDAGuard guard(logits.device());
   const PolicyArgs a = policy_args(logits, ids, mask, old, ref, adv, length, lo, hi, kl, temperature, reduction, weight);
@@ -428,13 +427,12 @@ at::Tensor policy_backward_op(const at::Tensor& grad, const at::Tensor& logits, 
               "einshard policy loss: fp32 gradient of the loss");
   TORCH_CHECK(a.tokens > 0, "einshard policy loss: no tokens");
   per_token(terms, logits, 4 * a.tokens, at::kFloat, "terms");
-  per_token(norm, logits, 2 * a.tokens, at::kFloat, "norms");
   per_token(shares, logits, a.tokens / length, at::kFloat, "token shares");
   TORCH_CHECK(kept.has_value() == factors.has_value(), "einshard policy loss: a kept gradient has factors");
   per_token(kept, logits, a.tokens * a.vocab, logits.scalar_type(), "kept gradient");
   per_token(factors, logits, a.tokens, at::kFloat, "factors");
   at::Tensor out = kept.has_value() ? *kept : at::empty(logits.sizes(), logits.options());
-  PolicyState s = policy_state(terms, norm, shares);
+  PolicyState s = policy_state(terms, shares);
   s.dlogits = out.data_ptr();
   s.factors = factors.has_value() ? factors->data_ptr<float>() : nullptr;
   counted(policy_backward(a, s, grad.data_ptr<float>(), at::cuda::getCurrentCUDAStream()), "policy loss backward");
@@ -457,10 +455,10 @@ struct PolicyFunction : public torch::autograd::Function<PolicyFunction> {
     const at::Tensor rows = rows_of(logits);
     auto r = policy_forward_op(rows, ids, mask, old, ref, adv, length, lo, hi, kl, temperature, reduction, weight, true);
     ctx->set_materialize_grads(false);
-    ctx->save_for_backward({logits, ids, none(mask), none(old), none(ref), adv, r[4], r[5], r[6]});
+    ctx->save_for_backward({logits, ids, none(mask), none(old), none(ref), adv, r[4], r[5]});
     ctx->saved_data["conf"] = c10::ivalue::Tuple::create({length, lo, hi, kl, temperature, reduction, weight});
-    ctx->saved_data["kept"] = r[7];
-    ctx->saved_data["factors"] = r[8];
+    ctx->saved_data["kept"] = r[6];
+    ctx->saved_data["factors"] = r[7];
     ctx->saved_data["captured"] = capturing();
     ctx->mark_non_differentiable({r[1], r[2], r[3]});
     return {r[0], r[1], r[2], r[3]};
@@ -486,7 +484,7 @@ struct PolicyFunction : public torch::autograd::Function<PolicyFunction> {
       at::AutoDispatchBelowAutograd below;
       found[0] = policy_backward_op(grads[0].contiguous(), rows_of(s[0]), s[1], some(s[2]), some(s[3]), some(s[4]), s[5],
                                     conf[0].toInt(), conf[1].toDouble(), conf[2].toDouble(), conf[3].toDouble(),
-                                    conf[4].toDouble(), conf[5].toInt(), conf[6].toDouble(), s[6], s[7], s[8], kept,
+                                    conf[4].toDouble(), conf[5].toInt(), conf[6].toDouble(), s[6], s[7], kept,
                                     factors)
                      .view(s[0].sizes());
     }

@@ -35,14 +35,11 @@ namespace es {
 namespace {
 
 constexpr int kUnroll = 4;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kRun = 128;  // tokens whose terms a block adds
+constexpr double kLog2e = 1.4426950408889634;
+constexpr float kLn2 = 0.6931471805599453f;
 
-// The larger one, NaN if either is.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
+__device__ __forceinline__ float scale_of(const PolicyArgs& a) { return static_cast<float>(a.inv_temp * kLog2e); }
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -50,58 +47,56 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
-// Logits beyond this take differences before they are scaled (their products with c could overflow).
-constexpr float kHuge = 1e30f;
+// Sums are relative to 2^q, q the whole number above m c (c = log2(e) / T): a larger maximum scales them by an exact
+// power of two, and z c - q takes one FMA.  Where m c is so large that its rounding would show (rows of mask values),
+// q is infinite and sums are relative to 2^(m c), of differences that are formed before they are scaled.
+constexpr float kLarge = 4194304.0f;
 
-// Running maximum and sum of 2^((z - m) c).
+__device__ __forceinline__ float base_of(float m, float c) {
+  const float p = m * c;
+  return fabsf(p) < kLarge ? ceilf(p) : INFINITY;
+}
+
+__device__ __forceinline__ float power_of(float z, float m, float q, float c) {
+  return exp2_fast(q == INFINITY ? (z - m) * c : fmaf(z, c, -q));
+}
+
+// The factor that takes a sum from (m, q) to a larger maximum's (m2, q2).
+__device__ __forceinline__ float rebased(float m, float q, float m2, float q2, float c) {
+  if (m == -INFINITY) return 0.0f;  // nothing summed yet but zeros
+  if (q != INFINITY && q2 != INFINITY)
+    return __int_as_float(static_cast<int>(fmaxf(q - q2, -127.0f) + 127.0f) << 23);
+  if (q == INFINITY && q2 == INFINITY) return exp2_fast((m - m2) * c);
+  return exp2_fast(q == INFINITY ? fmaf(m, c, -q2) : fmaf(-m2, c, q));
+}
+
+// Largest logit and sum of powers.
 struct Running {
   float m, s;
-  __device__ __forceinline__ static float base(float m) { return m == -INFINITY ? 0.0f : m; }
-  __device__ __forceinline__ void add(float z, float c) { merge(z, 1.0f, c); }
-  __device__ __forceinline__ void merge(float m2, float s2, float c) {
-    const float top = max_nan(m, m2);
-    const float b = base(top);
-    s = s * exp2_fast((m - b) * c) + s2 * exp2_fast((m2 - b) * c);
-    m = top;
-  }
   // Joined over the warp: the maximum as an integer of the same order (a NaN ends up in s), one scaling, the sum.
   __device__ __forceinline__ void over_warp(float c) {
     const int bits = __float_as_int(m);
     const int top = __reduce_max_sync(0xffffffffu, bits ^ ((bits >> 31) & 0x7fffffff));
     const float largest = __int_as_float(top ^ ((top >> 31) & 0x7fffffff));
-    s = warp_sum(s * exp2_fast((m - base(largest)) * c));
+    s = warp_sum(s * rebased(m, base_of(m, c), largest, base_of(largest, c), c));
     m = largest;
   }
 };
 
-// The same over a thread's chunks.  2^(z c - q) takes one FMA before the
-// exponential, exact up to its one rounding for any q; q is m c rounded, and
-// close() makes up for that rounding.
+// The same over a thread's chunks.
 struct ChunkSum {
   float m = -INFINITY, q = 0.0f, s = 0.0f;
   __device__ __forceinline__ void raise(float top, float c) {
     if (top > m) {
-      const float next = fabsf(top) < kHuge ? top * c : 0.0f;
-      if (m == -INFINITY) {
-        // nothing summed yet but zeros
-      } else if (fabsf(m) < kHuge && fabsf(top) < kHuge) {
-        s *= exp2_fast(q - next);
-      } else {
-        close(c);
-        s *= exp2_fast((m - top) * c);
-        if (fabsf(top) < kHuge) s *= exp2_fast(fmaf(top, c, -next));
-      }
+      const float next = base_of(top, c);
+      s *= rebased(m, q, top, next, c);
       m = top;
       q = next;
     }
   }
-  // s relative to 2^(m c) exactly
-  __device__ __forceinline__ void close(float c) {
-    if (fabsf(m) < kHuge) s *= exp2_fast(-fmaf(m, c, -q));
-  }
-  __device__ __forceinline__ Running total(float c) {
-    close(c);
-    return {m, s};
+  __device__ __forceinline__ void add(float z, float c) {
+    raise(z, c);
+    s += power_of(z, m, q, c);
   }
 };
 
@@ -113,27 +108,26 @@ __device__ __forceinline__ int head_of(const T* row, int n) {
   return head < n ? head : n;
 }
 
-// Eight columns from j0 of a token's gradient k (1[j = id] - 2^((z_j - norm.x) c - norm.y)).
+// Eight columns from j0 of a token's gradient k (1[j = id] - p_j), with p_j from the row's maximum and sum.
 struct GradientRow {
   float k, c, off, factor, m;
   int id;
-  bool huge;
-  __device__ __forceinline__ GradientRow(float k_, float2 norm, int id_, float c_) : k(k_), c(c_), m(norm.x), id(id_) {
-    huge = !(fabsf(norm.x) < kHuge);
-    // 2^(z c - q) and a factor for what the rounding of q = m c left, with the sum's
-    const float q = huge ? 0.0f : norm.x * c;
+  bool large;
+  __device__ __forceinline__ GradientRow(float k_, Running row, int id_, float c_) : k(k_), c(c_), m(row.m), id(id_) {
+    const float q = base_of(row.m, c);
+    large = q == INFINITY;
     off = -q;
-    factor = -k * exp2_fast((huge ? 0.0f : -fmaf(norm.x, c, -q)) - norm.y);
+    factor = -k / row.s;
   }
   __device__ __forceinline__ float minus_p(float z) const {
-    return factor * exp2_fast(huge ? (z - m) * c : fmaf(z, c, off));
+    return factor * exp2_fast(large ? (z - m) * c : fmaf(z, c, off));
   }
   // (scalar arithmetic: the exponentials' results would have to be moved into pairs)
   template <typename T>
   __device__ __forceinline__ void put(T* out, int j0, const Raw8<T>& raw) const {
     float z[8];
     unpack8(raw, z);
-    if (huge) {  // uniform
+    if (large) {  // uniform
 #pragma unroll
       for (int e = 0; e < 8; ++e) z[e] = minus_p(z[e]);
     } else {
@@ -153,12 +147,12 @@ struct GradientRow {
 
 // A token's gradient row; zeros for k = 0 without reading the logits.
 template <typename T>
-__device__ __forceinline__ void gradient_row(const T* row, T* out, int vocab, float k, float2 norm, int id, float c) {
+__device__ __forceinline__ void gradient_row(const T* row, T* out, int vocab, float k, Running sum, int id, float c) {
   const bool zero = k == 0.0f;  // NaN is not zero
   const int head = head_of(out, vocab);
   const bool vec = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
   const int chunks = (vocab - head) / 8, threads = static_cast<int>(blockDim.x), tid = static_cast<int>(threadIdx.x);
-  const GradientRow g(k, norm, id, c);
+  const GradientRow g(k, sum, id, c);
   auto one = [&](int j) { out[j] = from_float<T>(zero ? 0.0f : g.one(to_float<T>(row[j]), j)); };
   if (zero) {
     const Pair nil[4] = {0ull, 0ull, 0ull, 0ull};
@@ -224,56 +218,46 @@ struct Inputs {
   float z, adv, old, ref, share;
 };
 
-template <typename T>
+template <bool kGrad, typename T>
 __device__ __forceinline__ Inputs inputs_of(const PolicyArgs& a, const PolicyState& o, const T* row, long long t, int id) {
   Inputs in{__uint_as_float(0x7fc00000u), 0.0f, 0.0f, 0.0f, 0.0f};
-  if (threadIdx.x == 0) {
+  if (threadIdx.x == 0 && id >= 0) in.z = to_float<T>(row[id]);  // an id outside the vocabulary makes the loss NaN
+  if (kGrad && threadIdx.x == 0) {
     in.share = share_of(a, o, t);
     in.adv = a.adv[a.adv_per_sequence ? sequence_of(a, t) : t];
     if (a.old != nullptr) in.old = a.old[t];
     if (a.ref != nullptr) in.ref = a.ref[t];
-    if (id >= 0) in.z = to_float<T>(row[id]);  // an id outside the vocabulary makes the loss NaN
   }
   return in;
 }
 
-// The token's terms from its row's maximum and sum: loss, KL, clipped, slope.
-__device__ __forceinline__ float4 terms_of(const PolicyArgs& a, const Inputs& in, float m, float s, float* logp) {
-  const float lp = (in.z - m) * a.inv_temp - logf(s);
+// The derivative of the token's loss by its log-probability (without weights).
+__device__ __forceinline__ float slope_of(const PolicyArgs& a, const Inputs& in, const Running& r, float c) {
+  const float q = base_of(r.m, c);
+  const float d = q == INFINITY ? (in.z - r.m) * c : fmaf(in.z, c, -q);
+  const float lp = d * kLn2 - logf(r.s);
   const float ratio = expf(lp - (a.old != nullptr ? in.old : lp));
   const float kept = fminf(fmaxf(ratio, static_cast<float>(a.least)), static_cast<float>(a.most));
-  const float s1 = ratio * in.adv, s2 = kept * in.adv;
-  const bool clipped = s1 > s2;
-  float loss = 0.0f, slope = 0.0f, kl = 0.0f;
-  if (in.adv != 0.0f) {
-    // a clipped token's ratio is the border itself: its rounding to 32 bits would be every clipped token's error
-    loss = clipped ? static_cast<float>(-(ratio < 1.0f ? a.least : a.most) * in.adv) : -s1;
-    slope = clipped ? 0.0f : -s1;
-  }
-  if (a.ref != nullptr) {
-    const float away = in.ref - lp;
-    const float rise = expm1f(away);
-    kl = rise - away;
-    loss += a.kl * kl;
-    slope -= a.kl * rise;
-  }
-  *logp = lp;
-  return make_float4(loss, kl, clipped ? 1.0f : 0.0f, slope);
+  const float s1 = ratio * in.adv;
+  float slope = in.adv == 0.0f || s1 > kept * in.adv ? 0.0f : -s1;
+  if (a.ref != nullptr) slope -= a.kl * expm1f(in.ref - lp);
+  return slope;
 }
 
 __device__ __forceinline__ float coefficient(const PolicyArgs& a, float share, float slope) {
-  return slope == 0.0f ? 0.0f : a.weight * share * slope * a.inv_temp;
+  return slope == 0.0f ? 0.0f : a.weight * share * slope * static_cast<float>(a.inv_temp);
 }
 
 // What a token leaves behind for a row's blocks: shared words.
 struct RowWords {
   float2 red[32];
-  float2 norm;
+  Running sum;
   float k;
 };
 
-// The block's maxima and sums joined, the token's terms stored; the row's norm and the gradient's coefficient go to
-// w (behind a barrier of the caller's).
+// The block's maxima and sums joined and stored with the logit; with kGrad the slope, too, and the row's sum and the
+// gradient's coefficient go to w (behind a barrier of the caller's).
+template <bool kGrad>
 __device__ __forceinline__ void finish_token(const PolicyArgs& a, const PolicyState& o, RowWords& w, Running r, float c,
                                              const Inputs& in, long long t) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -287,23 +271,12 @@ __device__ __forceinline__ void finish_token(const PolicyArgs& a, const PolicySt
   r.s = v.y;
   r.over_warp(c);
   if (lane != 0) return;
-  float lp;
-  const float4 terms = terms_of(a, in, r.m, r.s, &lp);
-  const float2 norm = make_float2(r.m, log2f(r.s));
-  o.logp[t] = lp;
-  o.terms[t] = terms;
-  o.norm[t] = norm;
-  if (o.factors != nullptr) o.factors[t] = 1.0f;
-  w.norm = norm;
-  w.k = coefficient(a, in.share, terms.w);
-}
-
-__device__ __forceinline__ void masked_token(const PolicyState& o, long long t) {
-  if (threadIdx.x != 0) return;
-  o.logp[t] = 0.0f;
-  o.terms[t] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  o.norm[t] = make_float2(0.0f, 0.0f);
-  if (o.factors != nullptr) o.factors[t] = 1.0f;
+  const float slope = kGrad ? slope_of(a, in, r, c) : 0.0f;
+  o.terms[t] = make_float4(in.z, r.m, r.s, slope);
+  if (!kGrad) return;
+  o.factors[t] = 1.0f;
+  w.sum = r;
+  w.k = coefficient(a, in.share, slope);
 }
 
 // Exponentials of kCount chunks of eight under one maximum.
@@ -314,7 +287,7 @@ __device__ __forceinline__ void add_chunks(ChunkSum& r, const Raw8<T> (&raw)[kCo
   for (int u = 1; u < kCount; ++u) largest = fmaxf(largest, largest_of(raw[u]));
   r.raise(largest, c);
   float s[2] = {0.0f, 0.0f};
-  if (r.m == -INFINITY || fabsf(r.m) < kHuge) {
+  if (r.q != INFINITY) {
 #pragma unroll
     for (int u = 0; u < kCount; ++u) {
       float z[8];
@@ -339,7 +312,7 @@ template <typename T, bool kGrad>
 __global__ void __maxnreg__(kGrad && sizeof(T) == 2 ? 40 : 64)
     policy_rows_kernel(const PolicyArgs a, const PolicyState o, const long long run) {
   __shared__ RowWords w;
-  const float c = a.inv_temp * kLog2e;
+  const float c = scale_of(a);
   const int threads = static_cast<int>(blockDim.x), tid = static_cast<int>(threadIdx.x);
   const int vocab = static_cast<int>(a.vocab);
   const long long last = min(a.tokens, (blockIdx.x + 1) * run);
@@ -347,12 +320,17 @@ __global__ void __maxnreg__(kGrad && sizeof(T) == 2 ? 40 : 64)
     const T* row = static_cast<const T*>(a.logits) + t * a.ld;
     T* out = kGrad ? static_cast<T*>(o.dlogits) + t * a.vocab : nullptr;
     if (a.mask != nullptr && !a.mask[t]) {  // uniform
-      masked_token(o, t);
-      if (kGrad) gradient_row(row, out, vocab, 0.0f, make_float2(0.0f, 0.0f), -1, c);
+      if (kGrad) {
+        if (tid == 0) {
+          o.terms[t] = make_float4(0.0f, 0.0f, 1.0f, 0.0f);
+          o.factors[t] = 1.0f;
+        }
+        gradient_row(row, out, vocab, 0.0f, {0.0f, 1.0f}, -1, c);
+      }
       continue;
     }
     const int id = in_vocabulary(a.ids[t], a.vocab);
-    const Inputs in = inputs_of(a, o, row, t, id);
+    const Inputs in = inputs_of<kGrad>(a, o, row, t, id);
     const int head = head_of(row, vocab);
     const T* body = row + head;
     const int chunks = (vocab - head) / 8;
@@ -371,15 +349,14 @@ __global__ void __maxnreg__(kGrad && sizeof(T) == 2 ? 40 : 64)
       const Raw8<T> raw[1] = {load(p)};
       add_chunks(sum, raw, c);
     }
-    Running r = sum.total(c);
     // the ends of the row
     const int tail = vocab - head - chunks * 8;
-    if (tid < head) r.add(to_float<T>(row[tid]), c);
-    if (tid < tail) r.add(to_float<T>(body[chunks * 8 + tid]), c);
-    finish_token(a, o, w, r, c, in, t);
+    if (tid < head) sum.add(to_float<T>(row[tid]), c);
+    if (tid < tail) sum.add(to_float<T>(body[chunks * 8 + tid]), c);
+    finish_token<kGrad>(a, o, w, {sum.m, sum.s}, c, in, t);
     if (kGrad) {
       __syncthreads();
-      gradient_row(row, out, vocab, w.k, w.norm, id, c);
+      gradient_row(row, out, vocab, w.k, w.sum, id, c);
     }
   }
 }
@@ -449,15 +426,13 @@ __global__ void __launch_bounds__(1024) policy_shares_kernel(const PolicyArgs a,
   }
 }
 
-// Sum over the block of 1024 threads, in its first thread.  In 64 bits: terms of
-// both signs cancel in the loss, and at 12288 tokens 32-bit sums were as far off as
-// all the log-probabilities together.
+// Sum over a block, in its first thread.
 __device__ __forceinline__ PolicySums block_total(PolicySums s, PolicySums* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   s = {warp_sum(s.loss), warp_sum(s.kl), warp_sum(s.clipped)};
   if (lane == 0) red[warp] = s;
   __syncthreads();
-  s = red[lane];
+  s = lane < static_cast<int>(blockDim.x >> 5) ? red[lane] : PolicySums{0.0, 0.0, 0.0};
   return {warp_sum(s.loss), warp_sum(s.kl), warp_sum(s.clipped)};
 }
 
@@ -467,27 +442,44 @@ __device__ __forceinline__ void store_total(const PolicyArgs& a, const PolicySta
   *o.clipped = static_cast<float>(s.clipped);
 }
 
-// Loss, KL and clipped share: every block a run of tokens, the only (kLast) one the scalars.
+// A token's terms from what its row left, in 64 bits: terms of both signs cancel in the loss, and what 32 bits lose
+// in a log-probability has one sign for all tokens (at 12288 tokens 3e-5 of a loss of 10 to 100; 1e-6 like this).
+// kExpLow is what the row's exponentials are too small by on the average, measured over whole powers of two.
+__device__ __forceinline__ PolicySums terms_of(const PolicyArgs& a, const PolicyState& o, long long t, double* logp) {
+  constexpr double kExpLow = 5.05e-8;
+  const float4 row = o.terms[t];  // logit, largest logit, sum
+  const float c = scale_of(a);
+  const float q = base_of(row.y, c);
+  const double z = row.x, d = q == INFINITY ? (z - row.y) * c : z * c - q;
+  const double lp = d / kLog2e - log(static_cast<double>(row.z)) - kExpLow;
+  const double ratio = a.old != nullptr ? exp(lp - a.old[t]) : (lp == lp ? 1.0 : lp);
+  const double adv = a.adv[a.adv_per_sequence ? sequence_of(a, t) : t];
+  const double s1 = ratio * adv, s2 = fmin(fmax(ratio, a.least), a.most) * adv;
+  PolicySums r{0.0, 0.0, s1 > s2 ? 1.0 : 0.0};
+  if (adv != 0.0) r.loss = s1 > s2 ? -s2 : -s1;
+  if (a.ref != nullptr) {
+    const double away = a.ref[t] - lp;
+    r.kl = expm1(away) - away;
+    r.loss += a.kl * r.kl;
+  }
+  *logp = lp;
+  return r;
+}
+
+// Loss, KL and clipped share: a token a thread, every block kRun of them, the only one (kLast) the scalars.
 template <bool kLast>
-__global__ void __launch_bounds__(1024) policy_sum_kernel(const PolicyArgs a, const PolicyState o, long long run) {
+__global__ void __launch_bounds__(kRun) policy_sum_kernel(const PolicyArgs a, const PolicyState o) {
   __shared__ PolicySums red[32];
-  PolicySums s = {0.0, 0.0, 0.0};
-  const long long last = min(a.tokens, (blockIdx.x + 1) * run);
-  // eight tokens a thread in flight
-  for (long long t0 = blockIdx.x * run + threadIdx.x; t0 < last; t0 += 8 * 1024) {
-    float4 v[8];
-    float f[8];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const long long t = t0 + u * 1024;
-      v[u] = t < last ? o.terms[t] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // zeros where masked, too
-      f[u] = t < last ? share_of(a, o, t) : 0.0f;
+  PolicySums s{0.0, 0.0, 0.0};
+  const long long t = static_cast<long long>(blockIdx.x) * kRun + threadIdx.x;
+  if (t < a.tokens) {
+    double lp = 0.0;
+    if (a.mask == nullptr || a.mask[t]) {
+      s = terms_of(a, o, t, &lp);
+      const double share = share_of(a, o, t);
+      s = {share * s.loss, share * s.kl, share * s.clipped};
     }
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      const double share = f[u];
-      s.loss += share * v[u].x, s.kl += share * v[u].y, s.clipped += share * v[u].z;
-    }
+    o.logp[t] = static_cast<float>(lp);
   }
   s = block_total(s, red);
   if (threadIdx.x != 0) return;
@@ -497,10 +489,10 @@ __global__ void __launch_bounds__(1024) policy_sum_kernel(const PolicyArgs a, co
     o.sums[blockIdx.x] = s;
 }
 
-__global__ void __launch_bounds__(1024) policy_total_kernel(const PolicyArgs a, const PolicyState o, int blocks) {
+__global__ void __launch_bounds__(1024) policy_total_kernel(const PolicyArgs a, const PolicyState o, long long blocks) {
   __shared__ PolicySums red[32];
-  PolicySums s = {0.0, 0.0, 0.0};
-  for (int i = threadIdx.x; i < blocks; i += 1024) {
+  PolicySums s{0.0, 0.0, 0.0};
+  for (long long i = threadIdx.x; i < blocks; i += blockDim.x) {
     const PolicySums v = o.sums[i];
     s.loss += v.loss, s.kl += v.kl, s.clipped += v.clipped;
   }
@@ -511,7 +503,7 @@ __global__ void __launch_bounds__(1024) policy_total_kernel(const PolicyArgs a, 
 template <typename T>
 __global__ void __launch_bounds__(1024)
     policy_backward_kernel(const PolicyArgs a, const PolicyState o, const float* grad) {
-  const float c = a.inv_temp * kLog2e;
+  const float c = scale_of(a);
   const float g = *grad;
   if (o.factors != nullptr) {
     // rows of this block whose gradient is not for g (a NaN is for nothing)
@@ -525,9 +517,10 @@ __global__ void __launch_bounds__(1024)
     if (o.factors != nullptr && o.factors[t] == g) continue;  // uniform
     const T* row = static_cast<const T*>(a.logits) + t * a.ld;
     const bool live = a.mask == nullptr || a.mask[t];
-    const float slope = live ? o.terms[t].w : 0.0f;
+    const float4 term = o.terms[t];
+    const float slope = live ? term.w : 0.0f;
     const float k = slope == 0.0f ? 0.0f : g * coefficient(a, share_of(a, o, t), slope);
-    gradient_row(row, static_cast<T*>(o.dlogits) + t * a.vocab, static_cast<int>(a.vocab), k, o.norm[t],
+    gradient_row(row, static_cast<T*>(o.dlogits) + t * a.vocab, static_cast<int>(a.vocab), k, {term.y, term.z},
                  k == 0.0f ? -1 : in_vocabulary(a.ids[t], a.vocab), c);
     if (o.factors != nullptr) {
       __syncthreads();  // every thread has read the factor
@@ -546,9 +539,6 @@ int threads_for(const PolicyArgs& a) {
   return threads;
 }
 
-// A block adds the terms of this many tokens (16 bytes each at some 100 GB/s an SM against a launch more).
-constexpr long long kRun = 16384;
-
 template <typename T>
 int forward_type(const PolicyArgs& a, const PolicyState& s, cudaStream_t stream, int* launches) {
   const bool grad = s.dlogits != nullptr;
@@ -565,12 +555,12 @@ int forward_type(const PolicyArgs& a, const PolicyState& s, cudaStream_t stream,
     policy_rows_kernel<T, true><<<grid, threads, 0, stream>>>(a, s, run);
   else
     policy_rows_kernel<T, false><<<grid, threads, 0, stream>>>(a, s, run);
-  if (a.tokens <= kRun) {
-    policy_sum_kernel<true><<<1, 1024, 0, stream>>>(a, s, kRun);
+  const long long blocks = policy_sum_blocks(a.tokens);
+  if (blocks == 1) {
+    policy_sum_kernel<true><<<1, kRun, 0, stream>>>(a, s);
   } else {
-    const long long blocks = policy_sum_blocks(a.tokens);
-    policy_sum_kernel<false><<<static_cast<unsigned>(blocks), 1024, 0, stream>>>(a, s, (a.tokens + blocks - 1) / blocks);
-    policy_total_kernel<<<1, 1024, 0, stream>>>(a, s, static_cast<int>(blocks));
+    policy_sum_kernel<false><<<static_cast<unsigned>(blocks), kRun, 0, stream>>>(a, s);
+    policy_total_kernel<<<1, 1024, 0, stream>>>(a, s, blocks);
     ++*launches;
   }
   return static_cast<int>(cudaGetLastError());
@@ -586,10 +576,7 @@ int backward_type(const PolicyArgs& a, const PolicyState& s, const float* grad, 
 
 }  // namespace
 
-long long policy_sum_blocks(long long tokens) {
-  const long long blocks = (tokens + 4095) / 4096;
-  return blocks < 148 ? blocks : 148;
-}
+long long policy_sum_blocks(long long tokens) { return (tokens + kRun - 1) / kRun; }
 
 int policy_forward(const PolicyArgs& a, const PolicyState& s, cudaStream_t stream, int* launches) {
   *launches = 0;

@@ -20,7 +20,7 @@ struct PolicyArgs {
   const float* adv = nullptr;      // [tokens], or one a sequence
   int adv_per_sequence = 0;
   double least = 0.8, most = 1.2;  // the clip range
-  float kl = 0.0f, inv_temp = 1.0f;
+  double kl = 0.0, inv_temp = 1.0;
   float weight = 1.0f;             // factor of the loss
   int reduction = kReduceMean;
   int sms = 148;
@@ -32,8 +32,7 @@ struct PolicySums {
 
 struct PolicyState {
   float* logp = nullptr;    // [tokens] output: log-probability of the token, 0 where masked
-  float4* terms = nullptr;  // [tokens] loss, KL, clipped, derivative of the loss by logp (without weights)
-  float2* norm = nullptr;   // [tokens] largest logit and log2 of the sum of exponentials
+  float4* terms = nullptr;  // [tokens] logit, largest logit, sum of powers, derivative of the loss by logp (without weights)
   float* share = nullptr;   // [sequences] a token's share in the reduction, where the mask decides it
   PolicySums* sums = nullptr;  // [policy_sum_blocks] scratch
   float* loss = nullptr;    // scalars
@@ -44,7 +43,7 @@ struct PolicyState {
   float* factors = nullptr; // [tokens]
 };
 
-// Blocks that add the tokens' terms of a large batch.
+// Blocks that add the tokens' terms.
 long long policy_sum_blocks(long long tokens);
 int policy_forward(const PolicyArgs& a, const PolicyState& s, cudaStream_t stream, int* launches);
 // s.dlogits for the gradient *grad of the loss.  With s.factors, rows that hold it already are left.
