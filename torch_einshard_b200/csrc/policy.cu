@@ -9,10 +9,8 @@
 // sequence's tokens) or 1.  A masked token has no loss and a gradient of zeros,
 // whatever its logits, id and other inputs hold: its row is not read.
 //
-// A block reads a token's row with a running maximum m and sum s of
-// 2^((z - m) log2(e) / T) a thread; for very large m (rows of the type's lowest
-// value) the difference is formed before the scaling.  The
-// weights depend on the mask alone, so a training step's forward pass goes on to
+// A block reads a token's row with a running maximum and a sum of powers of two
+// a thread.  The weights depend on the mask alone, so a training step's forward pass goes on to
 // write the row's gradient for g = 1 while the row is still in L2: memory moves
 // 2 + 2 bytes a 16-bit logit instead of the 2 + 2 + 2 of separate passes.  The
 // backward pass then only looks at g; where it is not 1 it forms the gradient
@@ -22,8 +20,14 @@
 // the replay of a captured graph does, gives the gradient for the g of that run.
 // A row whose c is 0 (clipped) is written without a second read.
 //
-// Bounds: memory, then the exponentials (one a logit and pass, 16 a clock and SM).
-// Rows need no alignment: up to seven logits at either end are taken one by one.
+// Bounds: memory, then the exponentials (one a logit and pass, 16 a clock and SM)
+// and the instructions around them.  bf16 with gradient: 12288 rows of 128257 take
+// 1.00 ms, 6.3 TB/s (98 % of a copy's rate), 8192 rows of 32000 150 us (part of a
+// row's second read and of the writes stays in L2); fp32 without, 4084 rows of
+// 50257: 85 us.  Pairs of fp32 operations up to the exponentials, where the scale
+// takes two FMAs: 1.08 ms to 1.00 (behind them their results would have to be moved
+// into pairs).  Rows need no alignment: up to seven logits at either end are taken
+// one by one.
 #include "policy.h"
 
 #include "gemm.h"
@@ -39,7 +43,12 @@ constexpr int kRun = 128;  // tokens whose terms a block adds
 constexpr double kLog2e = 1.4426950408889634;
 constexpr float kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float scale_of(const PolicyArgs& a) { return static_cast<float>(a.inv_temp * kLog2e); }
+// log2(e) / T, and what its first 24 bits leave: rounded towards zero, so that an infinite logit gives the same
+// infinity with both.
+__device__ __forceinline__ float scale_of(const PolicyArgs& a) { return __double2float_rz(a.inv_temp * kLog2e); }
+__device__ __forceinline__ float scale_rest_of(const PolicyArgs& a, float c) {
+  return fmaxf(static_cast<float>(a.inv_temp * kLog2e - c), 1e-30f);
+}
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -57,28 +66,30 @@ __device__ __forceinline__ float base_of(float m, float c) {
   return fabsf(p) < kLarge ? ceilf(p) : INFINITY;
 }
 
-__device__ __forceinline__ float power_of(float z, float m, float q, float c) {
-  return exp2_fast(q == INFINITY ? (z - m) * c : fmaf(z, c, -q));
+// A logit's power.  The rest of the scale is one FMA more: without it a log-probability is off by up to 6e-8 of how
+// far the logit lies from the row's mean, with one sign for all tokens.
+__device__ __forceinline__ float power_of(float z, float q, float c, float rest) {
+  return exp2_fast(fmaf(z, rest, fmaf(z, c, -q)));
 }
 
 // The factor that takes a sum from (m, q) to a larger maximum's (m2, q2).
-__device__ __forceinline__ float rebased(float m, float q, float m2, float q2, float c) {
+__device__ __forceinline__ float rebased(float m, float q, float m2, float q2, float c, float rest) {
   if (m == -INFINITY) return 0.0f;  // nothing summed yet but zeros
   if (q != INFINITY && q2 != INFINITY)
     return __int_as_float(static_cast<int>(fmaxf(q - q2, -127.0f) + 127.0f) << 23);
   if (q == INFINITY && q2 == INFINITY) return exp2_fast((m - m2) * c);
-  return exp2_fast(q == INFINITY ? fmaf(m, c, -q2) : fmaf(-m2, c, q));
+  return exp2_fast(q == INFINITY ? fmaf(m, rest, fmaf(m, c, -q2)) : fmaf(-m2, rest, fmaf(-m2, c, q)));
 }
 
 // Largest logit and sum of powers.
 struct Running {
   float m, s;
   // Joined over the warp: the maximum as an integer of the same order (a NaN ends up in s), one scaling, the sum.
-  __device__ __forceinline__ void over_warp(float c) {
+  __device__ __forceinline__ void over_warp(float c, float rest) {
     const int bits = __float_as_int(m);
     const int top = __reduce_max_sync(0xffffffffu, bits ^ ((bits >> 31) & 0x7fffffff));
     const float largest = __int_as_float(top ^ ((top >> 31) & 0x7fffffff));
-    s = warp_sum(s * rebased(m, base_of(m, c), largest, base_of(largest, c), c));
+    s = warp_sum(s * rebased(m, base_of(m, c), largest, base_of(largest, c), c, rest));
     m = largest;
   }
 };
@@ -86,17 +97,17 @@ struct Running {
 // The same over a thread's chunks.
 struct ChunkSum {
   float m = -INFINITY, q = 0.0f, s = 0.0f;
-  __device__ __forceinline__ void raise(float top, float c) {
+  __device__ __forceinline__ void raise(float top, float c, float rest) {
     if (top > m) {
       const float next = base_of(top, c);
-      s *= rebased(m, q, top, next, c);
+      s *= rebased(m, q, top, next, c, rest);
       m = top;
       q = next;
     }
   }
-  __device__ __forceinline__ void add(float z, float c) {
-    raise(z, c);
-    s += power_of(z, m, q, c);
+  __device__ __forceinline__ void add(float z, float c, float rest) {
+    raise(z, c, rest);
+    s += q == INFINITY ? exp2_fast((z - m) * c) : power_of(z, q, c, rest);
   }
 };
 
@@ -113,11 +124,12 @@ struct GradientRow {
   float k, c, off, factor, m;
   int id;
   bool large;
-  __device__ __forceinline__ GradientRow(float k_, Running row, int id_, float c_) : k(k_), c(c_), m(row.m), id(id_) {
+  __device__ __forceinline__ GradientRow(float k_, Running row, int id_, float c_, float rest)
+      : k(k_), c(c_), m(row.m), id(id_) {
     const float q = base_of(row.m, c);
     large = q == INFINITY;
     off = -q;
-    factor = -k / row.s;
+    factor = -k / row.s * (large ? 1.0f : exp2_fast(m * rest));  // the scale's rest: at the largest logit for all
   }
   __device__ __forceinline__ float minus_p(float z) const {
     return factor * exp2_fast(large ? (z - m) * c : fmaf(z, c, off));
@@ -147,12 +159,13 @@ struct GradientRow {
 
 // A token's gradient row; zeros for k = 0 without reading the logits.
 template <typename T>
-__device__ __forceinline__ void gradient_row(const T* row, T* out, int vocab, float k, Running sum, int id, float c) {
+__device__ __forceinline__ void gradient_row(const T* row, T* out, int vocab, float k, Running sum, int id, float c,
+                                             float rest) {
   const bool zero = k == 0.0f;  // NaN is not zero
   const int head = head_of(out, vocab);
   const bool vec = ((reinterpret_cast<uintptr_t>(row) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
   const int chunks = (vocab - head) / 8, threads = static_cast<int>(blockDim.x), tid = static_cast<int>(threadIdx.x);
-  const GradientRow g(k, sum, id, c);
+  const GradientRow g(k, sum, id, c, rest);
   auto one = [&](int j) { out[j] = from_float<T>(zero ? 0.0f : g.one(to_float<T>(row[j]), j)); };
   if (zero) {
     const Pair nil[4] = {0ull, 0ull, 0ull, 0ull};
@@ -232,9 +245,9 @@ __device__ __forceinline__ Inputs inputs_of(const PolicyArgs& a, const PolicySta
 }
 
 // The derivative of the token's loss by its log-probability (without weights).
-__device__ __forceinline__ float slope_of(const PolicyArgs& a, const Inputs& in, const Running& r, float c) {
+__device__ __forceinline__ float slope_of(const PolicyArgs& a, const Inputs& in, const Running& r, float c, float rest) {
   const float q = base_of(r.m, c);
-  const float d = q == INFINITY ? (in.z - r.m) * c : fmaf(in.z, c, -q);
+  const float d = q == INFINITY ? (in.z - r.m) * c : fmaf(in.z, rest, fmaf(in.z, c, -q));
   const float lp = d * kLn2 - logf(r.s);
   const float ratio = expf(lp - (a.old != nullptr ? in.old : lp));
   const float kept = fminf(fmaxf(ratio, static_cast<float>(a.least)), static_cast<float>(a.most));
@@ -259,9 +272,9 @@ struct RowWords {
 // gradient's coefficient go to w (behind a barrier of the caller's).
 template <bool kGrad>
 __device__ __forceinline__ void finish_token(const PolicyArgs& a, const PolicyState& o, RowWords& w, Running r, float c,
-                                             const Inputs& in, long long t) {
+                                             float rest, const Inputs& in, long long t) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  r.over_warp(c);
+  r.over_warp(c, rest);
   __syncthreads();  // the previous token's words are read
   if (lane == 0) w.red[warp] = make_float2(r.m, r.s);
   __syncthreads();
@@ -269,9 +282,9 @@ __device__ __forceinline__ void finish_token(const PolicyArgs& a, const PolicySt
   const float2 v = lane < static_cast<int>(blockDim.x >> 5) ? w.red[lane] : make_float2(-INFINITY, 0.0f);
   r.m = v.x;
   r.s = v.y;
-  r.over_warp(c);
+  r.over_warp(c, rest);
   if (lane != 0) return;
-  const float slope = kGrad ? slope_of(a, in, r, c) : 0.0f;
+  const float slope = kGrad ? slope_of(a, in, r, c, rest) : 0.0f;
   o.terms[t] = make_float4(in.z, r.m, r.s, slope);
   if (!kGrad) return;
   o.factors[t] = 1.0f;
@@ -281,19 +294,23 @@ __device__ __forceinline__ void finish_token(const PolicyArgs& a, const PolicySt
 
 // Exponentials of kCount chunks of eight under one maximum.
 template <typename T, int kCount>
-__device__ __forceinline__ void add_chunks(ChunkSum& r, const Raw8<T> (&raw)[kCount], float c) {
+__device__ __forceinline__ void add_chunks(ChunkSum& r, const Raw8<T> (&raw)[kCount], float c, float rest) {
   float largest = largest_of(raw[0]);
 #pragma unroll
   for (int u = 1; u < kCount; ++u) largest = fmaxf(largest, largest_of(raw[u]));
-  r.raise(largest, c);
+  r.raise(largest, c, rest);
   float s[2] = {0.0f, 0.0f};
   if (r.q != INFINITY) {
 #pragma unroll
     for (int u = 0; u < kCount; ++u) {
-      float z[8];
+      Pair z[4];
       unpack8(raw[u], z);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) s[k & 1] += exp2_fast(fmaf(z[k], c, -r.q));
+      for (int k = 0; k < 4; ++k) {
+        const float2 y = both(fma2(z[k], pair(rest), fma2(z[k], pair(c), pair(-r.q))));
+        s[0] += exp2_fast(y.x);
+        s[1] += exp2_fast(y.y);
+      }
     }
   } else {
 #pragma unroll
@@ -312,7 +329,7 @@ template <typename T, bool kGrad>
 __global__ void __maxnreg__(kGrad && sizeof(T) == 2 ? 40 : 64)
     policy_rows_kernel(const PolicyArgs a, const PolicyState o, const long long run) {
   __shared__ RowWords w;
-  const float c = scale_of(a);
+  const float c = scale_of(a), rest = scale_rest_of(a, c);
   const int threads = static_cast<int>(blockDim.x), tid = static_cast<int>(threadIdx.x);
   const int vocab = static_cast<int>(a.vocab);
   const long long last = min(a.tokens, (blockIdx.x + 1) * run);
@@ -325,7 +342,7 @@ __global__ void __maxnreg__(kGrad && sizeof(T) == 2 ? 40 : 64)
           o.terms[t] = make_float4(0.0f, 0.0f, 1.0f, 0.0f);
           o.factors[t] = 1.0f;
         }
-        gradient_row(row, out, vocab, 0.0f, {0.0f, 1.0f}, -1, c);
+        gradient_row(row, out, vocab, 0.0f, {0.0f, 1.0f}, -1, c, rest);
       }
       continue;
     }
@@ -343,20 +360,20 @@ __global__ void __maxnreg__(kGrad && sizeof(T) == 2 ? 40 : 64)
       Raw8<T> raw[kUnroll];
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) raw[u] = load(p + u * stride);
-      add_chunks(sum, raw, c);
+      add_chunks(sum, raw, c, rest);
     }
     for (; i < chunks; i += threads, p += stride) {
       const Raw8<T> raw[1] = {load(p)};
-      add_chunks(sum, raw, c);
+      add_chunks(sum, raw, c, rest);
     }
     // the ends of the row
     const int tail = vocab - head - chunks * 8;
-    if (tid < head) sum.add(to_float<T>(row[tid]), c);
-    if (tid < tail) sum.add(to_float<T>(body[chunks * 8 + tid]), c);
-    finish_token<kGrad>(a, o, w, {sum.m, sum.s}, c, in, t);
+    if (tid < head) sum.add(to_float<T>(row[tid]), c, rest);
+    if (tid < tail) sum.add(to_float<T>(body[chunks * 8 + tid]), c, rest);
+    finish_token<kGrad>(a, o, w, {sum.m, sum.s}, c, rest, in, t);
     if (kGrad) {
       __syncthreads();
-      gradient_row(row, out, vocab, w.k, w.sum, id, c);
+      gradient_row(row, out, vocab, w.k, w.sum, id, c, rest);
     }
   }
 }
@@ -443,15 +460,16 @@ __device__ __forceinline__ void store_total(const PolicyArgs& a, const PolicySta
 }
 
 // A token's terms from what its row left, in 64 bits: terms of both signs cancel in the loss, and what 32 bits lose
-// in a log-probability has one sign for all tokens (at 12288 tokens 3e-5 of a loss of 10 to 100; 1e-6 like this).
+// in a log-probability has one sign for all tokens (over 12288 tokens a sum was off by 3e-5, and is by 3e-6 like this).
 // kExpLow is what the row's exponentials are too small by on the average, measured over whole powers of two.
 __device__ __forceinline__ PolicySums terms_of(const PolicyArgs& a, const PolicyState& o, long long t, double* logp) {
   constexpr double kExpLow = 5.05e-8;
   const float4 row = o.terms[t];  // logit, largest logit, sum
   const float c = scale_of(a);
   const float q = base_of(row.y, c);
-  const double z = row.x, d = q == INFINITY ? (z - row.y) * c : z * c - q;
-  const double lp = d / kLog2e - log(static_cast<double>(row.z)) - kExpLow;
+  const double z = row.x, d = q == INFINITY ? z - row.y : z - q / (a.inv_temp * kLog2e);
+  double lp = d * a.inv_temp - log(static_cast<double>(row.z)) - kExpLow;
+  if (lp > 0.0) lp = 0.0;  // a token that is certain
   const double ratio = a.old != nullptr ? exp(lp - a.old[t]) : (lp == lp ? 1.0 : lp);
   const double adv = a.adv[a.adv_per_sequence ? sequence_of(a, t) : t];
   const double s1 = ratio * adv, s2 = fmin(fmax(ratio, a.least), a.most) * adv;
@@ -503,7 +521,7 @@ __global__ void __launch_bounds__(1024) policy_total_kernel(const PolicyArgs a, 
 template <typename T>
 __global__ void __launch_bounds__(1024)
     policy_backward_kernel(const PolicyArgs a, const PolicyState o, const float* grad) {
-  const float c = scale_of(a);
+  const float c = scale_of(a), rest = scale_rest_of(a, c);
   const float g = *grad;
   if (o.factors != nullptr) {
     // rows of this block whose gradient is not for g (a NaN is for nothing)
@@ -521,7 +539,7 @@ __global__ void __launch_bounds__(1024)
     const float slope = live ? term.w : 0.0f;
     const float k = slope == 0.0f ? 0.0f : g * coefficient(a, share_of(a, o, t), slope);
     gradient_row(row, static_cast<T*>(o.dlogits) + t * a.vocab, static_cast<int>(a.vocab), k, {term.y, term.z},
-                 k == 0.0f ? -1 : in_vocabulary(a.ids[t], a.vocab), c);
+                 k == 0.0f ? -1 : in_vocabulary(a.ids[t], a.vocab), c, rest);
     if (o.factors != nullptr) {
       __syncthreads();  // every thread has read the factor
       if (threadIdx.x == 0) o.factors[t] = g;

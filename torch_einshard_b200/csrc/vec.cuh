@@ -177,26 +177,6 @@ __device__ __forceinline__ void store8(T* p, const Pair* f) {
   store8(p, v);
 }
 
-// The same, not to be read soon.
-template <typename T>
-__device__ __forceinline__ void store8_stream(T* p, const Pair* f) {
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) {
-    uint32_t w[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if constexpr (sizeof(T) == 4) {
-        const float2 e = both(f[2 * i + k / 2]);
-        w[k] = __float_as_uint(k & 1 ? e.y : e.x);
-      } else {
-        const float2 e = both(f[k]);
-        w[k] = floats_to_word<T>(e.x, e.y);
-      }
-    }
-    __stcs(reinterpret_cast<uint4*>(p) + i, make_uint4(w[0], w[1], w[2], w[3]));
-  }
-}
-
 // ------------------------------------------------------------------ asynchronous copies
 
 // 16 bytes to shared memory, past the registers; only the first `bytes` are read, the rest is zero.
