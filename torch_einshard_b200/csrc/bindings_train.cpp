@@ -227,7 +227,7 @@ std::vector<Opt> norm_backward_op(const Opt& dh, const Opt& dn, const at::Tensor
     }
   }
   if (s.dw || s.db || s.dpw || s.dpb || s.dgate) {
-    ws = at::empty({plan.units(), plan.sums(), a.d}, x.options().dtype(at::kFloat));
+    ws = at::empty({plan.units(), plan.sums(), plan.pitch(a.d)}, x.options().dtype(at::kFloat));
     g.ws = ws.data_ptr<float>();
   }
   if (!norm_in_registers(a)) {

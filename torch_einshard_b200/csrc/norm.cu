@@ -28,11 +28,20 @@
 // block's rows leaves its own sum and dpw's: S1 = sum D yh gives
 // dgate = pw S1 + pb S0 and gate S1.  Rows too wide for a block are shared by a
 // cluster, still wider ones take several passes through the caches.
+//
+// Measured, forward / backward with the finishing pass: 8192 rows of 2048 bf16
+// (layer, both norms, a gate a channel) 34 / 68 us, 4.0 and 3.0 TB/s of what has to
+// move; 16387 rows of 8192 (rms, a gate a sequence) 253 / 349 us, 4.2 and 4.6 TB/s;
+// 5331 rows of 1001 fp32, not aligned (layer, a gate a token) 30 / 57 us.  What is
+// left is the time between a row's last load and its reductions' results: with 16
+// elements a thread an SM has one to four rows at work.
 #include "norm.h"
 
 #include "gemm.h"
 #include "ptx.cuh"
 #include "vec.cuh"
+
+#include <type_traits>
 
 namespace es {
 namespace {
@@ -604,7 +613,7 @@ struct Sums {
     }
   }
   template <int kA>
-  __device__ __forceinline__ void flush(float* ws, long long d, const Span& s) const {
+  __device__ __forceinline__ void flush(float* ws, long long pitch, const Span& s) const {
 #pragma unroll
     for (int k = 0; k < kSums; ++k) {
       Pair v[kP];
@@ -619,7 +628,7 @@ struct Sums {
           v[2 * q + 1] = acc[kShared ? 0 : k][2 * q + 1];
         }
       }
-      put<float, kA>(ws + k * d, v, s);
+      put<float, kA>(ws + k * pitch, v, s);
     }
   }
 };
@@ -864,7 +873,7 @@ __global__ void __launch_bounds__(kThreads)
     }
     if (stages > 1) stage = stage == ahead ? 0 : stage + 1;
   }
-  if (o.ws != nullptr) sums.template flush<kA>(o.ws + unit * static_cast<long long>(kSums) * a.d, a.d, s);
+  if (o.ws != nullptr) sums.template flush<kA>(o.ws + unit * kSums * plan.pitch(a.d), plan.pitch(a.d), s);
   copy_wait<0>();
   if (blocks > 1) cluster_sync();  // no block leaves while another may still write its words
 }
@@ -960,7 +969,7 @@ __global__ void __launch_bounds__(256)
       s[2] += D;
       s[3] += e.dn;
     }
-    for (int k = 0; k < plan.sums(); ++k) o.ws[(unit * plan.sums() + k) * a.d + c] = s[k];
+    for (int k = 0; k < plan.sums(); ++k) o.ws[(unit * plan.sums() + k) * plan.pitch(a.d) + c] = s[k];
   }
 }
 
@@ -975,22 +984,26 @@ __device__ __forceinline__ void put1(void* p, int f32, int dtype, long long i, f
     static_cast<float*>(p)[i] = v;
 }
 
-// The units' sums to gradients: block (tile of 16 columns, job).  Job 0: the
-// parameters, and the gate's row where it has one; then a job a gate row.  Four
-// threads walk the columns four at a time, 64 the units; the order is fixed.
+// The units' sums to gradients: block (tile of 4 kQuads columns, job).  Job 0: the
+// parameters, and the gate's row where it has one; then a job a gate row.  kQuads
+// threads walk the columns four at a time, the others the units; the order is
+// fixed.  Tiles of 32 columns where there are two for every SM, else of 8 (a
+// sector): 592 units of 2048 columns 11.9 us with tiles of 16 and 6.9 with 8; 148
+// units in seven gate rows of 8192 columns 44 us with 8, 20 with 16 and 11.4 with 32.
 constexpr int kFinishThreads = 256;
 
-template <typename T>
+template <typename T, int kQuads>
 __global__ void __launch_bounds__(kFinishThreads)
     norm_finish_kernel(const NormArgs a, const NormPlan plan, const float* __restrict__ ws, const NormSums o) {
-  __shared__ float part[4][kFinishThreads / 32][16];
+  constexpr int kTile = 4 * kQuads;
+  __shared__ float part[4][kFinishThreads / 32][kTile];
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int quad = lane & 3;                       // columns 4 quad .. 4 quad + 3 of the tile
-  const int walker = w * 8 + (lane >> 2);
-  const long long c4 = blockIdx.x * 16ll + quad * 4;
-  const long long c = blockIdx.x * 16ll + (threadIdx.x & 15);
+  const int quad = lane % kQuads;  // columns 4 quad .. 4 quad + 3 of the tile
+  const int walker = w * (32 / kQuads) + lane / kQuads;
+  const long long c4 = static_cast<long long>(blockIdx.x) * kTile + quad * 4;
+  const long long c = static_cast<long long>(blockIdx.x) * kTile + threadIdx.x % kTile;
   const int n = plan.sums();
-  const bool vec = a.d % 4 == 0;
+  const long long pitch = plan.pitch(a.d);
   const long long jobs = o.dgate != nullptr && plan.groups > 1 ? 1 + plan.groups : 1;
   for (long long job = blockIdx.y; job < jobs; job += gridDim.y) {
     const long long first = job == 0 ? 0 : (job - 1) * plan.slices;
@@ -998,7 +1011,7 @@ __global__ void __launch_bounds__(kFinishThreads)
     const bool weigh = job == 0 && plan.grouped && plan.groups > 1;  // with the gate of the unit's group
     float s[4][4] = {};
 #pragma unroll 4
-    for (long long unit = first + walker; unit < last; unit += kFinishThreads / 4) {
+    for (long long unit = first + walker; unit < last; unit += kFinishThreads / kQuads) {
       float g[4] = {1.0f, 1.0f, 1.0f, 1.0f};
       if (weigh)
 #pragma unroll
@@ -1007,18 +1020,9 @@ __global__ void __launch_bounds__(kFinishThreads)
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if (k >= n) break;
-        const float* u = ws + (unit * n + k) * a.d + c4;
-        float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (vec) {
-          if (c4 < a.d) {
-            const float4 f = *reinterpret_cast<const float4*>(u);
-            v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (c4 + j < a.d) v[j] = u[j];
-        }
+        if (c4 >= pitch) break;
+        const float4 f = *reinterpret_cast<const float4*>(ws + (unit * n + k) * pitch + c4);
+        const float v[4] = {f.x, f.y, f.z, f.w};  // columns behind d hold nothing and go nowhere
         const bool gated = k == 0 || k == 2;
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[k][j] += gated ? g[j] * v[j] : v[j];
@@ -1030,13 +1034,12 @@ __global__ void __launch_bounds__(kFinishThreads)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         float v = s[k][j];
-        v += __shfl_xor_sync(0xffffffffu, v, 4);
-        v += __shfl_xor_sync(0xffffffffu, v, 8);
-        v += __shfl_xor_sync(0xffffffffu, v, 16);
-        if (lane < 4) part[k][w][quad * 4 + j] = v;
+#pragma unroll
+        for (int o = kQuads; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        if (lane < kQuads) part[k][w][quad * 4 + j] = v;
       }
     __syncthreads();
-    if (threadIdx.x < 16 && c < a.d) {
+    if (threadIdx.x < kTile && c < a.d) {
       float e[4];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -1251,8 +1254,15 @@ int backward_type(const NormArgs& a, const NormPlan& plan, const NormBackward& b
   }
   if (rc != 0 || b.ws == nullptr) return rc;
   const long long jobs = s.dgate != nullptr && plan.groups > 1 ? 1 + plan.groups : 1;
-  const dim3 grid(static_cast<unsigned>((a.d + 15) / 16), static_cast<unsigned>(jobs < 65535 ? jobs : 65535));
-  norm_finish_kernel<T><<<grid, kFinishThreads, 0, stream>>>(a, plan, b.ws, s);
+  const auto finish = [&](auto quads) {
+    constexpr int kQuads = decltype(quads)::value, kTile = 4 * kQuads;
+    const dim3 grid(static_cast<unsigned>((a.d + kTile - 1) / kTile), static_cast<unsigned>(jobs < 65535 ? jobs : 65535));
+    norm_finish_kernel<T, kQuads><<<grid, kFinishThreads, 0, stream>>>(a, plan, b.ws, s);
+  };
+  if ((a.d + 31) / 32 * jobs >= 2 * a.sms)
+    finish(std::integral_constant<int, 8>());
+  else
+    finish(std::integral_constant<int, 2>());
   ++*launches;
   return static_cast<int>(cudaGetLastError());
 }

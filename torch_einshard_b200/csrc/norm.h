@@ -42,6 +42,8 @@ struct NormPlan {
   long long groups = 1, slices = 1, len = 0;
   __host__ __device__ long long units() const { return groups * slices; }
   __host__ __device__ int sums() const { return full ? 4 : 2; }
+  // floats from one row of sums to the next
+  __host__ __device__ static long long pitch(long long d) { return (d + 7) / 8 * 8; }
 };
 
 struct NormBackward {
@@ -52,7 +54,7 @@ struct NormBackward {
   void* dy = nullptr;
   void* dgate_rows = nullptr;  // [rows, d] products of a gate that is not grouped; null: not wanted
   int dgate_f32 = 0;
-  float* ws = nullptr;       // [units][sums][d], null when no column sum is wanted
+  float* ws = nullptr;       // [units][sums][pitch(d)], null when no column sum is wanted
   float* coef = nullptr;     // [rows][4], for widths that take several passes (not norm_in_registers)
 };
 
