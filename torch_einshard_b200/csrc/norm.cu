@@ -30,9 +30,10 @@
 // cluster, still wider ones take several passes through the caches.
 //
 // Measured, forward / backward with the finishing pass: 8192 rows of 2048 bf16
-// (layer, both norms, a gate a channel) 34 / 68 us, 4.0 and 3.0 TB/s of what has to
-// move; 16387 rows of 8192 (rms, a gate a sequence) 253 / 349 us, 4.2 and 4.6 TB/s;
-// 5331 rows of 1001 fp32, not aligned (layer, a gate a token) 30 / 57 us.  What is
+// (layer, both norms, a gate a channel) 34 / 66 us, 4.0 and 3.0 TB/s of what has to
+// move; 16387 rows of 8192 (rms, a gate a sequence) 232 / 320 us, 4.6 and 5.0 TB/s;
+// 5331 rows of 1001 fp32, not aligned (layer, a gate a token) 29 / 62 us.  A
+// division a row to find its gate's row cost 8 % of the second.  What is
 // left is the time between a row's last load and its reductions' results: with 16
 // elements a thread an SM has one to four rows at work.
 #include "norm.h"
@@ -247,12 +248,20 @@ __device__ __forceinline__ void wait_row(int stages) {
     copy_wait<0>();
 }
 
-__device__ __forceinline__ long long gate_row(const NormArgs& a, long long row) {
-  if (a.gate_count == 1) return 0;
-  if (a.gate_count == a.rows) return row;
-  if (a.rows < (1ll << 31))
-    return static_cast<uint32_t>(row) / static_cast<uint32_t>(a.gate_inner) % static_cast<uint32_t>(a.gate_count);
-  return (row / a.gate_inner) % a.gate_count;
+// A row's row of the gate, and the first row behind it that may have another: found by division once a run of rows.
+struct GateRow {
+  long long at, end;
+};
+
+__device__ __forceinline__ GateRow gate_of(const NormArgs& a, long long row) {
+  if (a.gate_count == 1) return {0, a.rows};
+  if (a.gate_count == a.rows) return {row, row + 1};
+  if (a.rows < (1ll << 31)) {
+    const uint32_t q = static_cast<uint32_t>(row) / static_cast<uint32_t>(a.gate_inner);
+    return {q % static_cast<uint32_t>(a.gate_count), (q + 1ll) * a.gate_inner};
+  }
+  const long long q = row / a.gate_inner;
+  return {q % a.gate_count, (q + 1) * a.gate_inner};
 }
 
 // ------------------------------------------------------------------ reductions over a row
@@ -444,21 +453,19 @@ __global__ void __launch_bounds__(kThreads)
   Pair t[kP], u[kP], w[kP], b[kP];
   param<T, kA>(a.w, 0, 1.0f, w, s);
   param<T, kA>(a.b, 0, 0.0f, b, s);
-  long long gate_at = -1;
+  long long gate_until = a.y != nullptr ? 0 : a.rows;
   if (blocks > 1) cluster_sync();  // every block runs before one writes another's words
   int stage = 0;
   for (long long row = first; row < a.rows; row += step) {
-    if (a.y != nullptr) {
-      const long long g = gate_row(a, row);
-      if (g != gate_at) {
-        gate_at = g;
-        param<T, kA>(a.gate, g * a.d, 1.0f, t, s);
-        if (kPost) {
-          param<T, kA>(a.pb, 0, 0.0f, u, s);
+    if (row >= gate_until) {
+      const GateRow g = gate_of(a, row);
+      gate_until = g.end;
+      param<T, kA>(a.gate, g.at * a.d, 1.0f, t, s);
+      if (kPost) {
+        param<T, kA>(a.pb, 0, 0.0f, u, s);
 #pragma unroll
-          for (int i = 0; i < kP; ++i) u[i] = mul2(u[i], t[i]);
-          times<T, kA>(a.pw, 0, t, s);
-        }
+        for (int i = 0; i < kP; ++i) u[i] = mul2(u[i], t[i]);
+        times<T, kA>(a.pw, 0, t, s);
       }
     }
     wait_row(stages);
@@ -512,7 +519,7 @@ __global__ void __launch_bounds__(kWideThreads) norm_forward_wide_kernel(const N
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.ldx;
     const T* y = a.y == nullptr ? nullptr : static_cast<const T*>(a.y) + row * a.ldy;
-    const long long g0 = gate_row(a, row) * a.d;
+    const long long g0 = gate_of(a, row).at * a.d;
     float my = 0.0f, ry = 1.0f, mh = 0.0f, s = 0.0f;
     if (a.post) {
       if (a.center) {
@@ -703,18 +710,21 @@ __global__ void __launch_bounds__(kThreads)
     param<T, kA>(a.w, 0, 1.0f, f, s);
     keep(0, f);
   }
-  long long gate_at = -1;
+  long long gate_until = a.y != nullptr ? 0 : a.rows;
   if (blocks > 1) cluster_sync();  // every block runs before one writes another's words
   int stage = 0;
   float4 next_st = first < last ? reinterpret_cast<const float4*>(o.stats)[first] : make_float4(0.0f, 1.0f, 0.0f, 1.0f);
   for (long long row = first; row < last; ++row) {
     const float4 st = next_st;
     if (row + 1 < last) next_st = reinterpret_cast<const float4*>(o.stats)[row + 1];
-    const long long g = gate_row(a, row);
-    g0 = g * a.d;
+    const bool turn = row >= gate_until;  // another row of the gate
+    if (turn) {
+      const GateRow g = gate_of(a, row);
+      gate_until = g.end;
+      g0 = g.at * a.d;
+    }
     Pair hh[kP], yh[kP], t[kP], u[kP];
-    if (!kShared && a.y != nullptr && g != gate_at) {
-      gate_at = g;
+    if (!kShared && turn) {
       param<T, kA>(a.gate, g0, 1.0f, t, s);
       if (kPost) {
         if constexpr (kFull) {
@@ -909,7 +919,7 @@ __global__ void __launch_bounds__(kWideThreads)
   const float inv_d = 1.0f / static_cast<float>(a.d);
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const float4 st = reinterpret_cast<const float4*>(o.stats)[row];
-    const long long g0 = gate_row(a, row) * a.d;
+    const long long g0 = gate_of(a, row).at * a.d;
     float s1 = 0.0f, s2 = 0.0f;
     for (long long c = threadIdx.x; c < a.d; c += blockDim.x) {
       const Terms<T> e(a, o, row, c, st, g0);
@@ -962,7 +972,7 @@ __global__ void __launch_bounds__(256)
     for (long long row = first; row < last; ++row) {
       const float4 st = reinterpret_cast<const float4*>(o.stats)[row];
       const float4 cf = reinterpret_cast<const float4*>(o.coef)[row];
-      const Terms<T> e(a, o, row, c, st, gate_row(a, row) * a.d);
+      const Terms<T> e(a, o, row, c, st, gate_of(a, row).at * a.d);
       const float D = (e.dh + st.w * e.gn - cf.x - cf.y * e.hh) * (plan.grouped ? 1.0f : e.g);
       s[0] += D * e.yh;
       s[1] += e.dn * e.hh;
