@@ -21,11 +21,12 @@
 // A row whose c is 0 (clipped) is written without a second read.
 //
 // Bounds: memory, then the exponentials (one a logit and pass, 16 a clock and SM)
-// and the instructions around them.  bf16 with gradient: 12288 rows of 128257 take
-// 1.00 ms, 6.3 TB/s (98 % of a copy's rate), 8192 rows of 32000 150 us (part of a
-// row's second read and of the writes stays in L2); fp32 without, 4084 rows of
-// 50257: 85 us.  Pairs of fp32 operations up to the exponentials, where the scale
-// takes two FMAs: 1.08 ms to 1.00 (behind them their results would have to be moved
+// and the instructions around them.  bf16 with gradient, 58 % of the tokens kept:
+// 12288 rows of 128257 take 0.92 ms, 8192 rows of 32000 150 us, 5.4 and 5.5 TB/s of
+// what has to move (84 % of a copy's rate; part of the second reads misses L2); fp32
+// without, 4084 rows of 50257: 74 us, a copy's rate.  Pairs of fp32 operations up to
+// the exponentials, where the scale
+// takes two FMAs, saved 7 % (behind them their results would have to be moved
 // into pairs).  Rows need no alignment: up to seven logits at either end are taken
 // one by one.
 #include "policy.h"
@@ -547,13 +548,21 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-// Threads of a row's block: about sixteen chunks each.  With 40 registers a
-// thread an SM holds some 1500 of them, so that between its two reads a row of a
-// large vocabulary shares L2 (126 MB) with one or two of every other SM (fp32
-// rows and those read once take 64).
-int threads_for(const PolicyArgs& a) {
+// Threads of a row's block: about sixteen chunks each.  Without gradient many
+// small blocks are best (1024 bf16 rows of 32000: 15.5 us with 128 threads, 16.9 with 256, 18.5 with
+// 512).  With it a block waits between its two passes, and rows
+// between their reads have to fit in L2 (126 MB): 1500 threads an SM (40
+// registers each) with one or two rows of a large vocabulary.  bf16, 128 / 256 / 512 / 768 / 1024 threads: 8192
+// rows of 32000 175 / 152 / 161 / 193 / 241 us, 6144 of 100000 427 / 408 / 374 /
+// 348 / 410, 6144 of 128257 484 / 464 / 433 / 402 / 445; fp32, 6144 of 64001 558 /
+// 543 / 522 / 622 / 590.  Few rows take larger blocks, until the SMs are full (33 rows of
+// 32000: 8.8 us with 256, 6.5 with 1024).
+int threads_for(const PolicyArgs& a, bool grad) {
+  const int most = grad ? 512 : 128;
   int threads = 64;
-  while (threads < 1024 && threads * 128ll < a.vocab) threads *= 2;
+  while (threads < most && threads * 128ll < a.vocab) threads *= 2;
+  if (grad && a.dtype != kDtypeF32 && threads * 128ll < a.vocab) threads = 768;
+  while (threads <= 512 && threads * 8ll < a.vocab && 2 * threads * a.tokens <= a.sms * 1536ll) threads *= 2;
   return threads;
 }
 
@@ -565,7 +574,7 @@ int forward_type(const PolicyArgs& a, const PolicyState& s, cudaStream_t stream,
     policy_shares_kernel<<<1, 1024, 0, stream>>>(a, s);
     ++*launches;
   }
-  const int threads = threads_for(a);
+  const int threads = threads_for(a, grad);
   const long long resident = a.sms * (1536ll / threads);
   const long long run = a.tokens / (resident * 16) < 1 ? 1 : a.tokens / (resident * 16);
   const unsigned grid = static_cast<unsigned>((a.tokens + run - 1) / run);
@@ -586,7 +595,7 @@ int forward_type(const PolicyArgs& a, const PolicyState& s, cudaStream_t stream,
 
 template <typename T>
 int backward_type(const PolicyArgs& a, const PolicyState& s, const float* grad, cudaStream_t stream) {
-  const int threads = threads_for(a);
+  const int threads = threads_for(a, true);
   const long long cap = a.sms * (1024ll / threads);
   policy_backward_kernel<T><<<static_cast<unsigned>(a.tokens < cap ? a.tokens : cap), threads, 0, stream>>>(a, s, grad);
   return static_cast<int>(cudaGetLastError());
