@@ -525,6 +525,38 @@ def test_shared_operand_captured():
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_second_derivatives_are_refused(device):
+    x, w, dy, _, _ = shared_case(torch.bfloat16, device, (2, 16, 32), 2, torch.Generator().manual_seed(6))
+    for activation in (None, "silu"):
+        kept = es.checkpoint8(x)
+        ys = [es.einshard("b s c, n c -> b s n", kept, v, activation=activation) for v in w]
+        ys = [y.value if activation else y for y in ys]
+        dx, dw = torch.autograd.grad(ys, [x, w[0]], dy, create_graph=True)
+        for g in (dx, dw):
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad((g + 0 * w[0].sum()).sum(), w[0], retain_graph=True)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_operands_changed_in_place(device):
+    x, w, dy, _, _ = shared_case(torch.bfloat16, device, (2, 16, 32), 1, torch.Generator().manual_seed(7))
+    h = x * 1
+    kept = es.checkpoint8(h)
+    y = es.einshard("b s c, n c -> b s n", kept, w[0])
+    h.add_(1)  # the product is done, the codes are their own
+    torch.autograd.grad(y, x, dy[0], retain_graph=True)
+    with pytest.raises(RuntimeError):
+        es.einshard("b s c, n c -> b s n", kept, w[0])  # its value is no longer what the codes stand for
+    with torch.no_grad():
+        w[0].mul_(2)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(y, x, dy[0])
+    with torch.inference_mode():
+        es.einshard("b s c, n c -> b s n", es.checkpoint8(torch.ones(2, 3, 32, dtype=torch.bfloat16, device=device)),
+                    torch.ones(8, 32, dtype=torch.bfloat16, device=device))
+
+
 # ------------------------------------------------------------------ two ranks
 
 def _sharded_models(ctx):

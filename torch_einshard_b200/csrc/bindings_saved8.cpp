@@ -100,6 +100,7 @@ struct Part {
   std::shared_ptr<const ContractPlan> plan;
   at::Tensor dz, yt;
   c10::cuda::CUDAStream stream;
+  std::vector<at::Tensor> sources;  // what its gradient depends on
 };
 
 // One backward pass's: the parts, and the operand restored by the first contraction (for those on its stream).
@@ -173,7 +174,7 @@ struct ReadersNode : public Node {
         total[0] = total[0].defined() ? total[0] + dx : dx;
       }
     }
-    for (const Part& p : parts) from.push_back(p.dz), from.push_back(p.yt);
+    for (const Part& p : parts) from.insert(from.end(), p.sources.begin(), p.sources.end());
     finalise(total, from);
     return total;
   }
@@ -237,7 +238,9 @@ struct ContractNode : public Node {
       const at::Tensor y3 = plan->operand_y(yv), yt = y3.transpose(1, 2);
       at::Tensor x;  // the operand, for dy
       if (readers != nullptr) {
-        readers->add({plan, gz, yt, at::cuda::getCurrentCUDAStream()});
+        std::vector<at::Tensor> sources(grads);
+        sources.push_back(yv);
+        readers->add({plan, gz, yt, at::cuda::getCurrentCUDAStream(), sources});
       } else if (want_place && same_rows(c)) {
         // (dz y^T) silu'(h^) and silu(h^) from one product
         const auto both = g_ops.silu_grad(gz, prepared(yt), c, e, err);

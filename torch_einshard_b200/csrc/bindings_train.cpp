@@ -262,7 +262,6 @@ void finalise(std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& fro
     if (!input.defined() || !input.requires_grad()) continue;
     for (at::Tensor& g : grads)
       if (g.defined()) g = Final::apply(g, input);
-    return;
   }
 }
 

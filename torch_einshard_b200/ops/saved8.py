@@ -106,7 +106,7 @@ class Saved8:
     kept.  ``restore()`` gives the values that backward sees.
     """
 
-    __slots__ = ("value", "codes", "exps", "_act", "_base", "_order", "_pre", "_readers", "_box")
+    __slots__ = ("value", "codes", "exps", "_act", "_base", "_order", "_pre", "_readers", "_box", "_version")
 
     def __init__(self, value, codes, exps, act=False, base=None, order=None, pre=None):
         self.value, self.codes, self.exps = value, codes, exps
@@ -116,6 +116,7 @@ class Saved8:
         self._pre = pre  # the pre-activation's place in the graph (a tensor without values of its own)
         self._readers = None  # the place where the gradients of its native contractions meet
         self._box = None  # and of the others, with what they leave there
+        self._version = None if value.is_inference() else value._version  # what the codes were formed from
 
     @property
     def shape(self):
@@ -263,6 +264,27 @@ def _place_of(a):
     return a.new_empty(()).expand(a.shape)
 
 
+class _Final(torch.autograd.Function):
+    """A gradient without a derivative of its own: under create_graph, using it further raises."""
+
+    @staticmethod
+    def forward(ctx, t, source):
+        return t.view_as(t)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("trying to differentiate twice a function that was marked with once_differentiable")
+
+    @classmethod
+    def of(cls, grads, sources):
+        """``grads`` as results of ``sources``, where a graph of the backward pass is wanted."""
+        if torch.is_grad_enabled():
+            for source in sources:
+                if source is not None and source.requires_grad:
+                    grads = tuple(None if g is None else cls.apply(g, source) for g in grads)
+        return grads
+
+
 class _Readers(torch.autograd.Function):
     """The place in the graph where the gradients of an operand's contractions meet.
 
@@ -278,15 +300,18 @@ class _Readers(torch.autograd.Function):
         return _place_of(x)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, _):
         parts = ctx.box.pop(torch._C._current_graph_task_id(), [])
+        if not parts:
+            return None, None
         total = None
-        for equation, dz, y in parts:
-            wide = torch.promote_types(dz.dtype, torch.float32) if len(parts) > 1 else dz.dtype
-            dx = _operand_grad(equation, dz.to(wide), y.to(wide))
-            total = dx if total is None else total + dx
-        return None if total is None else total.to(parts[0][1].dtype), None
+        with torch.no_grad():
+            for equation, dz, y in parts:
+                wide = torch.promote_types(dz.dtype, torch.float32) if len(parts) > 1 else dz.dtype
+                dx = _operand_grad(equation, dz.to(wide), y.to(wide))
+                total = dx if total is None else total + dx
+            total = total.to(parts[0][1].dtype)
+        return _Final.of((total, None), [t for _, dz, y in parts for t in (dz, y)])
 
 
 def _operand_grad(equation, dz, y):
@@ -319,8 +344,13 @@ class _Contraction8(torch.autograd.Function):
         return a, _place_of(a), h_codes, h_exps
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, grad, grad_pre=None, *_):
+    def backward(ctx, *grads):
+        with torch.no_grad():
+            found = _Contraction8.gradients(ctx, *grads)
+        return _Final.of(found, (*grads, ctx.saved_tensors[0]))
+
+    @staticmethod
+    def gradients(ctx, grad, grad_pre=None, *_):
         y, codes, exps = ctx.saved_tensors[:3]
         if grad is not None and ctx.silu:
             grad = _silu_grad(grad, *ctx.saved_tensors[3:], None)
@@ -351,6 +381,8 @@ def contract_saved(equation, saved, y, activation=None):
     if y.dtype != x.dtype or y.device != x.device:
         raise ValueError(f"a Saved8 operand of {x.dtype} on {x.device} needs the other one alike, "
                          f"not {y.dtype} on {y.device}")
+    if saved._version is not None and x._version != saved._version:
+        raise RuntimeError("a Saved8 operand's value has been modified in place since its codes were formed")
     plan = _product(equation, tuple(x.shape), tuple(y.shape))
     silu = activation is not None
     if all(plan.gemm) and gemm.eligible(x, y):
