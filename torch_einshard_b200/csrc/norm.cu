@@ -32,7 +32,7 @@
 // Measured, forward / backward with the finishing pass: 8192 rows of 2048 bf16
 // (layer, both norms, a gate a channel) 34 / 66 us, 4.0 and 3.0 TB/s of what has to
 // move; 16387 rows of 8192 (rms, a gate a sequence) 232 / 320 us, 4.6 and 5.0 TB/s;
-// 5331 rows of 1001 fp32, not aligned (layer, a gate a token) 29 / 62 us.  A
+// 5331 rows of 1001 fp32, not aligned (layer, a gate a token) 29 / 54 us.  A
 // division a row to find its gate's row cost 8 % of the second.  What is
 // left is the time between a row's last load and its reductions' results: with 16
 // elements a thread an SM has one to four rows at work.
@@ -710,6 +710,7 @@ __global__ void __launch_bounds__(kThreads)
     param<T, kA>(a.w, 0, 1.0f, f, s);
     keep(0, f);
   }
+  const bool each = a.y != nullptr && a.gate_count == a.rows;
   long long gate_until = a.y != nullptr ? 0 : a.rows;
   if (blocks > 1) cluster_sync();  // every block runs before one writes another's words
   int stage = 0;
@@ -717,8 +718,10 @@ __global__ void __launch_bounds__(kThreads)
   for (long long row = first; row < last; ++row) {
     const float4 st = next_st;
     if (row + 1 < last) next_st = reinterpret_cast<const float4*>(o.stats)[row + 1];
-    const bool turn = row >= gate_until;  // another row of the gate
-    if (turn) {
+    const bool turn = each || row >= gate_until;  // another row of the gate
+    if (each) {
+      g0 = row * a.d;
+    } else if (turn) {
       const GateRow g = gate_of(a, row);
       gate_until = g.end;
       g0 = g.at * a.d;
