@@ -30,7 +30,7 @@
 // cluster, still wider ones take several passes through the caches.
 //
 // Measured, forward / backward with the finishing pass: 8192 rows of 2048 bf16
-// (layer, both norms, a gate a channel) 34 / 66 us, 4.0 and 3.0 TB/s of what has to
+// (layer, both norms, a gate a channel) 31 / 67 us, 4.4 and 3.0 TB/s of what has to
 // move; 16387 rows of 8192 (rms, a gate a sequence) 232 / 320 us, 4.6 and 5.0 TB/s;
 // 5331 rows of 1001 fp32, not aligned (layer, a gate a token) 29 / 54 us.  A
 // division a row to find its gate's row cost 8 % of the second.  What is
@@ -359,27 +359,34 @@ __device__ __forceinline__ void row_stats(const Pair (&v)[kP], const Span& s, co
   const float2* set = reinterpret_cast<const float2*>(ex.share(lane == 0 ? mw : sq, lane));
   float m = 0.0f, q = 0.0f;
   if (entries <= 4) {
-    // few words: every thread adds them all
-    for (int e = 0; e < entries; ++e) {
-      const float2 w = set[e];
-      m += w.x * count(e / ex.warps, e % ex.warps);
-      q += w.y;
+    // few words, of one block: every thread adds them all
+    float2 w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      w[e] = e < entries ? set[e] : make_float2(0.0f, 0.0f);
+      q += w[e].y;
     }
-    m *= inv_d;
-    if (a.center)
-      for (int e = 0; e < entries; ++e) {
-        const float off = set[e].x - m;
-        q += off * off * count(e / ex.warps, e % ex.warps);
+    if (a.center) {
+      float n[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        n[e] = e < entries ? static_cast<float>(count(0, e)) : 0.0f;
+        m += w[e].x * n[e];
       }
+      m *= inv_d;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q += (w[e].x - m) * (w[e].x - m) * n[e];
+    }
   } else if (!a.center) {
     for (int e = lane; e < entries; e += 32) q += set[e].y;
     q = warp_sum(q);
   } else {
-    for (int e = lane; e < entries; e += 32) m += set[e].x * count(e / ex.warps, e % ex.warps);
+    auto of = [&](int e) { return ex.blocks == 1 ? count(0, e) : count(e / ex.warps, e % ex.warps); };
+    for (int e = lane; e < entries; e += 32) m += set[e].x * of(e);
     m = warp_sum(m) * inv_d;
     for (int e = lane; e < entries; e += 32) {
       const float2 w = set[e];
-      q += w.y + (w.x - m) * (w.x - m) * count(e / ex.warps, e % ex.warps);
+      q += w.y + (w.x - m) * (w.x - m) * of(e);
     }
     q = warp_sum(q);
   }
