@@ -431,7 +431,7 @@ def shared_case(dtype, device, shape, outs, gen):
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("shape,outs", [((2, 5, 24), 2), ((1, 300, 136), 3), ((3, 64, 129), 4), ((2, 33, 256), 6),
-                                        ((1, 1, 64), 3), ((1, 1024, 512), 3)])
+                                        ((1, 1, 64), 3), ((1, 1024, 512), 3), ((1, 700, 615), 3), ((2, 3, 7), 2)])
 def test_shared_operand_is_rounded_once(device, dtype, shape, outs):
     """dx = sum_i dz_i w_i: half a step of the result, and for the 32-bit sums 2^-22 of the sum of absolute values.
 
@@ -440,6 +440,12 @@ def test_shared_operand_is_rounded_once(device, dtype, shape, outs):
     x, w, dy, want, size = shared_case(dtype, device, shape, outs, torch.Generator().manual_seed(outs))
     kept = es.checkpoint8(x)
     ys = [es.einshard("b s c, n c -> b s n", kept, v) for v in w]
+    assert all(y.is_contiguous() for y in ys)
+    for y, v in zip(ys, w):
+        exact = x.detach().double() @ v.detach().double().t()
+        sums = (x.shape[-1] + 1) * 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -22
+        bound = half_step(dtype) * exact.abs() + sums * (x.detach().double().abs() @ v.detach().double().abs().t())
+        assert ((y.detach().double() - exact).abs() <= bound + torch.finfo(dtype).tiny).all()
     dx = torch.autograd.grad(ys, x, dy, retain_graph=True)[0]
     terms = sum(v.shape[0] for v in w)
     sums = (terms + 1) * 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -22

@@ -61,6 +61,10 @@ struct ContractPlan {
   at::Tensor operand_y(const at::Tensor& y) const { return moved(y, y_order).reshape({batch, red, cols}); }
   at::Tensor result(const at::Tensor& z) const { return moved(z.view(z_shape), z_order); }
   at::Tensor product_of(const at::Tensor& z) const { return moved(z, z_back).reshape({batch, rows, cols}); }
+  // whether the operands' matrices are the same
+  bool reads_like(const ContractPlan& p) const {
+    return x_order == p.x_order && batch == p.batch && rows == p.rows;
+  }
   at::Tensor x_of(const at::Tensor& t) const { return moved(t.view(x_shape), x_back); }
 };
 
@@ -73,9 +77,11 @@ bool readable(const at::Tensor& t, int64_t dim) {
   return row * size % 16 == 0 && (t.size(0) == 1 || t.stride(0) * size % 16 == 0);
 }
 
-// The matrix in a layout that the products read; a copy has rows that are a multiple of 16 bytes apart.
+// The matrix in a layout that the products read; a copy has rows (columns, where these are in a row) that are a
+// multiple of 16 bytes apart.
 at::Tensor prepared(const at::Tensor& t) {
   if (readable(t, 2) || readable(t, 1)) return t;
+  if (t.stride(1) == 1 && t.stride(2) != 1) return prepared(t.transpose(1, 2)).transpose(1, 2);
   const int64_t unit = 16 / t.element_size(), pitch = (t.size(2) + unit - 1) / unit * unit;
   at::Tensor copy = at::empty({t.size(0), t.size(1), pitch}, t.options()).narrow(2, 0, t.size(2));
   copy.copy_(t);
@@ -103,10 +109,12 @@ struct Part {
   std::vector<at::Tensor> sources;  // what its gradient depends on
 };
 
-// One backward pass's: the parts, and the operand restored by the first contraction (for those on its stream).
+// One backward pass's: the parts, and the operand restored by the first contraction, for those on its stream that
+// read it in the same order.
 struct Pass {
   std::vector<Part> parts;
   at::Tensor operand;
+  std::shared_ptr<const ContractPlan> plan;
   c10::optional<c10::cuda::CUDAStream> stream;
 };
 
@@ -123,13 +131,15 @@ struct ReadersNode : public Node {
   }
 
   template <class Restore>
-  at::Tensor operand(const c10::cuda::CUDAStream& stream, const Restore& restore) {
+  at::Tensor operand(const std::shared_ptr<const ContractPlan>& plan, const Restore& restore) {
+    const auto stream = at::cuda::getCurrentCUDAStream();
     const std::lock_guard<std::mutex> held(lock);
     Pass& pass = passes[torch::autograd::get_current_graph_task_id()];
-    if (pass.stream.has_value() && *pass.stream == stream) return pass.operand;
+    if (pass.stream.has_value() && *pass.stream == stream && pass.plan->reads_like(*plan)) return pass.operand;
     const at::Tensor x = restore();
     if (!pass.stream.has_value()) {
       pass.operand = x;
+      pass.plan = plan;
       pass.stream = stream;
     }
     return x;
@@ -165,7 +175,7 @@ struct ReadersNode : public Node {
         std::vector<at::Tensor> dz, yt;
         for (size_t j = i; j < parts.size(); ++j) {
           const ContractPlan& p = *parts[j].plan;
-          if (used[j] || p.x_order != plan.x_order || p.batch != plan.batch || p.rows != plan.rows) continue;
+          if (used[j] || !p.reads_like(plan)) continue;
           used[j] = true;
           dz.push_back(parts[j].dz);
           yt.push_back(prepared(parts[j].yt));
@@ -255,9 +265,8 @@ struct ContractNode : public Node {
       }
       if (task_should_compute_output(2)) {
         if (!x.defined()) {
-          const auto restore = [&] { return restored(c, e); };
-          const at::Tensor whole = readers == nullptr ? restore() : readers->operand(at::cuda::getCurrentCUDAStream(), restore);
-          x = prepared(plan->operand_x(whole));
+          const auto restore = [&] { return prepared(plan->operand_x(restored(c, e))); };
+          x = readers == nullptr ? restore() : readers->operand(plan, restore);
         }
         // a transposed y (an [out, in] weight) gets its gradient in its own memory order
         const bool turned = y3.stride(1) == 1 && y3.size(1) > 1;
@@ -293,29 +302,37 @@ at::Tensor readers_of(const at::Tensor& x, const at::Tensor& err) {
 }
 
 // The contraction of x, whose gradient goes to `place` where there is one (a pre-activation's place, or readers_of),
-// with y: (z), or with `silu` (silu(z), its pre-activation's place, codes and exponents).
+// with y: (z), or with `silu` (silu(z), its pre-activation's place, codes and exponents).  `ready` is x's matrix as an
+// earlier contraction read it; where that takes a copy, the matrix is the last result.
 std::vector<at::Tensor> contract8(const at::Tensor& x, const Opt& place, const at::Tensor& y,
                                   const std::shared_ptr<ContractPlan>& plan, const at::Tensor& codes,
                                   const at::Tensor& exps, bool act, const Order& base, const Order& order, bool silu,
-                                  const at::Tensor& err) {
+                                  const at::Tensor& err, const Opt& ready) {
   TORCH_CHECK(x.is_cuda() && y.device() == x.device() && codes.device() == x.device() && exps.device() == x.device(),
               "einshard: operands of an 8-bit contraction on one CUDA device");
   const c10::cuda::CUDAGuard guard(x.device());
   std::vector<at::Tensor> out;
+  at::Tensor copied;
+  const auto results = [&]() -> std::vector<at::Tensor>& {
+    if (copied.defined()) out.push_back(copied);
+    return out;
+  };
   {
     const at::AutoDispatchBelowADInplaceOrView below;
-    const at::Tensor xv = prepared(plan->operand_x(x.detach())), yv = prepared(plan->operand_y(y.detach()));
+    const at::Tensor own = ready.has_value() ? *ready : plan->operand_x(x.detach());
+    const at::Tensor xv = prepared(own), yv = prepared(plan->operand_y(y.detach()));
+    if (!xv.is_same(own)) copied = xv;
     if (silu) {
       out = g_ops.silu(xv, yv, err);
       out[0] = plan->result(out[0]);
       out.insert(out.begin() + 1, place_of(out[0]));
     } else {
-      out = {plan->result(g_ops.product(xv, yv, err))};
+      out = {plan->result(g_ops.product(xv, yv, err).contiguous())};
     }
   }
   const at::Tensor from = place.has_value() ? at::Tensor() : x;
   const at::Tensor at = place.has_value() ? *place : at::Tensor();
-  if (!torch::autograd::compute_requires_grad(from, at, y)) return out;
+  if (!torch::autograd::compute_requires_grad(from, at, y)) return results();
   auto node = std::shared_ptr<ContractNode>(new ContractNode(), torch::autograd::deleteNode);
   node->set_next_edges(torch::autograd::collect_next_edges(from, at, y));
   node->plan = plan;
@@ -332,7 +349,7 @@ std::vector<at::Tensor> contract8(const at::Tensor& x, const Opt& place, const a
   }
   torch::autograd::set_history(out[0], node);
   if (silu) torch::autograd::set_history(out[1], node);
-  return out;
+  return results();
 }
 
 }  // namespace

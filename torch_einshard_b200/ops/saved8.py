@@ -106,7 +106,7 @@ class Saved8:
     kept.  ``restore()`` gives the values that backward sees.
     """
 
-    __slots__ = ("value", "codes", "exps", "_act", "_base", "_order", "_pre", "_readers", "_box", "_version")
+    __slots__ = ("value", "codes", "exps", "_act", "_base", "_order", "_pre", "_readers", "_box", "_version", "_ready")
 
     def __init__(self, value, codes, exps, act=False, base=None, order=None, pre=None):
         self.value, self.codes, self.exps = value, codes, exps
@@ -116,6 +116,7 @@ class Saved8:
         self._pre = pre  # the pre-activation's place in the graph (a tensor without values of its own)
         self._readers = None  # the place where the gradients of its native contractions meet
         self._box = None  # and of the others, with what they leave there
+        self._ready = None  # the operand's matrix where contractions read it from a copy with padded rows
         self._version = None if value.is_inference() else value._version  # what the codes were formed from
 
     @property
@@ -393,11 +394,14 @@ def contract_saved(equation, saved, y, activation=None):
             if place is None:
                 place = saved._readers = mod.readers8(x, err)
         order = () if saved._order is None else saved._order
+        key, ready = saved._ready or (None, None)
         out = mod.contract8(x, place, y, plan.on_kernels, saved.codes, saved.exps, saved._act, saved._base, order,
-                            silu, err)
+                            silu, err, ready if key == (plan.x_order, plan.gemm[:2]) else None)
+        if len(out) > (4 if silu else 1):
+            saved._ready = (plan.x_order, plan.gemm[:2]), out[-1]
         if not silu:
             return out[0]
-        a, pre, codes, exps = out
+        a, pre, codes, exps = out[:4]
         return Saved8(a, codes, exps, True, plan.z_shape, plan.z_order, pre)
     place, box = saved._pre, None
     if place is None and x.requires_grad and torch.is_grad_enabled():
