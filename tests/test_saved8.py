@@ -10,6 +10,7 @@ accumulation (2^-23 a term at most, which the same product bounds).
 import pytest
 import torch
 import torch.distributed as dist
+import torch.utils.checkpoint
 from dist_harness import run_ranks
 
 import torch_einshard_b200 as es
@@ -529,6 +530,40 @@ def test_shared_operand_captured():
     graph.replay()
     for a, b in zip(out, step()):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_copies_stay_on_their_stream():
+    """An odd width is read from a copy: a contraction on another stream does not take one that is still being made."""
+    gen = torch.Generator().manual_seed(8)
+    x, w, dy, _, _ = shared_case(torch.bfloat16, "cuda", (8, 1024, 1021), 2, gen)
+    want = [es.einshard("b s c, n c -> b s n", es.checkpoint8(x), v) for v in w]
+    side = torch.cuda.Stream()
+    for _ in range(4):
+        kept = es.checkpoint8(x)
+        torch.cuda.synchronize()
+        first = es.einshard("b s c, n c -> b s n", kept, w[0])
+        with torch.cuda.stream(side):
+            second = es.einshard("b s c, n c -> b s n", kept, w[1])
+        torch.cuda.synchronize()
+        assert torch.equal(first, want[0]) and torch.equal(second, want[1])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("width", [64, 37])
+def test_inside_a_recomputed_block(device, width):
+    x, w, dy, _, _ = shared_case(torch.bfloat16, device, (2, 16, width), 2, torch.Generator().manual_seed(10))
+
+    def block(x, *w):
+        kept = es.checkpoint8(x)
+        a = es.einshard("b s c, n c -> b s n", kept, w[0], activation="silu")
+        return es.einshard("b s n, n c -> b s c", a, w[0]), es.einshard("b s c, n c -> b s n", kept, w[1])
+
+    dz = [torch.randn(2, 16, width, generator=torch.Generator().manual_seed(11)).to(x), dy[1]]
+    plain = torch.autograd.grad(block(x, *w), [x, *w], dz)
+    again = torch.utils.checkpoint.checkpoint(block, x, *w, use_reentrant=False)
+    for g, h in zip(plain, torch.autograd.grad(again, [x, *w], dz)):
+        assert torch.equal(g, h)
 
 
 @pytest.mark.parametrize("device", DEVICES)

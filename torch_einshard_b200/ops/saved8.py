@@ -347,14 +347,15 @@ class _Contraction8(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *grads):
         with torch.no_grad():
-            found = _Contraction8.gradients(ctx, *grads)
-        return _Final.of(found, (*grads, ctx.saved_tensors[0]))
+            saved = ctx.saved_tensors  # once: a recomputed block's are given out once
+            found = _Contraction8.gradients(ctx, saved, *grads)
+        return _Final.of(found, (*grads, saved[0]))
 
     @staticmethod
-    def gradients(ctx, grad, grad_pre=None, *_):
-        y, codes, exps = ctx.saved_tensors[:3]
+    def gradients(ctx, saved, grad, grad_pre=None, *_):
+        y, codes, exps = saved[:3]
         if grad is not None and ctx.silu:
-            grad = _silu_grad(grad, *ctx.saved_tensors[3:], None)
+            grad = _silu_grad(grad, *saved[3:], None)
         if grad_pre is not None:
             grad = grad_pre if grad is None else grad + grad_pre
         if grad is None:
@@ -372,6 +373,12 @@ class _Contraction8(torch.autograd.Function):
             (ex, ey), ez = ctx.equation.split("->")[0].split(","), ctx.equation.split("->")[1]
             dy = contract(f"{ez},{ex}->{ey}", grad, _restore_operand(codes, exps, ctx.meta))
         return dx, dplace, None, dy, None, None, None, None, None
+
+
+def _reading(plan, x):
+    """What has to be alike for a contraction to read an earlier one's copy: the matrix, the stream, the capture."""
+    return (plan.x_order, plan.gemm[:2], torch.cuda.current_stream(x.device),
+            torch.cuda.is_current_stream_capturing())
 
 
 def contract_saved(equation, saved, y, activation=None):
@@ -394,11 +401,13 @@ def contract_saved(equation, saved, y, activation=None):
             if place is None:
                 place = saved._readers = mod.readers8(x, err)
         order = () if saved._order is None else saved._order
-        key, ready = saved._ready or (None, None)
+        ready = None
+        if saved._ready is not None and saved._ready[0] == _reading(plan, x):
+            ready = saved._ready[1]
         out = mod.contract8(x, place, y, plan.on_kernels, saved.codes, saved.exps, saved._act, saved._base, order,
-                            silu, err, ready if key == (plan.x_order, plan.gemm[:2]) else None)
+                            silu, err, ready)
         if len(out) > (4 if silu else 1):
-            saved._ready = (plan.x_order, plan.gemm[:2]), out[-1]
+            saved._ready = _reading(plan, x), out[-1]
         if not silu:
             return out[0]
         a, pre, codes, exps = out[:4]
