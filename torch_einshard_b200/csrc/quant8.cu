@@ -285,11 +285,12 @@ __global__ void __launch_bounds__(kThreads) restore8_any_kernel(const int8_t* __
 // memory (integer maxima: any order gives the same), and a tile reads 32
 // elements more on both sides, for the blocks that it shares with its
 // neighbours.  Against one element a lane (the kernels above), fp16: 24004 rows of
-// 8191 quantised in 224 us instead of 314, restored in 153 instead of 207;
-// 3000000 rows of 65 in 248 and 171 us instead of 1925 and 1427.  Aligned rows
-// of 8192 take 103 and 111: the difference is instructions, 78 % of the issue
-// slots; a step formed once a block in shared memory and 16-bit maxima of two
-// elements at once took 267 us to 224.
+// 8191 quantised in 208 us instead of 314, restored in 152 instead of 207;
+// 3000000 rows of 65 in 259 and 172 us instead of 1925 and 1427.  Aligned rows
+// of 8192 take 101 and 109: the difference is instructions (78 % of the issue
+// slots in the first form).  A step formed once a block in shared memory and
+// 16-bit maxima of two elements at once took 267 us to 224, the third span's
+// maximum only where there is one, to 208.
 
 constexpr int kTile = kThreads * 8 * kUnroll;
 constexpr int kTileStep = kTile - 2 * kQuantBlock;
@@ -347,11 +348,19 @@ __device__ __forceinline__ void span_maxima(const Raw8<T>& raw, const Spans& s, 
     uint32_t top[3] = {0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t a = w[i] & 0x7fff7fffu;
-      const uint32_t below1 = low_bits(16 * (s.p1 - 2 * i)), below2 = low_bits(16 * (s.p2 - 2 * i));
-      top[0] = __vmaxs2(top[0], a & below1);
-      top[1] = __vmaxs2(top[1], a & below2 & ~below1);
-      top[2] = __vmaxs2(top[2], a & ~below2);
+      const uint32_t a = w[i] & 0x7fff7fffu, below = low_bits(16 * (s.p1 - 2 * i));
+      top[0] = __vmaxs2(top[0], a & below);
+      top[1] = __vmaxs2(top[1], a & ~below);
+    }
+    if (s.p2 < 8) {  // a short block's end
+      top[1] = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a = w[i] & 0x7fff7fffu;
+        const uint32_t below1 = low_bits(16 * (s.p1 - 2 * i)), below2 = low_bits(16 * (s.p2 - 2 * i));
+        top[1] = __vmaxs2(top[1], a & below2 & ~below1);
+        top[2] = __vmaxs2(top[2], a & ~below2);
+      }
     }
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
