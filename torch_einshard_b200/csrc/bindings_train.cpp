@@ -394,10 +394,11 @@ std::vector<at::Tensor> policy_forward_op(const at::Tensor& logits, const at::Te
   at::Tensor loss = at::empty({}, f32), kl_out = at::empty({}, f32), clipped = at::empty({}, f32);
   at::Tensor logp = at::empty({a.tokens}, f32), terms = at::empty({a.tokens, 4}, f32);
   at::Tensor shares = at::empty({sequences}, f32);
-  at::Tensor sums = at::empty({policy_sum_blocks(a.tokens), 3}, f32.dtype(at::kDouble));
+  at::Tensor sums = at::empty({3 * policy_sum_blocks(a.tokens) + 1}, f32.dtype(at::kDouble));
   PolicyState s = policy_state(terms, shares);
   s.logp = logp.data_ptr<float>();
   s.sums = reinterpret_cast<PolicySums*>(sums.data_ptr<double>());
+  s.done = reinterpret_cast<unsigned*>(sums.data_ptr<double>() + 3 * policy_sum_blocks(a.tokens));
   s.loss = loss.data_ptr<float>();
   s.kl = kl_out.data_ptr<float>();
   s.clipped = clipped.data_ptr<float>();

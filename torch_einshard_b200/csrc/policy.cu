@@ -333,6 +333,7 @@ __global__ void __maxnreg__(kGrad && sizeof(T) == 2 ? 40 : 64)
   const float c = scale_of(a), rest = scale_rest_of(a, c);
   const int threads = static_cast<int>(blockDim.x), tid = static_cast<int>(threadIdx.x);
   const int vocab = static_cast<int>(a.vocab);
+  if (blockIdx.x == 0 && tid == 0) *o.done = 0u;  // for the kernel behind this one
   const long long last = min(a.tokens, (blockIdx.x + 1) * run);
   for (long long t = blockIdx.x * run; t < last; ++t) {
     const T* row = static_cast<const T*>(a.logits) + t * a.ld;
@@ -485,10 +486,11 @@ __device__ __forceinline__ PolicySums terms_of(const PolicyArgs& a, const Policy
   return r;
 }
 
-// Loss, KL and clipped share: a token a thread, every block kRun of them, the only one (kLast) the scalars.
-template <bool kLast>
+// Loss, KL and clipped share: a token a thread, every block kRun of them; the block that is done last adds the
+// blocks' sums in their order.
 __global__ void __launch_bounds__(kRun) policy_sum_kernel(const PolicyArgs a, const PolicyState o) {
   __shared__ PolicySums red[32];
+  __shared__ bool last;
   PolicySums s{0.0, 0.0, 0.0};
   const long long t = static_cast<long long>(blockIdx.x) * kRun + threadIdx.x;
   if (t < a.tokens) {
@@ -501,19 +503,22 @@ __global__ void __launch_bounds__(kRun) policy_sum_kernel(const PolicyArgs a, co
     o.logp[t] = static_cast<float>(lp);
   }
   s = block_total(s, red);
-  if (threadIdx.x != 0) return;
-  if (kLast)
-    store_total(a, o, s);
-  else
+  if (gridDim.x == 1) {
+    if (threadIdx.x == 0) store_total(a, o, s);
+    return;
+  }
+  if (threadIdx.x == 0) {
     o.sums[blockIdx.x] = s;
-}
-
-__global__ void __launch_bounds__(1024) policy_total_kernel(const PolicyArgs a, const PolicyState o, long long blocks) {
-  __shared__ PolicySums red[32];
-  PolicySums s{0.0, 0.0, 0.0};
-  for (long long i = threadIdx.x; i < blocks; i += blockDim.x) {
-    const PolicySums v = o.sums[i];
-    s.loss += v.loss, s.kl += v.kl, s.clipped += v.clipped;
+    __threadfence();
+    last = atomicAdd(o.done, 1u) == gridDim.x - 1;
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  s = {0.0, 0.0, 0.0};
+  for (unsigned i = threadIdx.x; i < gridDim.x; i += kRun) {
+    const double* v = &o.sums[i].loss;
+    s.loss += __ldcg(v), s.kl += __ldcg(v + 1), s.clipped += __ldcg(v + 2);
   }
   s = block_total(s, red);
   if (threadIdx.x == 0) store_total(a, o, s);
@@ -582,14 +587,7 @@ int forward_type(const PolicyArgs& a, const PolicyState& s, cudaStream_t stream,
     policy_rows_kernel<T, true><<<grid, threads, 0, stream>>>(a, s, run);
   else
     policy_rows_kernel<T, false><<<grid, threads, 0, stream>>>(a, s, run);
-  const long long blocks = policy_sum_blocks(a.tokens);
-  if (blocks == 1) {
-    policy_sum_kernel<true><<<1, kRun, 0, stream>>>(a, s);
-  } else {
-    policy_sum_kernel<false><<<static_cast<unsigned>(blocks), kRun, 0, stream>>>(a, s);
-    policy_total_kernel<<<1, 1024, 0, stream>>>(a, s, blocks);
-    ++*launches;
-  }
+  policy_sum_kernel<<<static_cast<unsigned>(policy_sum_blocks(a.tokens)), kRun, 0, stream>>>(a, s);
   return static_cast<int>(cudaGetLastError());
 }
 

@@ -35,6 +35,7 @@ struct PolicyState {
   float4* terms = nullptr;  // [tokens] logit, largest logit, sum of powers, derivative of the loss by logp (without weights)
   float* share = nullptr;   // [sequences] a token's share in the reduction, where the mask decides it
   PolicySums* sums = nullptr;  // [policy_sum_blocks] scratch
+  unsigned* done = nullptr;    // scratch: blocks that are done
   float* loss = nullptr;    // scalars
   float* kl = nullptr;
   float* clipped = nullptr;
