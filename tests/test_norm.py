@@ -187,6 +187,36 @@ def test_rms_with_biases(device):
     check(t, dict(conf, kind="rms"), dh, dn)
 
 
+def without(made, *keys):
+    t, *rest = made
+    return ({k: v for k, v in t.items() if k not in keys}, *rest)
+
+
+ABSENT = [(), ("weight", "bias"), ("bias", "post_bias"), ("post_weight",), ("post_weight", "post_bias"),
+          ("weight", "bias", "post_weight", "post_bias")]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kind", ["layer", "rms"])
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("gate", ["none", "channel", "token"])
+@pytest.mark.parametrize("absent", ABSENT)
+def test_absent_vectors(device, dtype, kind, post, gate, absent):
+    """Columns that a row does not have add nothing, whichever vectors are there: rows that fill a block and rows that
+    do not, aligned and not."""
+    for d in (33, 64, 256, 1000):
+        check(*without(make(device, dtype, (2, 9, d), gate=gate, kind=kind, post=post), *absent))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [512, 2047, 4104, 8191, 8200, 10001, 32776, 65544])
+@pytest.mark.parametrize("absent", [("post_weight",), ("weight", "bias", "post_weight", "post_bias")])
+def test_absent_vectors_of_wide_rows(dtype, d, absent):
+    check(*without(make("cuda", dtype, (2, 21, d), gate="none"), *absent))
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("kind", ["layer", "rms"])
 @pytest.mark.parametrize("d", [64, 37])

@@ -195,12 +195,15 @@ __device__ __forceinline__ float param1(const NormParam& q, long long i, float o
   return q.f32 ? static_cast<const float*>(q.p)[i] : to_float<T>(static_cast<const T*>(q.p)[i]);
 }
 
-// A column vector's elements in fp32, `other` where there is none.
+// A column vector's elements in fp32, `other` where there is none; zero in columns that the row does not have (sums
+// over a row take a vector's elements as they are).
 template <typename T, int kA, int kP>
 __device__ __forceinline__ void param(const NormParam& q, long long offset, float other, Pair (&f)[kP],
                                       const Span& s) {
   if (q.p == nullptr) {
-    fill(f, other);
+    const Pair v = pair(other);
+#pragma unroll
+    for (int i = 0; i < kP; ++i) f[i] = only<kA>(v, i, s);
   } else if (kA != kAny) {
 #pragma unroll
     for (int r = 0; r < kP / 4; ++r) {
