@@ -486,6 +486,52 @@ def test_backward_captured_apart_from_forward(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+def test_forward_and_backward_in_graphs_of_their_own(dtype):
+    """The backward graph's result is its own: a replay of the forward graph leaves it alone, and so does a caller who
+    changes it in place."""
+    t = off_border(make("cuda", dtype, 2, 9, 130), 0.2, 0.2)
+    values = [t.pop("logits")]
+    values.append(torch.randn(values[0].shape, generator=torch.Generator().manual_seed(9)).to(values[0]))
+    z = values[0].clone().requires_grad_(True)
+
+    def gradient(value):
+        leaf = value.clone().requires_grad_(True)
+        return torch.autograd.grad(es.einpolicy("b s v", leaf, axis="v", kl=0.1, **t).loss, leaf)[0]
+
+    want = [gradient(v) for v in values]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    forward, backward = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(forward, stream=side):
+        loss = es.einpolicy("b s v", z, axis="v", kl=0.1, **t).loss
+    with torch.cuda.graph(backward, stream=side):
+        (g,) = torch.autograd.grad(loss, z)
+
+    def replay(i):
+        with torch.no_grad():
+            z.copy_(values[i])
+        forward.replay()
+        backward.replay()
+        torch.cuda.synchronize()
+
+    replay(0)
+    assert torch.equal(g, want[0])
+    with torch.no_grad():
+        z.copy_(values[1])
+    forward.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(g, want[0])
+    backward.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(g, want[1])
+    g.mul_(3)
+    backward.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(g, want[1])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("tokens", [(1, 16385), (4100, 5), (3, 7001)])
 @pytest.mark.parametrize("reduction", ["mean", "sequence", "sum"])
 def test_many_tokens(tokens, reduction):

@@ -4,7 +4,6 @@
 #include "bindings_train.h"
 
 #include <ATen/cuda/CUDAContext.h>
-#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <ATen/core/LegacyTypeDispatch.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -256,6 +255,13 @@ struct Final : public torch::autograd::Function<Final> {
 
 }  // namespace
 
+int64_t capture_of(c10::DeviceIndex device) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(at::cuda::getCurrentCUDAStream(device), &status, &id));
+  return status == cudaStreamCaptureStatusNone ? 0 : static_cast<int64_t>(id);
+}
+
 void finalise(std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& from) {
   if (!at::GradMode::is_enabled()) return;
   for (const at::Tensor& input : from) {
@@ -441,13 +447,9 @@ at::Tensor policy_backward_op(const at::Tensor& grad, const at::Tensor& logits, 
 
 // The forward pass writes the gradient for an upstream gradient of 1 while it has the logits at hand; the first
 // backward pass hands it out (formed again in place where the upstream gradient is another), later ones form their
-// own.  A backward pass captured apart from its forward pass, or the other way round, has its own too: a replay of the
-// one would write under the other's result.
+// own.  A backward pass captured apart from its forward pass (in another graph, or one of the two eager) has its own
+// too: a replay of the one would write under the other's result.
 struct PolicyFunction : public torch::autograd::Function<PolicyFunction> {
-  static bool capturing() {
-    return at::cuda::currentStreamCaptureStatusMayInitCtx() != at::cuda::CaptureStatus::None;
-  }
-
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits,
                                                 const at::Tensor& ids, const Opt& mask, const Opt& old, const Opt& ref,
                                                 const at::Tensor& adv, int64_t length, double lo, double hi, double kl, double temperature, int64_t reduction,
@@ -459,7 +461,7 @@ struct PolicyFunction : public torch::autograd::Function<PolicyFunction> {
     ctx->saved_data["conf"] = c10::ivalue::Tuple::create({length, lo, hi, kl, temperature, reduction, weight});
     ctx->saved_data["kept"] = r[6];
     ctx->saved_data["factors"] = r[7];
-    ctx->saved_data["captured"] = capturing();
+    ctx->saved_data["capture"] = capture_of(logits.get_device());
     ctx->mark_non_differentiable({r[1], r[2], r[3]});
     return {r[0], r[1], r[2], r[3]};
   }
@@ -472,7 +474,7 @@ struct PolicyFunction : public torch::autograd::Function<PolicyFunction> {
     const auto conf = ctx->saved_data["conf"].toTuple()->elements();
     Opt kept, factors;
     if (ctx->saved_data.count("kept")) {
-      if (ctx->saved_data["captured"].toBool() == capturing()) {
+      if (ctx->saved_data["capture"].toInt() == capture_of(s[0].get_device())) {
         kept = ctx->saved_data["kept"].toTensor();
         factors = ctx->saved_data["factors"].toTensor();
       }

@@ -25,6 +25,9 @@ void bind_saved8_ops(pybind11::module_& m, const GemmOps& ops);
 at::Tensor restore8_op(const at::Tensor& codes, const at::Tensor& exps, const c10::optional<at::Tensor>& grad,
                        int64_t dtype, int64_t mode);
 
+// The number of the capture that the device's current stream takes part in (each has its own), or 0.
+int64_t capture_of(c10::DeviceIndex device);
+
 // `grads` as results of `from`, where a graph of the backward pass is wanted: they have no derivatives of their own,
 // using them further raises.
 void finalise(std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& from);
