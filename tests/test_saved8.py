@@ -549,6 +549,31 @@ def test_copies_stay_on_their_stream():
         assert torch.equal(first, want[0]) and torch.equal(second, want[1])
 
 
+@pytest.mark.gpu
+def test_kept_operand_in_two_graphs():
+    """An odd width is read from a copy: each graph makes its own, so they may be replayed in any order."""
+    gen = torch.Generator().manual_seed(14)
+    x, w, _, _, _ = shared_case(torch.bfloat16, "cuda", (2, 64, 127), 3, gen)
+    other = torch.randn(x.shape, generator=gen).to(x)
+    side = torch.cuda.Stream()
+    with torch.no_grad():
+        kept = es.checkpoint8(x)
+        for v in w:
+            es.einshard("b s c, n c -> b s n", es.checkpoint8(x), v)
+        torch.cuda.synchronize()
+        graphs, outs = [], []
+        for v in w:
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=side):
+                outs.append(es.einshard("b s c, n c -> b s n", kept, v))
+        want = [es.einshard("b s c, n c -> b s n", es.checkpoint8(other), v) for v in w]
+        x.copy_(other)
+        for i in (2, 1, 0):
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[i], want[i])
+
+
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("width", [64, 37])
 def test_inside_a_recomputed_block(device, width):

@@ -514,6 +514,7 @@ void bind_training_ops(pybind11::module_& m, std::atomic<long long>& launches) {
   m.def("norm", &norm_op, "norm_forward with gradients", pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("policy", &policy_op, "policy_forward with gradients", pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("policy_forward", &policy_forward_op, "clipped policy loss of token logits, with what its gradient needs");
+  m.def("capture_of", &capture_of, "number of the capture on the device's current stream, or 0");
   m.def("restore8", &restore8_op, "what 8-bit codes stand for, its silu, or grad * silu'");
 }
 

@@ -376,9 +376,10 @@ class _Contraction8(torch.autograd.Function):
 
 
 def _reading(plan, x):
-    """What has to be alike for a contraction to read an earlier one's copy: the matrix, the stream, the capture."""
+    """What has to be alike for a contraction to read an earlier one's copy: the matrix, the stream, the capture (a
+    graph makes the copies that it reads)."""
     return (plan.x_order, plan.gemm[:2], torch.cuda.current_stream(x.device),
-            torch.cuda.is_current_stream_capturing())
+            _native.require().capture_of(x.device.index))
 
 
 def contract_saved(equation, saved, y, activation=None):
