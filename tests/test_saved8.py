@@ -623,6 +623,18 @@ def test_operands_changed_in_place(device):
                     torch.ones(8, 32, dtype=torch.bfloat16, device=device))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+def test_inference_tensors_are_read_as_they_are(device):
+    """They carry no version that would show a change: every product reads the operand itself, not an earlier copy."""
+    with torch.inference_mode():
+        x = torch.randn(2, 8, 37, generator=torch.Generator().manual_seed(15)).to(torch.bfloat16).to(device)
+        w = torch.eye(37, device=device).to(torch.bfloat16)
+        kept = es.checkpoint8(x)
+        assert torch.equal(es.einshard("b s c, n c -> b s n", kept, w), x)
+        x.mul_(2)
+        assert torch.equal(es.einshard("b s c, n c -> b s n", kept, w), x)
+
+
 # ------------------------------------------------------------------ two ranks
 
 def _sharded_models(ctx):

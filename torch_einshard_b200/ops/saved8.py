@@ -407,7 +407,7 @@ def contract_saved(equation, saved, y, activation=None):
             ready = saved._ready[1]
         out = mod.contract8(x, place, y, plan.on_kernels, saved.codes, saved.exps, saved._act, saved._base, order,
                             silu, err, ready)
-        if len(out) > (4 if silu else 1):
+        if len(out) > (4 if silu else 1) and saved._version is not None:  # a copy that a change would be told from
             saved._ready = _reading(plan, x), out[-1]
         if not silu:
             return out[0]
