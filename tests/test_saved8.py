@@ -704,3 +704,23 @@ def _sharded_equations(ctx):
 @pytest.mark.parametrize("body", [_sharded_models, _sharded_equations])
 def test_two_ranks(body):
     run_ranks(body, world_size=2)
+
+
+def _changed_operand(ctx):
+    """Where a plan hands the operand on unchanged, a change since its codes were formed is noticed there too."""
+    mesh = ctx.mesh((2,), ("tp",))
+    gen = torch.Generator().manual_seed(2)
+    x = torch.randn(2, 6, 32, generator=gen).requires_grad_(True)
+    w = torch.randn(16, 32, generator=gen)
+    for formula, v in (("b s c, n c -> b s n/tp", w), ("b s c, n/tp c -> b s n", w[:8])):
+        h = x * 1
+        kept = es.checkpoint8(h)
+        es.einshard(formula, kept, v, mesh=mesh)
+        with torch.no_grad():
+            h.add_(1)
+        with pytest.raises(RuntimeError, match="modified in place"):
+            es.einshard(formula, kept, v, mesh=mesh)
+
+
+def test_changed_operand_on_two_ranks():
+    run_ranks(_changed_operand, world_size=2)

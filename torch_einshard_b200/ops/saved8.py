@@ -143,9 +143,15 @@ class Saved8:
 
     def with_value(self, value):
         """The same codes for a value that differs by its place in the graph alone."""
+        self.check_unchanged()
         if value is self.value:
             return self
         return Saved8(value, self.codes, self.exps, self._act, self._base, self._order)
+
+    def check_unchanged(self):
+        """Raise where the value has been modified in place since its codes were formed."""
+        if self._version is not None and self.value._version != self._version:
+            raise RuntimeError("a Saved8 operand's value has been modified in place since its codes were formed")
 
     def _meta(self):
         return self._act, self._base, self._order, self.value.dtype
@@ -390,8 +396,7 @@ def contract_saved(equation, saved, y, activation=None):
     if y.dtype != x.dtype or y.device != x.device:
         raise ValueError(f"a Saved8 operand of {x.dtype} on {x.device} needs the other one alike, "
                          f"not {y.dtype} on {y.device}")
-    if saved._version is not None and x._version != saved._version:
-        raise RuntimeError("a Saved8 operand's value has been modified in place since its codes were formed")
+    saved.check_unchanged()
     plan = _product(equation, tuple(x.shape), tuple(y.shape))
     silu = activation is not None
     if all(plan.gemm) and gemm.eligible(x, y):
