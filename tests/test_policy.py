@@ -9,6 +9,7 @@ derivatives of the formula, and a gradient is rounded once to the logits' type.
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.distributed as dist
 
 import torch_einshard_b200 as es
@@ -361,6 +362,28 @@ def test_no_second_derivative():
     assert torch.equal(g.detach(), torch.autograd.grad(es.einpolicy("b s v", z, axis="v", **t).loss, z)[0])
     with pytest.raises(RuntimeError, match="twice"):
         torch.autograd.grad(g.sum(), z, allow_unused=True)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("which", ["logits", "old_logp", "ref_logp", "advantages"])
+def test_forward_mode(device, which):
+    """Torch's path carries tangents; the kernels have none and say so."""
+    t = off_border(make(device, torch.float32, 2, 5, 40), 0.2, 0.2)
+    gen = torch.Generator().manual_seed(2)
+    v = torch.randn(t[which].shape, generator=gen).to(t[which])
+    with forward_ad.dual_level():
+        u = {**t, which: forward_ad.make_dual(t[which], v)}
+        z = u.pop("logits")
+        if device == "cuda":
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                es.einpolicy("b s v", z, axis="v", kl=0.1, **u)
+            return
+        tangent = forward_ad.unpack_dual(es.einpolicy("b s v", z, axis="v", kl=0.1, **u).loss).tangent
+        assert tangent is not None
+    if which == "logits":
+        z = t.pop("logits").requires_grad_(True)
+        (g,) = torch.autograd.grad(es.einpolicy("b s v", z, axis="v", kl=0.1, **t).loss, z)
+        assert torch.allclose(tangent, (g * v).sum(), rtol=1e-4, atol=1e-6)
 
 
 @pytest.mark.parametrize("device", DEVICES)

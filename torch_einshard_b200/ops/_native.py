@@ -14,9 +14,10 @@ out records its code in the error word and the kernel returns.
 import os
 
 import torch
+from torch.autograd import forward_ad
 
 __all__ = ["module", "available", "require", "error_word", "check_errors", "reset_errors", "EinshardCommTimeout",
-           "set_wait_timeout_us", "wait_timeout_us"]
+           "set_wait_timeout_us", "wait_timeout_us", "refuse_tangents"]
 
 _state = {"loaded": False, "module": None, "error": None}
 _ERROR_WORDS = {}
@@ -62,6 +63,14 @@ def set_wait_timeout_us(us):
 
 def wait_timeout_us():
     return require().get_wait_timeout_ns() / 1000.0
+
+
+def refuse_tangents(what, *tensors):
+    """Raise where a kernel would drop a tangent (forward-mode differentiation) of one of ``tensors``."""
+    if forward_ad._current_level < 0:
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what} has no forward-mode gradients on the native kernels")
 
 
 def error_word(device) -> torch.Tensor:

@@ -193,7 +193,9 @@ def einpolicy(shard, logits, ids, *, axis, advantages, old_logp=None, ref_logp=N
     args = (rows, _flat(ids.long()), mask, old, ref, adv, conf)
     if not _on_kernels(logits):
         loss, kl_value, clipped, logp = _torch_policy(*args)
-    elif torch.is_grad_enabled() and rows.requires_grad:
+        return PolicyLoss(loss, logp.view(shape), kl_value, clipped)
+    _native.refuse_tangents("einpolicy", logits, adv, old, ref)
+    if torch.is_grad_enabled() and rows.requires_grad:
         loss, kl_value, clipped, logp = _native.require().policy(*args[:-1], *conf)
     else:
         rows = rows.reshape(tokens, vocab)
