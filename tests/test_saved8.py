@@ -9,6 +9,7 @@ accumulation (2^-23 a term at most, which the same product bounds).
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.distributed as dist
 import torch.utils.checkpoint
 from dist_harness import run_ranks
@@ -602,6 +603,22 @@ def test_second_derivatives_are_refused(device):
         for g in (dx, dw):
             with pytest.raises(RuntimeError):
                 torch.autograd.grad((g + 0 * w[0].sum()).sum(), w[0], retain_graph=True)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("which", ["x", "w"])
+@pytest.mark.parametrize("activation", [None, "silu"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(device, which, activation, grad):
+    x, w, _, _, _ = _case(device, torch.bfloat16, 2, 5, 40, 48)
+    x.requires_grad_(grad)
+    with forward_ad.dual_level():
+        if which == "x":
+            x = forward_ad.make_dual(x, torch.ones_like(x))
+        else:
+            w = forward_ad.make_dual(w, torch.ones_like(w))
+        with pytest.raises((NotImplementedError, RuntimeError), match="forward-mode|forward mode|forward AD"):
+            es.einshard("b s c, h c -> b s h", es.checkpoint8(x), w, activation=activation)
 
 
 @pytest.mark.parametrize("device", DEVICES)

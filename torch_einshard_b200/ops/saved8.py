@@ -400,6 +400,7 @@ def contract_saved(equation, saved, y, activation=None):
     plan = _product(equation, tuple(x.shape), tuple(y.shape))
     silu = activation is not None
     if all(plan.gemm) and gemm.eligible(x, y):
+        _native.refuse_tangents("a Saved8 contraction", x, y)
         mod, err = _native.require(), _native.error_word(x.device)
         place = saved._pre
         if place is None and x.requires_grad and torch.is_grad_enabled():
