@@ -17,6 +17,7 @@ from dist_harness import run_ranks
 import torch_einshard_b200 as es
 from torch_einshard_b200.models.tp_mlp import TPMLP
 from torch_einshard_b200.models.transformer import TPTransformer, TransformerConfig
+from torch_einshard_b200.ops.saved8 import silu_saved
 
 cuda = pytest.param("cuda", marks=pytest.mark.gpu)
 DEVICES = ["cpu", cuda]
@@ -299,6 +300,27 @@ def test_activation_layouts_16_bit(order):
     dh = dz.double() * sig * (1 + pre * (1 - sig))
     want = torch.einsum(f"{order.replace(' ', '')},bsc->hc", dh, x.double())
     assert (dw.double() - want).norm() <= 0.02 * want.norm()
+
+
+def same_value(got, want):
+    """Two values of silu in one type: each within half a step of the exact one, and 2^-20 of it from the sigmoid."""
+    far = (torch.finfo(got.dtype).eps + 2.0 ** -19) * want.double().abs() + torch.finfo(got.dtype).smallest_normal
+    return bool(((got.double() - want.double()).abs() <= far).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [64, 40, 37, 5])
+def test_nan_values_stay_in_their_place(device, dtype, width):
+    """The same for the activation of a pre-activation in memory (where a plan's last step is not the product)."""
+    h = (3 * torch.randn(4, 6, width, generator=torch.Generator().manual_seed(13))).to(dtype).to(device)
+    clean = silu_saved(h).value
+    bad = torch.zeros(h.shape, dtype=torch.bool, device=device)
+    bad.flatten()[1::7] = True
+    got = silu_saved(torch.where(bad, float("nan"), h)).value
+    assert torch.isnan(got[bad]).all() and same_value(got[~bad], clean[~bad])
+    up = torch.where(bad, float("inf"), h)
+    assert same_value(silu_saved(up).value[~bad], clean[~bad]) and torch.isinf(silu_saved(up).value[bad]).all()
 
 
 @pytest.mark.parametrize("device", DEVICES)

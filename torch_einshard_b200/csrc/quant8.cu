@@ -77,7 +77,7 @@ __device__ __forceinline__ float decoded(float code, float scale) {
   return kMode == kRestoreValue ? value_of<T>(code, scale) : value_of<float>(code, scale);  // pre-activations: 32 bits
 }
 
-// Two values of different blocks: they share a reciprocal, and a NaN block must not reach the other one.
+// Two values of different blocks, or not from codes: they share a reciprocal, and a NaN must not reach the other one.
 template <typename T, int kMode>
 __device__ __forceinline__ void restored_apart(float& x1, float& x2, float g1, float g2) {
   if (kMode == kRestoreValue) return;
@@ -151,8 +151,13 @@ __global__ void __launch_bounds__(kThreads) quant8_kernel(const T* __restrict__ 
           make_uint2(codes8_of(f[0], f[1], f[2], f[3], s), codes8_of(f[4], f[5], f[6], f[7], s));
       if ((lane & 3) == 0) exps[pl[u].block] = static_cast<uint8_t>(s.byte);
       if (kSilu) {
+        if (s.byte != kQuantNan) {
 #pragma unroll
-        for (int i = 0; i < 8; i += 2) restored2<OutT, kRestoreSilu>(f[i], f[i + 1], 0.0f, 0.0f);
+          for (int i = 0; i < 8; i += 2) restored2<OutT, kRestoreSilu>(f[i], f[i + 1], 0.0f, 0.0f);
+        } else {  // the values themselves: a NaN is one value's
+#pragma unroll
+          for (int i = 0; i < 8; i += 2) restored_apart<OutT, kRestoreSilu>(f[i], f[i + 1], 0.0f, 0.0f);
+        }
         store8(out + pl[u].elem, f);
       }
     }
