@@ -310,6 +310,23 @@ def same_value(got, want):
 
 @pytest.mark.parametrize("device", DEVICES)
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [64, 40, 37])
+def test_nan_columns_stay_in_their_column(device, dtype, width):
+    """A NaN row of the weight is a NaN column of the activation: its neighbours keep their values, whatever they are."""
+    x, w, _, _, _ = _case(device, dtype, 2, 9, 48, width, seed=12)
+    w[1] = 0
+    w[4] *= 100
+    clean = es.einshard("b s c, h c -> b s h", es.checkpoint8(x), w, activation="silu").value
+    bad = [0, 5, 6, 33]
+    w[bad[:2]] = float("nan")
+    w[bad[2:], 3] = float("nan")
+    got = es.einshard("b s c, h c -> b s h", es.checkpoint8(x), w, activation="silu").value
+    fine = [i for i in range(width) if i not in bad]
+    assert torch.isnan(got[..., bad]).all() and same_value(got[..., fine], clean[..., fine])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("width", [64, 40, 37, 5])
 def test_nan_values_stay_in_their_place(device, dtype, width):
     """The same for the activation of a pre-activation in memory (where a plan's last step is not the product)."""

@@ -74,6 +74,7 @@ struct Silu8Epilogue {
       const int col = et.c.n0 + sub * 32;
       if (col >= s.N) break;  // uniform across the warp
       uint32_t r[32];
+      __syncwarp();  // the load is the whole warp's
       tmem_ld32(et.tmem + sub * 32, r);
       tmem_ld_wait();
       if (row >= s.M) continue;
@@ -87,11 +88,20 @@ struct Silu8Epilogue {
       for (int i = 0; i < 8; ++i)
         q[i] = codes8_of(__uint_as_float(r[4 * i]), __uint_as_float(r[4 * i + 1]), __uint_as_float(r[4 * i + 2]),
                          __uint_as_float(r[4 * i + 3]), step);
+      if (step.byte != kQuantNan) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float x1 = __uint_as_float(r[2 * i]), x2 = __uint_as_float(r[2 * i + 1]), s1, s2;
-        sigmoid_pair(x1, x2, s1, s2);
-        w[i] = floats_to_word<T>(x1 * s1, x2 * s2);
+        for (int i = 0; i < 16; ++i) {
+          float x1 = __uint_as_float(r[2 * i]), x2 = __uint_as_float(r[2 * i + 1]), s1, s2;
+          sigmoid_pair(x1, x2, s1, s2);
+          w[i] = floats_to_word<T>(x1 * s1, x2 * s2);
+        }
+      } else {  // a NaN column leaves the one beside it alone
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float x1 = __uint_as_float(r[2 * i]), x2 = __uint_as_float(r[2 * i + 1]), s1, s2;
+          sigmoid_apart(x1, x2, s1, s2);
+          w[i] = floats_to_word<T>(x1 * s1, x2 * s2);
+        }
       }
       int8_t* code_row = kept.codes + at * kept.pitch + col;
       T* out_row = out + at * kept.pitch + col;
@@ -153,6 +163,7 @@ struct Silu8GradEpilogue {
       const int col = et.c.n0 + sub * 32;
       if (col >= s.N) break;  // uniform across the warp
       uint32_t r[32];
+      __syncwarp();  // the load is the whole warp's
       tmem_ld32(et.tmem + sub * 32, r);
       tmem_ld_wait();
       if (row >= s.M) continue;

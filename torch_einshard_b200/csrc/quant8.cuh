@@ -81,8 +81,8 @@ __device__ __forceinline__ float exp2_approx(float x) {
 
 // Sigmoids of two values with one reciprocal, s1 = e2' / (e1' e2') with
 // e' = 1 + e^-x.  Below -43, where silu is under 10^-17, x is taken as -43: the
-// product of the two stays in range.  (A NaN makes both NaN; NaN blocks are NaN
-// whole.)  For results of 16 bits.
+// product of the two stays in range.  (A NaN makes both NaN: for what codes stand
+// for, where NaN blocks are NaN whole.)  For results of 16 bits.
 __device__ __forceinline__ void sigmoid_pair(float& x1, float& x2, float& s1, float& s2) {
   x1 = max_nan(x1, -43.0f);
   x2 = max_nan(x2, -43.0f);
@@ -91,6 +91,16 @@ __device__ __forceinline__ void sigmoid_pair(float& x1, float& x2, float& s1, fl
   const float r = __fdividef(1.0f, e1 * e2);
   s1 = r * e2;
   s2 = r * e1;
+}
+
+// The same of values that may be NaN each by itself.
+__device__ __forceinline__ void sigmoid_apart(float& x1, float& x2, float& s1, float& s2) {
+  const bool bad1 = x1 != x1, bad2 = x2 != x2;
+  if (bad1) x1 = 0.0f;
+  if (bad2) x2 = 0.0f;
+  sigmoid_pair(x1, x2, s1, s2);
+  if (bad1) x1 = __uint_as_float(0x7fc00000u);
+  if (bad2) x2 = __uint_as_float(0x7fc00000u);
 }
 
 __device__ __forceinline__ float silu_slope(float x, float s) { return s * fmaf(x, 1.0f - s, 1.0f); }
