@@ -165,6 +165,30 @@ def test_gates(device, kind, post, gate, shape):
     check(*make(device, torch.float32, shape, gate=gate, kind=kind, post=post))
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize("post", [False, True])
+@pytest.mark.parametrize("gate", list(GATES))
+@pytest.mark.parametrize("shape", [(3, 20, 96), (2, 16, 41), (5, 1, 64), (1, 24, 64)])
+def test_gates_of_16_bits(device, dtype, post, gate, shape):
+    """A gate's gradient is summed in 32 bits, over the normalised axis too, and rounded once."""
+    check(*make(device, dtype, shape, gate=gate, post=post))
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES[:2])
+def test_gate_of_16_bits_over_separated_axes(device, dtype):
+    gen = torch.Generator().manual_seed(0)
+    x, y, g = (torch.randn(*s, generator=gen).to(dtype).to(device).requires_grad_(True)
+               for s in ((2, 33, 4, 16), (2, 33, 4, 16), (4, 2, 16)))
+    h, _ = es.einnorm("b s h d", x, y, axis="d", gate=g, gate_axes="h b d")
+    dh = torch.randn(h.shape, generator=gen).to(dtype).to(device)
+    (got,) = torch.autograd.grad(h, g, dh)
+    terms = (dh.double() * y.detach().double()).cpu()
+    # 33 products and additions in 32 bits, one rounding
+    close(got, terms.sum(1).permute(1, 0, 2), terms.abs().sum(1).permute(1, 0, 2), 33)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", [(1, 5000), (7, 700), (300, 3), (40, 16)])
 @pytest.mark.parametrize("gate", ["channel", "batch", "token", "seq"])

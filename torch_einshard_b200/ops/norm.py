@@ -144,6 +144,9 @@ def _check_param(t, x, name):
 
 
 def _gate_rows(gate, plan):
+    if plan.spread or plan.run is not None:
+        # written out below: autograd sums the written-out rows' gradients, 32-bit ones, and rounds the sum once
+        gate = gate.to(torch.promote_types(gate.dtype, torch.float32))
     if plan.spread:
         gate = gate.unsqueeze(-1).expand(*gate.shape, plan.d)
     if plan.order is not None:
