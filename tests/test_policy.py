@@ -267,6 +267,28 @@ def test_bad_ids_and_logits_are_not_hidden(device):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+def test_bad_tokens_without_advantage(device):
+    """An advantage of 0 weighs nothing, but an id outside the vocabulary or a NaN logit still shows."""
+    t = make(device, torch.float32, 2, 4, 12)
+    t["mask"][:] = True
+    t["advantages"][1] = 0
+    for fault in ("id", "logit"):
+        ids, z = t["ids"].clone(), t["logits"].clone()
+        if fault == "id":
+            ids[1, 2] = 12
+        else:
+            z[1, 2, 3] = float("nan")
+        z.requires_grad_(True)
+        for old in (t["old_logp"], None):
+            r = es.einpolicy("b s v", z, ids, axis="v", advantages=t["advantages"], old_logp=old, mask=t["mask"])
+            assert torch.isnan(r.loss) and torch.isnan(r.logp[1, 2]) and torch.isfinite(r.logp[0]).all()
+    # a ratio past 32 bits times 0 is 0
+    r = es.einpolicy("b s v", t["logits"], t["ids"], axis="v", advantages=0 * t["advantages"],
+                     old_logp=t["old_logp"] - 200, mask=t["mask"])
+    assert float(r.loss) == 0
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_axes_and_strides(device):
     t = off_border(make(device, torch.float32, 3, 5, 41), 0.2, 0.2)
     args = dict(advantages=t["advantages"], old_logp=t["old_logp"], ref_logp=t["ref_logp"], mask=t["mask"], kl=0.1)

@@ -253,7 +253,7 @@ __device__ __forceinline__ float slope_of(const PolicyArgs& a, const Inputs& in,
   const float ratio = expf(lp - (a.old != nullptr ? in.old : lp));
   const float kept = fminf(fmaxf(ratio, static_cast<float>(a.least)), static_cast<float>(a.most));
   const float s1 = ratio * in.adv;
-  float slope = in.adv == 0.0f || s1 > kept * in.adv ? 0.0f : -s1;
+  float slope = (in.adv == 0.0f && lp == lp) || s1 > kept * in.adv ? 0.0f : -s1;  // a NaN stays
   if (a.ref != nullptr) slope -= a.kl * expm1f(in.ref - lp);
   return slope;
 }
@@ -476,7 +476,7 @@ __device__ __forceinline__ PolicySums terms_of(const PolicyArgs& a, const Policy
   const double adv = a.adv[a.adv_per_sequence ? sequence_of(a, t) : t];
   const double s1 = ratio * adv, s2 = fmin(fmax(ratio, a.least), a.most) * adv;
   PolicySums r{0.0, 0.0, s1 > s2 ? 1.0 : 0.0};
-  if (adv != 0.0) r.loss = s1 > s2 ? -s2 : -s1;
+  if (adv != 0.0 || lp != lp) r.loss = s1 > s2 ? -s2 : -s1;  // a NaN stays
   if (a.ref != nullptr) {
     const double away = a.ref[t] - lp;
     r.kl = expm1(away) - away;

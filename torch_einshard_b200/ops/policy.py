@@ -76,7 +76,7 @@ def _torch_policy(logits, ids, mask, old, ref, adv, conf):
     adv = kept(adv if adv.shape[0] == tokens else adv.repeat_interleave(length))
     ratio = torch.exp(lp - (lp.detach() if old is None else torch.where(keep, old.to(wide), lp.detach())))
     clip = ratio.clamp(1 - low, 1 + high)
-    gain = torch.where(adv == 0, 0, torch.minimum(ratio * adv, clip * adv))
+    gain = torch.where((adv == 0) & ~torch.isnan(lp), 0, torch.minimum(ratio * adv, clip * adv))
     clipped = (ratio * adv > clip * adv).to(wide)
     if ref is None:
         kl = torch.zeros_like(lp)
