@@ -230,15 +230,15 @@ struct ContractNode : public Node {
 
   variable_list apply(variable_list&& grads) override {
     const std::lock_guard<std::mutex> held(lock);
-    variable_list out(3);
+    variable_list out(2);  // of the place, of y
     const bool any = grads[0].defined() || (silu && grads[1].defined());
     if (!any) return out;
     const at::Tensor yv = y.unpack(), c = codes.unpack(), e = exps.unpack();
     const c10::cuda::CUDAGuard guard(yv.device());
     ReadersNode* readers = nullptr;
-    const bool want_place = task_should_compute_output(1);
-    if (want_place) readers = dynamic_cast<ReadersNode*>(next_edge(1).function.get());
-    std::vector<at::Tensor> found(3);
+    const bool want_place = task_should_compute_output(0);
+    if (want_place) readers = dynamic_cast<ReadersNode*>(next_edge(0).function.get());
+    std::vector<at::Tensor> found(2);
     {
       const at::AutoDispatchBelowAutograd below;
       at::Tensor grad = grads[0];
@@ -254,16 +254,12 @@ struct ContractNode : public Node {
       } else if (want_place && same_rows(c)) {
         // (dz y^T) silu'(h^) and silu(h^) from one product
         const auto both = g_ops.silu_grad(gz, prepared(yt), c, e, err);
-        found[1] = plan->x_of(both[0]);
+        found[0] = plan->x_of(both[0]);
         x = both[1];
-      } else if (want_place || task_should_compute_output(0)) {
-        const at::Tensor dx = plan->x_of(g_ops.product(gz, prepared(yt), err));
-        if (want_place)
-          found[1] = through_silu(dx, c, e, kept.order);
-        else
-          found[0] = dx;
+      } else if (want_place) {
+        found[0] = through_silu(plan->x_of(g_ops.product(gz, prepared(yt), err)), c, e, kept.order);
       }
-      if (task_should_compute_output(2)) {
+      if (task_should_compute_output(1)) {
         if (!x.defined()) {
           const auto restore = [&] { return prepared(plan->operand_x(restored(c, e))); };
           x = readers == nullptr ? restore() : readers->operand(plan, restore);
@@ -272,12 +268,12 @@ struct ContractNode : public Node {
         const bool turned = y3.stride(1) == 1 && y3.size(1) > 1;
         at::Tensor dy = turned ? g_ops.product(prepared(gz.transpose(1, 2)), x, err).transpose(1, 2)
                                : g_ops.product(prepared(x.transpose(1, 2)), gz, err);
-        found[2] = moved(dy.reshape(plan->y_shape), plan->y_back);
+        found[1] = moved(dy.reshape(plan->y_shape), plan->y_back);
       }
     }
     finalise(found, grads);
     finalise(found, {yv});
-    for (size_t i = 0; i < 3; ++i) out[i] = found[i];
+    for (size_t i = 0; i < 2; ++i) out[i] = found[i];
     return out;
   }
 
@@ -301,7 +297,7 @@ at::Tensor readers_of(const at::Tensor& x, const at::Tensor& err) {
   return place;
 }
 
-// The contraction of x, whose gradient goes to `place` where there is one (a pre-activation's place, or readers_of),
+// The contraction of x, whose gradient goes to `place` (a pre-activation's place, or readers_of; none: it has none),
 // with y: (z), or with `silu` (silu(z), its pre-activation's place, codes and exponents).  `ready` is x's matrix as an
 // earlier contraction read it; where that takes a copy, the matrix is the last result.
 std::vector<at::Tensor> contract8(const at::Tensor& x, const Opt& place, const at::Tensor& y,
@@ -330,11 +326,10 @@ std::vector<at::Tensor> contract8(const at::Tensor& x, const Opt& place, const a
       out = {plan->result(g_ops.product(xv, yv, err).contiguous())};
     }
   }
-  const at::Tensor from = place.has_value() ? at::Tensor() : x;
   const at::Tensor at = place.has_value() ? *place : at::Tensor();
-  if (!torch::autograd::compute_requires_grad(from, at, y)) return results();
+  if (!torch::autograd::compute_requires_grad(at, y)) return results();
   auto node = std::shared_ptr<ContractNode>(new ContractNode(), torch::autograd::deleteNode);
-  node->set_next_edges(torch::autograd::collect_next_edges(from, at, y));
+  node->set_next_edges(torch::autograd::collect_next_edges(at, y));
   node->plan = plan;
   node->y = SavedVariable(y, false);
   node->codes = SavedVariable(codes, false);

@@ -332,7 +332,7 @@ class _Contraction8(torch.autograd.Function):
     ``x`` carries the values.  Its gradient goes to ``place`` (``x`` is detached
     then): its pre-activation's place in the graph where x is a silu, and with a
     ``box`` the place where its contractions' gradients meet.  Without a place it
-    goes to ``x``.  With ``silu`` the result is silu(x y), its pre-activation in
+    has none.  With ``silu`` the result is silu(x y), its pre-activation in
     8 bits and that one's place."""
 
     @staticmethod
@@ -366,19 +366,17 @@ class _Contraction8(torch.autograd.Function):
             grad = grad_pre if grad is None else grad + grad_pre
         if grad is None:
             return (None,) * 9
-        want_x, want_place, _, want_y = ctx.needs_input_grad[:4]
-        dx = dplace = dy = None
+        want_place, _, want_y = ctx.needs_input_grad[1:4]
+        dplace = dy = None
         if ctx.box is not None:
             if torch._C._will_engine_execute_node(ctx.next_functions[1][0]):  # the operand's gradient is asked for
                 ctx.box.setdefault(torch._C._current_graph_task_id(), []).append((ctx.equation, grad, y))
-        elif want_x or want_place:
-            dx = _operand_grad(ctx.equation, grad, y)
-            if want_place:
-                dx, dplace = None, _silu_grad(dx, codes, exps, ctx.meta[2])
+        elif want_place:
+            dplace = _silu_grad(_operand_grad(ctx.equation, grad, y), codes, exps, ctx.meta[2])
         if want_y:
             (ex, ey), ez = ctx.equation.split("->")[0].split(","), ctx.equation.split("->")[1]
             dy = contract(f"{ez},{ex}->{ey}", grad, _restore_operand(codes, exps, ctx.meta))
-        return dx, dplace, None, dy, None, None, None, None, None
+        return None, dplace, None, dy, None, None, None, None, None
 
 
 def _reading(plan, x):
