@@ -349,6 +349,25 @@ def test_axes_strides_and_offsets(device):
         assert torch.allclose(a, b, atol=1e-6)
 
 
+def negated(t):
+    """-t as a view that only says so (what the imaginary part of a conjugate is)."""
+    return torch._neg_view(t.detach())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_negated_views(device):
+    """Inputs and gradients whose sign is kept beside their memory."""
+    t, conf, dh, dn = make(device, torch.float32, (2, 9, 40), gate="batch")
+    minus = {k: (-v.detach()).requires_grad_(True) for k, v in t.items()}
+    views = {k: negated(v).requires_grad_(True) for k, v in t.items()}
+    want = run(minus, conf)
+    want = (*want, *torch.autograd.grad(want, list(minus.values()), (-dh, -dn)))
+    got = run(views, conf)
+    got = (*got, *torch.autograd.grad(got, list(views.values()), (negated(dh), negated(dn))))
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_gate_over_separated_axes(device):
     """A gate that skips an axis between its own (b h of b s h d)."""

@@ -276,6 +276,10 @@ namespace {
 Opt some(const at::Tensor& t) { return t.defined() ? Opt(t) : Opt(); }
 at::Tensor none(const Opt& t) { return t.has_value() ? *t : at::Tensor(); }
 
+// The kernels read raw memory: a view that only says it is negated is written out.
+at::Tensor plain(const at::Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+Opt plain(const Opt& t) { return t.has_value() ? Opt(plain(*t)) : t; }
+
 // [rows, d] of a tensor whose last axis is the row, with a unit stride.
 at::Tensor rows_of(const at::Tensor& t) {
   if (!t.defined()) return t;
@@ -294,7 +298,7 @@ struct NormFunction : public torch::autograd::Function<NormFunction> {
     ctx->set_materialize_grads(false);
     ctx->save_for_backward({x, none(y), none(w), none(b), none(pw), none(pb), none(gate), *out[2]});
     ctx->saved_data["conf"] = c10::ivalue::Tuple::create({inner, count, post, center, scale, eps});
-    at::AutoDispatchBelowADInplaceOrView plain;  // results of their own, not views
+    at::AutoDispatchBelowADInplaceOrView own;  // results of their own, not views
     if (!y.has_value()) return {out[1]->view(x.sizes())};
     return {out[0]->view(x.sizes()), out[1]->view(x.sizes())};
   }
@@ -313,8 +317,10 @@ struct NormFunction : public torch::autograd::Function<NormFunction> {
     {
       at::AutoDispatchBelowAutograd below;
       const at::Tensor xr = rows_of(s[0]), yr = rows_of(s[1]);
-      auto plain = [&](const at::Tensor& g) { return g.defined() ? Opt(g.reshape(xr.sizes()).contiguous()) : Opt(); };
-      auto got = norm_backward_op(plain(dh), plain(dn), xr, some(yr), some(s[2]), some(s[3]), some(s[4]),
+      auto whole = [&](const at::Tensor& g) {
+        return g.defined() ? Opt(plain(g).reshape(xr.sizes()).contiguous()) : Opt();
+      };
+      auto got = norm_backward_op(whole(dh), whole(dn), xr, some(yr), some(s[2]), some(s[3]), some(s[4]),
                                   some(s[5]), some(s[6]), conf[0].toInt(), conf[1].toInt(), conf[2].toBool(),
                                   conf[3].toBool(), conf[4].toDouble(), conf[5].toDouble(), s[7], want);
       for (size_t i = 0; i < 7; ++i) {
@@ -333,7 +339,8 @@ struct NormFunction : public torch::autograd::Function<NormFunction> {
 std::vector<at::Tensor> norm_op(const at::Tensor& x, const Opt& y, const Opt& w, const Opt& b, const Opt& pw,
                                 const Opt& pb, const Opt& gate, int64_t inner, int64_t count, bool post, bool center,
                                 double scale, double eps) {
-  return NormFunction::apply(x, y, w, b, pw, pb, gate, inner, count, post, center, scale, eps);
+  return NormFunction::apply(plain(x), plain(y), plain(w), plain(b), plain(pw), plain(pb), plain(gate), inner, count,
+                             post, center, scale, eps);
 }
 
 // ------------------------------------------------------------------ policy loss
