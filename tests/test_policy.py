@@ -288,6 +288,29 @@ def test_bad_tokens_without_advantage(device):
     assert float(r.loss) == 0
 
 
+def negated(t):
+    """-t as a view that only says so (what the imaginary part of a conjugate is)."""
+    return torch._neg_view(t.detach())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_negated_views(device):
+    """Inputs and gradients whose sign is kept beside their memory."""
+    t = off_border(make(device, torch.float32, 2, 9, 40), 0.2, 0.2)
+    results = []
+    for sign in (torch.neg, negated):
+        u = {k: sign(-v) if v.is_floating_point() else v for k, v in t.items()}
+        z = u.pop("logits").detach().requires_grad_(True)
+        for upstream in (torch.ones((), device=device), sign(torch.ones((), device=device))):
+            r = es.einpolicy("b s v", z, axis="v", kl=0.1, **u)
+            results.append([r.loss.detach(), r.logp, torch.autograd.grad(r.loss, z, upstream)[0]])
+        with torch.no_grad():
+            results[-1].append(es.einpolicy("b s v", z, axis="v", kl=0.1, **u).loss)
+    for got, want in zip(results[2:], results[:2]):
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_axes_and_strides(device):
     t = off_border(make(device, torch.float32, 3, 5, 41), 0.2, 0.2)

@@ -491,7 +491,7 @@ struct PolicyFunction : public torch::autograd::Function<PolicyFunction> {
     std::vector<at::Tensor> found(1);
     {
       at::AutoDispatchBelowAutograd below;
-      found[0] = policy_backward_op(grads[0].contiguous(), rows_of(s[0]), s[1], some(s[2]), some(s[3]), some(s[4]), s[5],
+      found[0] = policy_backward_op(plain(grads[0]).contiguous(), rows_of(s[0]), s[1], some(s[2]), some(s[3]), some(s[4]), s[5],
                                     conf[0].toInt(), conf[1].toDouble(), conf[2].toDouble(), conf[3].toDouble(),
                                     conf[4].toDouble(), conf[5].toInt(), conf[6].toDouble(), s[6], s[7], kept,
                                     factors)

@@ -127,7 +127,7 @@ def _token_input(t, name, shapes, logits):
         raise ValueError(f"{name} must have the shape {' or '.join(str(s) for s in shapes)}, not {tuple(t.shape)}")
     if t.requires_grad:
         raise ValueError(f"{name} is a constant of the loss: detach it")
-    return _flat(t.to(torch.float64 if logits.dtype == torch.float64 else torch.float32))
+    return _flat(t.to(torch.float64 if logits.dtype == torch.float64 else torch.float32).resolve_neg())
 
 
 def _flat(t):
@@ -186,7 +186,8 @@ def einpolicy(shard, logits, ids, *, axis, advantages, old_logp=None, ref_logp=N
     if tokens == 0:
         zero = logits.detach().new_zeros((), dtype=torch.promote_types(logits.dtype, torch.float32))
         return PolicyLoss(logits.sum(dtype=zero.dtype), zero.expand(shape), zero, zero)
-    rows = logits if place == len(shape) else logits.movedim(place, -1)
+    rows = logits.resolve_neg()  # the kernels read raw memory
+    rows = rows if place == len(shape) else rows.movedim(place, -1)
     mask = None if mask is None else _flat(mask)
     conf = (max(shape[-1], 1) if shape else 1, float(low), float(high), float(kl), float(temperature),
             _REDUCTIONS[reduction], float(weight))
