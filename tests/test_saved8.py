@@ -257,6 +257,32 @@ def test_gradients_against_differences(device):
             assert float(grad.flatten()[i]) == float((f(*args[0]) - f(*args[1])) / 2)
 
 
+def negated(t):
+    """-t as a view that only says so (what the imaginary part of a conjugate is)."""
+    return torch._neg_view(t.detach())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("width", [40, 37])
+def test_negated_views(device, dtype, width):
+    """Operands and gradients whose sign is kept beside their memory."""
+    x, w1, w2, dy, da = _case(device, dtype, 2, 6, width, 48, seed=16)
+    results = []
+    for sign in (torch.neg, negated):
+        u = [sign(-t).detach().requires_grad_(True) for t in (x, w1, w2)]
+        kept = es.checkpoint8(u[0])
+        a = es.einshard("b s c, h c -> b s h", kept, u[1], activation="silu")
+        y = es.einshard("b s h, c h -> b s c", a, u[2])
+        z = es.einshard("b s c, h c -> b s h", kept, u[1])
+        s = silu_saved(z)
+        grads = torch.autograd.grad((y, z, a.value, s.value), u, tuple(sign(t) for t in (dy, da, da, da)))
+        results.append([kept.restore(), y.detach(), z.detach(), s.value.detach(), s.restore(), *grads,
+                        silu_saved(sign(da)).value])
+    for got, want in zip(*results):
+        assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("device", DEVICES)
 def test_axis_orders_and_ellipsis(device):
     x, w, _, _, _ = _case(device, torch.float32, 2, 6, 40, 48, seed=7)

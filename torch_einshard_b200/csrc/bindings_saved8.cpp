@@ -241,9 +241,9 @@ struct ContractNode : public Node {
     std::vector<at::Tensor> found(2);
     {
       const at::AutoDispatchBelowAutograd below;
-      at::Tensor grad = grads[0];
+      at::Tensor grad = plain(grads[0]);
       if (grad.defined() && silu) grad = through_silu(grad, h_codes.unpack(), h_exps.unpack(), plan->z_order);
-      if (silu && grads[1].defined()) grad = grad.defined() ? grad + grads[1] : grads[1];
+      if (silu && grads[1].defined()) grad = grad.defined() ? grad + grads[1] : plain(grads[1]);
       const at::Tensor gz = prepared(plan->product_of(grad));
       const at::Tensor y3 = plan->operand_y(yv), yt = y3.transpose(1, 2);
       at::Tensor x;  // the operand, for dy

@@ -262,6 +262,8 @@ int64_t capture_of(c10::DeviceIndex device) {
   return status == cudaStreamCaptureStatusNone ? 0 : static_cast<int64_t>(id);
 }
 
+at::Tensor plain(const at::Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
 void finalise(std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& from) {
   if (!at::GradMode::is_enabled()) return;
   for (const at::Tensor& input : from) {
@@ -276,9 +278,7 @@ namespace {
 Opt some(const at::Tensor& t) { return t.defined() ? Opt(t) : Opt(); }
 at::Tensor none(const Opt& t) { return t.has_value() ? *t : at::Tensor(); }
 
-// The kernels read raw memory: a view that only says it is negated is written out.
-at::Tensor plain(const at::Tensor& t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
-Opt plain(const Opt& t) { return t.has_value() ? Opt(plain(*t)) : t; }
+Opt plain_opt(const Opt& t) { return t.has_value() ? Opt(plain(*t)) : t; }
 
 // [rows, d] of a tensor whose last axis is the row, with a unit stride.
 at::Tensor rows_of(const at::Tensor& t) {
@@ -339,8 +339,8 @@ struct NormFunction : public torch::autograd::Function<NormFunction> {
 std::vector<at::Tensor> norm_op(const at::Tensor& x, const Opt& y, const Opt& w, const Opt& b, const Opt& pw,
                                 const Opt& pb, const Opt& gate, int64_t inner, int64_t count, bool post, bool center,
                                 double scale, double eps) {
-  return NormFunction::apply(plain(x), plain(y), plain(w), plain(b), plain(pw), plain(pb), plain(gate), inner, count,
-                             post, center, scale, eps);
+  return NormFunction::apply(plain(x), plain_opt(y), plain_opt(w), plain_opt(b), plain_opt(pw), plain_opt(pb),
+                             plain_opt(gate), inner, count, post, center, scale, eps);
 }
 
 // ------------------------------------------------------------------ policy loss

@@ -28,6 +28,9 @@ at::Tensor restore8_op(const at::Tensor& codes, const at::Tensor& exps, const c1
 // The number of the capture that the device's current stream takes part in (each has its own), or 0.
 int64_t capture_of(c10::DeviceIndex device);
 
+// The kernels read raw memory: a view that only says it is negated is written out.
+at::Tensor plain(const at::Tensor& t);
+
 // `grads` as results of `from`, where a graph of the backward pass is wanted: they have no derivatives of their own,
 // using them further raises.
 void finalise(std::vector<at::Tensor>& grads, const std::vector<at::Tensor>& from);

@@ -176,6 +176,7 @@ def checkpoint8(x):
         raise ValueError("checkpoint8 needs at least one axis")
     if x.dtype not in (torch.bfloat16, torch.float16, torch.float32, torch.float64):
         raise TypeError(f"checkpoint8 takes a floating-point tensor, not {x.dtype}")
+    x = x.resolve_neg()  # the kernels read raw memory
     codes, exps = _quantise(_rows(x.detach()))
     return Saved8(x, codes, exps)
 
@@ -261,7 +262,7 @@ def _silu_forward(h, dtype):
 
 def _silu_grad(grad, codes, exps, order):
     """grad * silu'(h^), in grad's axes; ``order`` leads from the quantised tensor's axes to them."""
-    g = _moved(grad, None if order is None else _inverse(order))
+    g = _moved(grad.resolve_neg(), None if order is None else _inverse(order))
     d = _restored(codes, exps, grad.dtype, _SILU_GRAD, g.reshape(codes.shape).contiguous()).view(g.shape)
     return _moved(d, order)
 
@@ -395,6 +396,7 @@ def contract_saved(equation, saved, y, activation=None):
         raise ValueError(f"a Saved8 operand of {x.dtype} on {x.device} needs the other one alike, "
                          f"not {y.dtype} on {y.device}")
     saved.check_unchanged()
+    y = y.resolve_neg()
     plan = _product(equation, tuple(x.shape), tuple(y.shape))
     silu = activation is not None
     if all(plan.gemm) and gemm.eligible(x, y):
@@ -436,6 +438,7 @@ class _SiluSaved(torch.autograd.Function):
     def forward(ctx, h):
         wide = torch.promote_types(h.dtype, torch.float32)
         ctx.set_materialize_grads(False)
+        h = h.resolve_neg()
         a, codes, exps = _silu_forward((_rows(h) if h.dim() else h.view(1, 1)).to(wide), h.dtype)
         ctx.save_for_backward(codes, exps)
         ctx.mark_non_differentiable(codes, exps)
