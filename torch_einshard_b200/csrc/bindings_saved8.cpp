@@ -119,7 +119,8 @@ struct Pass {
 };
 
 // The place where the gradients of an operand's contractions meet.  A backward pass is known by its number: passes
-// over one graph (again, or from two threads) do not meet.
+// over one graph (again, or from two threads) do not meet.  What a pass has brought when it raises stays until the
+// graph goes.
 struct ReadersNode : public Node {
   std::mutex lock;
   std::map<int, Pass> passes;

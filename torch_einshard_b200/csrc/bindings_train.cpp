@@ -455,7 +455,8 @@ at::Tensor policy_backward_op(const at::Tensor& grad, const at::Tensor& logits, 
 // The forward pass writes the gradient for an upstream gradient of 1 while it has the logits at hand; the first
 // backward pass hands it out (formed again in place where the upstream gradient is another), later ones form their
 // own.  A backward pass captured apart from its forward pass (in another graph, or one of the two eager) has its own
-// too: a replay of the one would write under the other's result.
+// too: a replay of the one would write under the other's result.  The buffer is no saved tensor: hooks that recompute
+// or offload saved tensors do not see it.
 struct PolicyFunction : public torch::autograd::Function<PolicyFunction> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits,
                                                 const at::Tensor& ids, const Opt& mask, const Opt& old, const Opt& ref,

@@ -32,7 +32,7 @@
 // Measured, forward / backward with the finishing pass: 8192 rows of 2048 bf16
 // (layer, both norms, a gate a channel) 31 / 67 us, 4.4 and 3.0 TB/s of what has to
 // move; 16387 rows of 8192 (rms, a gate a sequence) 232 / 320 us, 4.6 and 5.0 TB/s;
-// 5331 rows of 1001 fp32, not aligned (layer, a gate a token) 29 / 54 us.  A
+// 5331 rows of 1001 fp32, not aligned (layer, a gate a token) 31 / 55 us.  A
 // division a row to find its gate's row cost 8 % of the second.  What is
 // left is the time between a row's last load and its reductions' results: with 16
 // elements a thread an SM has one to four rows at work.

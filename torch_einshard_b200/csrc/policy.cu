@@ -463,7 +463,10 @@ __device__ __forceinline__ void store_total(const PolicyArgs& a, const PolicySta
 
 // A token's terms from what its row left, in 64 bits: terms of both signs cancel in the loss, and what 32 bits lose
 // in a log-probability has one sign for all tokens (over 12288 tokens a sum was off by 3e-5, and is by 3e-6 like this).
-// kExpLow is what the row's exponentials are too small by on the average, measured over whole powers of two.
+// kExpLow is what the row's exponentials are too small by on the average, measured over whole powers of two: a row
+// that one logit dominates has that logit's own error instead (a token that is certain reads up to 6e-8 below 0).  The
+// row kernel's slope is formed in 32 bits without it: within 2^-20 or so of a clip border the loss and the clipped
+// share may take one side and the gradient the other.
 __device__ __forceinline__ PolicySums terms_of(const PolicyArgs& a, const PolicyState& o, long long t, double* logp) {
   constexpr double kExpLow = 5.05e-8;
   const float4 row = o.terms[t];  // logit, largest logit, sum

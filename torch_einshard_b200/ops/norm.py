@@ -9,8 +9,10 @@ For a residual stream ``x`` and a block's output ``y`` over named axes,
 in one pass over x and y (``csrc/norm.cu``), and one for the gradients of all of
 them.  ``kind`` is "layer" (mean and variance) or "rms".  The gate has its own
 axes: a vector of the normalised axis, a row for every batch entry, one for
-every token, a scalar; its gradient is summed over the axes it lacks.  The
-statistics, h before its norm and all sums are 32-bit; h and n are rounded
+every token, a scalar; its gradient is summed over the axes it lacks.  (A gate
+without the normalised axis, or with axes of the stream between its own, is
+written out to rows in 32 bits, and so is its gradient before it is summed.)
+The statistics, h before its norm and all sums are 32-bit; h and n are rounded
 once, and n is the norm of h before that rounding.
 
 Every axis but the normalised one may be sharded (the operation is local to a
