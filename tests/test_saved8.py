@@ -233,6 +233,36 @@ def check_mlp(device, dtype, shape, transposed):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("odd", [0, 5])
+def test_slope_of_large_pre_activations(device, dtype, odd):
+    """silu' far from 0 is 1 or 0: 1 - sigmoid has no error of its own there that x could multiply.  Blocks with large
+    values at their ends beside blocks of small ones; the gradient is one product with 1 (and zeros), rounded to the
+    type once or, behind the second product, twice."""
+    gen = torch.Generator().manual_seed(17)
+    sizes = [3.0, 12.0, 40.0, 300.0, 5e3, 2.0 ** 15] + ([1e6, 1e12, 1e30] if dtype != torch.float16 else [])
+    values = torch.tensor([s * sign for s in sizes for sign in (1, -1)], dtype=torch.float64)
+    width = 64 * len(values) + odd
+    x = torch.randn(8, width, generator=gen).double()
+    for i, v in enumerate(values):
+        x[:, 64 * i:64 * i + 32] *= 0.004 * v.abs()
+        x[:, 64 * i] = x[:, 64 * i + 31] = v
+    x = x.to(dtype).to(device).requires_grad_(True)
+    w = torch.eye(width, dtype=dtype, device=device)
+    a = es.einshard("b c, h c -> b h", es.checkpoint8(x), w, activation="silu")
+    y = es.einshard("b h, c h -> b c", a, w)
+    kept = a.codes.double().cpu() * torch.exp2(a.exps.cpu().double().repeat_interleave(32, 1)[:, :width] - 127)
+    s, rest = torch.sigmoid(kept), torch.sigmoid(-kept)
+    want = s * (1 + kept * rest)
+    for out in (a.value, y):
+        (dx,) = torch.autograd.grad(out, x, torch.ones_like(out), retain_graph=True)
+        # the sigmoid and what is left of 1 are each off by 2^-20 of themselves; 16-bit results take what is below -43
+        # as -43, where |silu'| < 42 e^-43 < 1e-17
+        bound = 2.01 * half_step(dtype) * want.abs() + 2.0 ** -20 * s * (1 + kept.abs() * rest) + 1e-17
+        assert ((dx.double().cpu() - want).abs() <= bound + torch.finfo(dtype).smallest_normal).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_gradients_against_differences(device):
     """Where x is on the grid of its blocks, x^ = x and gradients are those of the product: central differences of
     a bilinear form have no error but rounding (64 bits on the CPU, whole numbers on the GPU)."""

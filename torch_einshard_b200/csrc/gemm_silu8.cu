@@ -172,11 +172,11 @@ struct Silu8GradEpilogue {
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const uint32_t w = code[8 * sub + i / 2];
-        float x1 = code8_at(w, (2 * i) & 3) * scale, x2 = code8_at(w, (2 * i + 1) & 3) * scale, s1, s2;
-        sigmoid_pair(x1, x2, s1, s2);
+        float x1 = code8_at(w, (2 * i) & 3) * scale, x2 = code8_at(w, (2 * i + 1) & 3) * scale, s1, s2, e1, e2;
+        sigmoid_pair(x1, x2, s1, s2, e1, e2);
         aw[i] = floats_to_word<T>(x1 * s1, x2 * s2);
-        dh[i] = floats_to_word<T>(__uint_as_float(r[2 * i]) * silu_slope(x1, s1),
-                                  __uint_as_float(r[2 * i + 1]) * silu_slope(x2, s2));
+        dh[i] = floats_to_word<T>(__uint_as_float(r[2 * i]) * silu_slope(x1, s1, e1),
+                                  __uint_as_float(r[2 * i + 1]) * silu_slope(x2, s2, e2));
       }
       T* out_row = out + at * kept.pitch + col;
       T* act_row = act + at * kept.pitch + col;

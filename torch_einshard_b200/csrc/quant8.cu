@@ -56,19 +56,15 @@ __device__ __forceinline__ float value_of(float code, float scale) {
 template <typename T, int kMode>
 __device__ __forceinline__ void restored2(float& x1, float& x2, float g1, float g2) {
   if (kMode == kRestoreValue) return;
-  float s1, s2;
   if constexpr (sizeof(T) == 4) {
-    s1 = 1.0f / (1.0f + expf(-x1));
-    s2 = 1.0f / (1.0f + expf(-x2));
+    const float s1 = 1.0f / (1.0f + expf(-x1)), s2 = 1.0f / (1.0f + expf(-x2));  // 1 from x = 17 on
+    x1 = kMode == kRestoreSilu ? x1 * s1 : g1 * (s1 * fmaf(x1, 1.0f - s1, 1.0f));
+    x2 = kMode == kRestoreSilu ? x2 * s2 : g2 * (s2 * fmaf(x2, 1.0f - s2, 1.0f));
   } else {
-    sigmoid_pair(x1, x2, s1, s2);
-  }
-  if (kMode == kRestoreSilu) {
-    x1 *= s1;
-    x2 *= s2;
-  } else {
-    x1 = g1 * silu_slope(x1, s1);
-    x2 = g2 * silu_slope(x2, s2);
+    float s1, s2, e1, e2;
+    sigmoid_pair(x1, x2, s1, s2, e1, e2);
+    x1 = kMode == kRestoreSilu ? x1 * s1 : g1 * silu_slope(x1, s1, e1);
+    x2 = kMode == kRestoreSilu ? x2 * s2 : g2 * silu_slope(x2, s2, e2);
   }
 }
 

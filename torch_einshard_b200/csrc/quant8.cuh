@@ -82,15 +82,20 @@ __device__ __forceinline__ float exp2_approx(float x) {
 // Sigmoids of two values with one reciprocal, s1 = e2' / (e1' e2') with
 // e' = 1 + e^-x.  Below -43, where silu is under 10^-17, x is taken as -43: the
 // product of the two stays in range.  (A NaN makes both NaN: for what codes stand
-// for, where NaN blocks are NaN whole.)  For results of 16 bits.
-__device__ __forceinline__ void sigmoid_pair(float& x1, float& x2, float& s1, float& s2) {
+// for, where NaN blocks are NaN whole.)  e1, e2: e^-x.  For results of 16 bits.
+__device__ __forceinline__ void sigmoid_pair(float& x1, float& x2, float& s1, float& s2, float& e1, float& e2) {
   x1 = max_nan(x1, -43.0f);
   x2 = max_nan(x2, -43.0f);
-  const float e1 = 1.0f + exp2_approx(x1 * -1.4426950408889634f);
-  const float e2 = 1.0f + exp2_approx(x2 * -1.4426950408889634f);
-  const float r = __fdividef(1.0f, e1 * e2);
-  s1 = r * e2;
-  s2 = r * e1;
+  e1 = exp2_approx(x1 * -1.4426950408889634f);
+  e2 = exp2_approx(x2 * -1.4426950408889634f);
+  const float d1 = 1.0f + e1, d2 = 1.0f + e2;
+  const float r = __fdividef(1.0f, d1 * d2);
+  s1 = r * d2;
+  s2 = r * d1;
+}
+__device__ __forceinline__ void sigmoid_pair(float& x1, float& x2, float& s1, float& s2) {
+  float e1, e2;
+  sigmoid_pair(x1, x2, s1, s2, e1, e2);
 }
 
 // The same of values that may be NaN each by itself.
@@ -103,6 +108,7 @@ __device__ __forceinline__ void sigmoid_apart(float& x1, float& x2, float& s1, f
   if (bad2) x2 = __uint_as_float(0x7fc00000u);
 }
 
-__device__ __forceinline__ float silu_slope(float x, float s) { return s * fmaf(x, 1.0f - s, 1.0f); }
+// silu' = s (1 + x (1 - s)) with 1 - s = e^-x s: a difference would leave a rounding of s, which a large x multiplies.
+__device__ __forceinline__ float silu_slope(float x, float s, float e) { return s * fmaf(x * e, s, 1.0f); }
 
 }  // namespace es
