@@ -263,6 +263,25 @@ def test_slope_of_large_pre_activations(device, dtype, odd):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("width", [40, 64])
+def test_pre_activations_of_the_largest_value(device, width):
+    """bf16's largest value is kept as 64 steps of 2^122, which is past 32 bits: it reads back as the largest 32-bit value,
+    where silu' is 1 (and 0 on the other side)."""
+    top = torch.finfo(torch.bfloat16).max
+    x = torch.zeros(2, 3, width, dtype=torch.bfloat16, device=device)
+    x[0, 0, 1], x[0, 1, 2], x[1, 2, 5] = top, -top, top / 2
+    x.requires_grad_(True)
+    w = torch.eye(width, dtype=torch.bfloat16, device=device)
+    a = es.einshard("b s c, h c -> b s h", es.checkpoint8(x), w, activation="silu")
+    y = es.einshard("b s h, c h -> b s c", a, w)
+    for out in (a.value, y):  # through both forms of the gradient
+        (dx,) = torch.autograd.grad(out, x, torch.ones_like(out), retain_graph=True)
+        want = torch.full(x.shape, 0.5, device=device)
+        want[0, 0, 1], want[0, 1, 2], want[1, 2, 5] = 1, 0, 1
+        assert ((dx.float() - want).abs() <= half_step(x.dtype)).all()
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_gradients_against_differences(device):
     """Where x is on the grid of its blocks, x^ = x and gradients are those of the product: central differences of
     a bilinear form have no error but rounding (64 bits on the CPU, whole numbers on the GPU)."""

@@ -167,7 +167,7 @@ struct Silu8GradEpilogue {
       tmem_ld32(et.tmem + sub * 32, r);
       tmem_ld_wait();
       if (row >= s.M) continue;
-      const float scale = scale8_of(byte[sub]);
+      const float scale = finite_scale8_of(byte[sub]);
       uint32_t dh[16], aw[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) {

@@ -33,6 +33,13 @@ __device__ __forceinline__ float scale8_of(int byte) {
   return byte == kQuantNan ? __uint_as_float(0x7fc00000u) : __uint_as_float(static_cast<uint32_t>(byte) << 23);
 }
 
+// The same where nothing clamps what codes stand for: 64 steps of 2^122, the largest there are, would be past 32 bits,
+// and are the largest 32-bit value with a step that is one rounding smaller.
+constexpr int kTopStep = 122 + 127;
+__device__ __forceinline__ float finite_scale8_of(int byte) {
+  return byte == kTopStep ? __uint_as_float((static_cast<uint32_t>(byte) << 23) - 1u) : scale8_of(byte);
+}
+
 // The low bytes of four words.
 __device__ __forceinline__ uint32_t bytes_of(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
